@@ -443,6 +443,58 @@ TVB_API int tvb_addmm(int device, const void* a, int dtype, int64_t a_s0, int64_
               const void* bias, int bias_dtype, const void* residual, int residual_dtype, int64_t residual_ld, void* out,
               int out_dtype, int64_t m, int64_t n, int64_t k, int variant);
 
+/* ---- a fused Linear layer, forward and backward (no counterpart in the reference, which dispatches the product, the bias, the
+ *      activation and the residual addition one by one: crates/pyvk/csrc/linalg.cpp:227-321 and its elementwise kernels) ----
+ * y[m, n] = act(x[m, k] @ w[n, k]^T + bias[n]) + residual[m, n]
+ * float32 sums, one rounding to `dtype` (TVB_F32, TVB_F16 or TVB_BF16, of every operand and output). Rows of x, w and the
+ * residual begin x_sm (>= k), w_sn (>= k) and residual_sm (>= n) elements apart, their columns are contiguous; bias and
+ * residual may be NULL; y and preact are contiguous [m, n]. preact, unless NULL, receives x w^T + bias rounded to dtype: what
+ * tvb_linear_backward needs of a forward pass with an activation. y may be the residual itself (residual_sm == n); no other
+ * output may overlap an operand. 16-bit products run on the tensor cores whatever their sizes; operands whose rows do not
+ * begin on 16 bytes are first copied into the workspace (tvb_linear_workspace_bytes of them; 0 for aligned ones), which the
+ * caller owns, 256-byte aligned, and which is free again when the queued work has run. float32 runs on the CUDA cores. */
+enum TvbActivation {
+  TVB_ACT_NONE = 0,
+  TVB_ACT_RELU = 1,
+  TVB_ACT_GELU = 2,      /* z Phi(z), by erf */
+  TVB_ACT_GELU_TANH = 3, /* 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+  TVB_ACT_SILU = 4       /* z / (1 + exp(-z)) */
+};
+TVB_API uint64_t tvb_linear_workspace_bytes(int dtype, const void* x, int64_t x_sm, const void* w, int64_t w_sn, int64_t m, int64_t n,
+                                            int64_t k);
+TVB_API int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, const void* w, int64_t w_sn, const void* bias, int activation,
+                       const void* residual, int64_t residual_sm, void* y, void* preact, int64_t m, int64_t n, int64_t k,
+                       void* workspace, uint64_t workspace_bytes);
+
+/* The gradients of the layer above, given dy = dL/dy (rows dy_sm >= n apart) and the forward pass's preact (contiguous
+ * [m, n]; may be NULL without an activation):
+ *   dz = dy * act'(preact)   dx[m, k] = dz @ w   dw[n, k] = dz^T @ x   db[n] = sum of dz over the rows
+ * (the residual's gradient is dy itself). dx, dw and db are contiguous, of `dtype`, and any of them may be NULL. relu's
+ * derivative at 0 is 0. dz is rounded to dtype once on its way into the two products; db sums the unrounded values in
+ * float32, in a fixed order. Workspace as above; `want`: the TVB_WANT_* of the outputs that are not NULL. */
+enum TvbWant { TVB_WANT_DX = 1, TVB_WANT_DW = 2, TVB_WANT_DB = 4 };
+TVB_API uint64_t tvb_linear_backward_workspace_bytes(int dtype, const void* dy, int64_t dy_sm, const void* x, int64_t x_sm, const void* w,
+                                                     int64_t w_sn, int activation, int want, int64_t m, int64_t n, int64_t k);
+TVB_API int tvb_linear_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* preact, const void* x, int64_t x_sm,
+                                const void* w, int64_t w_sn, int activation, void* dx, void* dw, void* db, int64_t m, int64_t n,
+                                int64_t k, void* workspace, uint64_t workspace_bytes);
+
+/* ---- layer norm over the last dimension: aten::native_layer_norm and its backward (what a model has between its Linears) ----
+ * y = (x - mean) * rstd * weight + bias per row of d values; mean and rstd = 1 / sqrt(var + eps) of every row in float32 (var:
+ * the mean of the squared deviations). Rows of x begin x_sm (>= d) elements apart; y is contiguous. weight and bias are of x's
+ * dtype or float32 (param_dtype), each may be NULL (1 and 0); mean and rstd may be NULL. With rows == 0 or d == 0 nothing is
+ * written. No output may overlap an operand. */
+TVB_API int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm, const void* weight, const void* bias, int param_dtype,
+                           float eps, void* y, float* mean, float* rstd, int64_t rows, int64_t d);
+/* With h = (x - mean) * rstd and u = dy * weight: dx = rstd * (u - <u> - h <u h>) (<.>: the mean over the row), dweight = sum
+ * over the rows of dy h, dbias = sum of dy. Any of the three may be NULL; dweight and dbias are of param_dtype. The sums over
+ * the rows are float32, in a fixed order (partial sums in the caller's workspace, 16-byte aligned; needed when dweight or
+ * dbias is wanted). */
+TVB_API uint64_t tvb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d);
+TVB_API int tvb_layer_norm_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* x, int64_t x_sm, const float* mean,
+                                    const float* rstd, const void* weight, int param_dtype, void* dx, void* dweight, void* dbias,
+                                    int64_t rows, int64_t d, void* workspace, uint64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,137 @@
+// tvb_linear and tvb_linear_backward: argument checks and the choice of kernels.
+#include "../core/common.h"
+#include "launch.h"
+#include "linear.h"
+
+namespace tvb {
+namespace {
+
+bool is_float(int dt) { return dt == TVB_F32 || dt == TVB_F16 || dt == TVB_BF16; }
+
+int check_linear(const std::string& fn, int dtype, int activation, int64_t m, int64_t n, int64_t k) {
+  TVB_REQUIRE(is_float(dtype), fn + ": float32, float16 or bfloat16 only");
+  TVB_REQUIRE(activation >= TVB_ACT_NONE && activation <= TVB_ACT_SILU, fn + ": unknown activation");
+  TVB_REQUIRE(m >= 0 && n >= 0 && k >= 0, fn + ": negative size");
+  TVB_REQUIRE(m < (int64_t(1) << 31) && n < (int64_t(1) << 31) && k < (int64_t(1) << 31), fn + ": a size beyond 2^31 - 1");
+  return 0;
+}
+
+// Bytes from the first element of a matrix to behind its last.
+int64_t span(int64_t rows, int64_t cols, int64_t ld, int64_t es) { return rows == 0 || cols == 0 ? 0 : ((rows - 1) * ld + cols) * es; }
+
+}  // namespace
+}  // namespace tvb
+
+using namespace tvb;
+
+extern "C" uint64_t tvb_linear_workspace_bytes(int dtype, const void* x, int64_t x_sm, const void* w, int64_t w_sn, int64_t m, int64_t n,
+                                               int64_t k) {
+  return 0;
+}
+
+extern "C" int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, const void* w, int64_t w_sn, const void* bias,
+                          int activation, const void* residual, int64_t residual_sm, void* y, void* preact, int64_t m, int64_t n,
+                          int64_t k, void* workspace, uint64_t workspace_bytes) {
+  if (check_linear("tvb_linear", dtype, activation, m, n, k) != 0) return -1;
+  TVB_REQUIRE((m <= 1 || x_sm >= k) && (n <= 1 || w_sn >= k), "tvb_linear: rows of x and w must be at least k apart");
+  TVB_REQUIRE(residual == nullptr || m <= 1 || residual_sm >= n, "tvb_linear: rows of the residual must be at least n apart");
+  if (m == 0 || n == 0) return 0;
+  TVB_REQUIRE(y != nullptr && (k == 0 || (x != nullptr && w != nullptr)), "tvb_linear: NULL pointer");
+  if (m <= 1) x_sm = k, residual_sm = n;
+  if (n <= 1) w_sn = k;
+  const int64_t es = dtype_size(dtype), y_bytes = m * n * es;
+  const uint64_t need = tvb_linear_workspace_bytes(dtype, x, x_sm, w, w_sn, m, n, k);
+  TVB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0),
+              "tvb_linear: the workspace is too small or not 256-byte aligned");
+  const void* outs[3] = {y, preact, need != 0 ? workspace : nullptr};
+  const int64_t out_bytes[3] = {y_bytes, y_bytes, static_cast<int64_t>(need)};
+  for (int i = 0; i < 3; i++) {
+    const bool in_place = i == 0 && residual == y && residual_sm == n;  // every element is read by the thread that writes it
+    TVB_REQUIRE(!overlap(outs[i], out_bytes[i], x, span(m, k, x_sm, es)) && !overlap(outs[i], out_bytes[i], w, span(n, k, w_sn, es)) &&
+                    !overlap(outs[i], out_bytes[i], bias, n * es) &&
+                    (in_place || !overlap(outs[i], out_bytes[i], residual, span(m, n, residual_sm, es))),
+                "tvb_linear: an output or the workspace overlaps an operand (only y may be the residual itself)");
+    for (int j = 0; j < i; j++) TVB_REQUIRE(!overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]), "tvb_linear: two outputs overlap");
+  }
+  cudaStream_t stream;
+  if (enter(device, &stream) != 0) return -1;
+  LinearProduct p{};
+  p.p = w; p.p_si = w_sn; p.p_sr = 1;
+  p.q = x; p.q_sj = x_sm; p.q_sr = 1;
+  p.bias = bias; p.residual = residual; p.residual_ld = residual_sm;
+  p.out = y; p.preact = preact;
+  p.I = n; p.J = m; p.R = k;
+  p.dtype = dtype; p.activation = activation;
+  return linear_simt(stream, p);
+}
+
+extern "C" uint64_t tvb_linear_backward_workspace_bytes(int dtype, const void* dy, int64_t dy_sm, const void* x, int64_t x_sm, const void* w,
+                                                        int64_t w_sn, int activation, int want, int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || activation == TVB_ACT_NONE || (want & (TVB_WANT_DX | TVB_WANT_DW)) == 0) return 0;
+  return static_cast<uint64_t>(m) * static_cast<uint64_t>(n) * dtype_size(dtype);
+}
+
+extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* preact, const void* x, int64_t x_sm,
+                                   const void* w, int64_t w_sn, int activation, void* dx, void* dw, void* db, int64_t m, int64_t n,
+                                   int64_t k, void* workspace, uint64_t workspace_bytes) {
+  if (check_linear("tvb_linear_backward", dtype, activation, m, n, k) != 0) return -1;
+  TVB_REQUIRE((m <= 1 || (x_sm >= k && dy_sm >= n)) && (n <= 1 || w_sn >= k),
+              "tvb_linear_backward: rows of x and w must be at least k apart, those of dy at least n");
+  TVB_REQUIRE(activation == TVB_ACT_NONE || m == 0 || n == 0 || preact != nullptr,
+              "tvb_linear_backward: an activation's gradient needs the values before it");
+  if (m <= 1) x_sm = k, dy_sm = n;
+  if (n <= 1) w_sn = k;
+  const bool want_dx = dx != nullptr && m > 0 && k > 0, want_dw = dw != nullptr && n > 0 && k > 0, want_db = db != nullptr && n > 0;
+  if (!want_dx && !want_dw && !want_db) return 0;
+  TVB_REQUIRE((m == 0 || n == 0 || dy != nullptr) && (!want_dw || m == 0 || x != nullptr) && (!want_dx || n == 0 || w != nullptr),
+              "tvb_linear_backward: NULL pointer");
+  const int64_t es = dtype_size(dtype);
+  const int want = (want_dx ? TVB_WANT_DX : 0) | (want_dw ? TVB_WANT_DW : 0) | (want_db ? TVB_WANT_DB : 0);
+  const uint64_t need = tvb_linear_backward_workspace_bytes(dtype, dy, dy_sm, x, x_sm, w, w_sn, activation, want, m, n, k);
+  TVB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0),
+              "tvb_linear_backward: the workspace is too small or not 256-byte aligned");
+  const void* outs[4] = {want_dx ? dx : nullptr, want_dw ? dw : nullptr, want_db ? db : nullptr, need != 0 ? workspace : nullptr};
+  const int64_t out_bytes[4] = {m * k * es, n * k * es, n * es, static_cast<int64_t>(need)};
+  for (int i = 0; i < 4; i++) {
+    TVB_REQUIRE(!overlap(outs[i], out_bytes[i], dy, span(m, n, dy_sm, es)) && !overlap(outs[i], out_bytes[i], preact, m * n * es) &&
+                    !overlap(outs[i], out_bytes[i], x, span(m, k, x_sm, es)) && !overlap(outs[i], out_bytes[i], w, span(n, k, w_sn, es)),
+                "tvb_linear_backward: an output or the workspace overlaps an operand");
+    for (int j = 0; j < i; j++)
+      TVB_REQUIRE(!overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]), "tvb_linear_backward: two outputs overlap");
+  }
+  cudaStream_t stream;
+  if (enter(device, &stream) != 0) return -1;
+  const void* dz = dy;
+  int64_t dz_ld = dy_sm;
+  const bool make_dz = need != 0;
+  if (make_dz) {
+    dz = workspace;
+    dz_ld = n;
+  }
+  if (make_dz || want_db) {
+    LinearDz d{};
+    d.dy = dy; d.z = preact; d.dz = make_dz ? workspace : nullptr; d.db = want_db ? db : nullptr;
+    d.dy_ld = dy_sm; d.dz_ld = dz_ld; d.m = m; d.n = n;
+    d.dtype = dtype; d.activation = activation;
+    if (linear_dz(device, stream, d) != 0) return -1;
+  }
+  if (want_dx) {
+    LinearProduct p{};
+    p.p = w; p.p_si = 1; p.p_sr = w_sn;
+    p.q = dz; p.q_sj = dz_ld; p.q_sr = 1;
+    p.out = dx;
+    p.I = k; p.J = m; p.R = n;
+    p.dtype = dtype;
+    if (linear_simt(stream, p) != 0) return -1;
+  }
+  if (want_dw) {
+    LinearProduct p{};
+    p.p = x; p.p_si = 1; p.p_sr = x_sm;
+    p.q = dz; p.q_sj = 1; p.q_sr = dz_ld;
+    p.out = dw;
+    p.I = k; p.J = n; p.R = m;
+    p.dtype = dtype;
+    if (linear_simt(stream, p) != 0) return -1;
+  }
+  return 0;
+}
