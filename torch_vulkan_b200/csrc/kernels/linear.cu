@@ -19,6 +19,42 @@ int check_linear(const std::string& fn, int dtype, int activation, int64_t m, in
 // Bytes from the first element of a matrix to behind its last.
 int64_t span(int64_t rows, int64_t cols, int64_t ld, int64_t es) { return rows == 0 || cols == 0 ? 0 : ((rows - 1) * ld + cols) * es; }
 
+int64_t round8(int64_t n) { return (n + 7) & ~int64_t(7); }
+
+// Whether TMA can read a 16-bit matrix where it is: it begins on 16 bytes, and so does every row.
+bool readable(const void* p, int64_t rows, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (rows <= 1 || ld % 8 == 0); }
+
+// Bytes of the copy that an unreadable 16-bit operand takes in the workspace, each begun on 256 bytes.
+uint64_t copy_bytes(int dtype, const void* p, int64_t rows, int64_t cols, int64_t ld) {
+  if (dtype == TVB_F32 || rows <= 0 || cols <= 0 || readable(p, rows, ld)) return 0;
+  return (static_cast<uint64_t>(rows) * static_cast<uint64_t>(round8(cols)) * 2 + 255) & ~uint64_t(255);
+}
+
+// The operand where TMA can read it: in place, or copied to the workspace at *at (which moves on).
+int make_readable(int device, cudaStream_t stream, int dtype, const void** p, int64_t rows, int64_t cols, int64_t* ld, uint8_t** at) {
+  const uint64_t bytes = copy_bytes(dtype, *p, rows, cols, *ld);
+  if (bytes != 0) {
+    if (linear_pad(device, stream, *at, round8(cols), *p, *ld, rows, cols) != 0) return -1;
+    *p = *at;
+    *ld = round8(cols);
+    *at += bytes;
+  } else if (rows <= 1) {
+    *ld = round8(cols);  // (one row: the distance to the next is never used, but has to be a legal one)
+  }
+  return 0;
+}
+
+int run_product(int device, cudaStream_t stream, const LinearProduct& p) {
+  return p.dtype == TVB_F32 ? linear_simt(stream, p) : linear_split(device, stream, p);
+}
+
+// dz needs a matrix of its own: there is an activation to differentiate, or TMA cannot read dy.
+uint64_t dz_bytes(int dtype, const void* dy, int64_t dy_sm, int activation, int want, int64_t m, int64_t n) {
+  if (m <= 0 || n <= 0 || (want & (TVB_WANT_DX | TVB_WANT_DW)) == 0) return 0;
+  if (activation == TVB_ACT_NONE && (dtype == TVB_F32 || readable(dy, m, dy_sm))) return 0;
+  return (static_cast<uint64_t>(m) * static_cast<uint64_t>(round8(n)) * dtype_size(dtype) + 255) & ~uint64_t(255);
+}
+
 }  // namespace
 }  // namespace tvb
 
@@ -26,7 +62,7 @@ using namespace tvb;
 
 extern "C" uint64_t tvb_linear_workspace_bytes(int dtype, const void* x, int64_t x_sm, const void* w, int64_t w_sn, int64_t m, int64_t n,
                                                int64_t k) {
-  return 0;
+  return copy_bytes(dtype, x, m, k, x_sm) + copy_bytes(dtype, w, n, k, w_sn);
 }
 
 extern "C" int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, const void* w, int64_t w_sn, const void* bias,
@@ -55,6 +91,9 @@ extern "C" int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, co
   }
   cudaStream_t stream;
   if (enter(device, &stream) != 0) return -1;
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  if (make_readable(device, stream, dtype, &x, m, k, &x_sm, &at) != 0 || make_readable(device, stream, dtype, &w, n, k, &w_sn, &at) != 0)
+    return -1;
   LinearProduct p{};
   p.p = w; p.p_si = w_sn; p.p_sr = 1;
   p.q = x; p.q_sj = x_sm; p.q_sr = 1;
@@ -62,13 +101,13 @@ extern "C" int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, co
   p.out = y; p.preact = preact;
   p.I = n; p.J = m; p.R = k;
   p.dtype = dtype; p.activation = activation;
-  return linear_simt(stream, p);
+  return run_product(device, stream, p);
 }
 
 extern "C" uint64_t tvb_linear_backward_workspace_bytes(int dtype, const void* dy, int64_t dy_sm, const void* x, int64_t x_sm, const void* w,
                                                         int64_t w_sn, int activation, int want, int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || activation == TVB_ACT_NONE || (want & (TVB_WANT_DX | TVB_WANT_DW)) == 0) return 0;
-  return static_cast<uint64_t>(m) * static_cast<uint64_t>(n) * dtype_size(dtype);
+  return dz_bytes(dtype, dy, dy_sm, activation, want, m, n) + ((want & TVB_WANT_DW) != 0 ? copy_bytes(dtype, x, m, k, x_sm) : 0) +
+         ((want & TVB_WANT_DX) != 0 ? copy_bytes(dtype, w, n, k, w_sn) : 0);
 }
 
 extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* preact, const void* x, int64_t x_sm,
@@ -102,36 +141,40 @@ extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_
   cudaStream_t stream;
   if (enter(device, &stream) != 0) return -1;
   const void* dz = dy;
-  int64_t dz_ld = dy_sm;
-  const bool make_dz = need != 0;
-  if (make_dz) {
-    dz = workspace;
-    dz_ld = n;
+  int64_t dz_ld = m > 1 ? dy_sm : round8(n);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  const uint64_t own_dz = dz_bytes(dtype, dy, dy_sm, activation, want, m, n);
+  if (own_dz != 0) {
+    dz = at;
+    dz_ld = round8(n);
+    at += own_dz;
   }
-  if (make_dz || want_db) {
+  if (own_dz != 0 || want_db) {
     LinearDz d{};
-    d.dy = dy; d.z = preact; d.dz = make_dz ? workspace : nullptr; d.db = want_db ? db : nullptr;
+    d.dy = dy; d.z = preact; d.dz = own_dz != 0 ? workspace : nullptr; d.db = want_db ? db : nullptr;
     d.dy_ld = dy_sm; d.dz_ld = dz_ld; d.m = m; d.n = n;
     d.dtype = dtype; d.activation = activation;
     if (linear_dz(device, stream, d) != 0) return -1;
   }
+  if (want_dw && make_readable(device, stream, dtype, &x, m, k, &x_sm, &at) != 0) return -1;
+  if (want_dx && make_readable(device, stream, dtype, &w, n, k, &w_sn, &at) != 0) return -1;
   if (want_dx) {
     LinearProduct p{};
-    p.p = w; p.p_si = 1; p.p_sr = w_sn;
+    p.p = w; p.p_si = 1; p.p_sr = w_sn; p.p_mn = true;
     p.q = dz; p.q_sj = dz_ld; p.q_sr = 1;
     p.out = dx;
     p.I = k; p.J = m; p.R = n;
     p.dtype = dtype;
-    if (linear_simt(stream, p) != 0) return -1;
+    if (run_product(device, stream, p) != 0) return -1;
   }
   if (want_dw) {
     LinearProduct p{};
-    p.p = x; p.p_si = 1; p.p_sr = x_sm;
-    p.q = dz; p.q_sj = 1; p.q_sr = dz_ld;
+    p.p = x; p.p_si = 1; p.p_sr = x_sm; p.p_mn = true;
+    p.q = dz; p.q_sj = 1; p.q_sr = dz_ld; p.q_mn = true;
     p.out = dw;
     p.I = k; p.J = n; p.R = m;
     p.dtype = dtype;
-    if (linear_simt(stream, p) != 0) return -1;
+    if (run_product(device, stream, p) != 0) return -1;
   }
   return 0;
 }

@@ -1,6 +1,6 @@
 // The products behind tvb_linear and tvb_linear_backward, as one form:
 //   out[j, i] = act(sum_r P(i, r) Q(j, r) + bias[i]) + residual[j, i]        i < I, j < J, r < R
-// with P(i, r) at p[i * p_si + r * p_sr] and Q(j, r) at q[j * q_sj + r * q_sr], one of the two strides of each being 1.
+// with P(i, r) at p[i * p_si + r * p_sr] and Q(j, r) at q[j * q_sj + r * q_sr], one of the two strides of each being 1 (p_mn, q_mn: which).
 //   forward  y = act(x w^T + b) + res   P = w  (i: output feature, r: input feature)  Q = x   (j: row)
 //   dx = dz w                           P = w^T (i: input feature, r: output feature) Q = dz  (j: row)
 //   dw = dz^T x                         P = x^T (i: input feature, r: row)            Q = dz^T (j: output feature)
@@ -17,6 +17,7 @@ struct LinearProduct {
   const void* p;
   const void* q;
   int64_t p_si, p_sr, q_sj, q_sr;
+  bool p_mn, q_mn;       // the operand is contiguous in i / j (else in r)
   const void* bias;      // I values, or NULL
   const void* residual;  // [J, I], row stride residual_ld, or NULL
   void* out;             // [J, I] contiguous
@@ -27,7 +28,12 @@ struct LinearProduct {
   int activation;        // TvbActivation
 };
 
-int linear_simt(cudaStream_t stream, const LinearProduct& p);
+int linear_simt(cudaStream_t stream, const LinearProduct& p);  // float32
+// float16 and bfloat16, on the tensor cores; every operand begins on 16 bytes and its rows are a multiple of 16 bytes apart.
+int linear_split(int device, cudaStream_t stream, const LinearProduct& p);
+
+// Copies a 16-bit [rows, cols] matrix to rows dst_ld (a multiple of 8) apart.
+int linear_pad(int device, cudaStream_t stream, void* dst, int64_t dst_ld, const void* src, int64_t src_ld, int64_t rows, int64_t cols);
 
 // dz = dy * act'(z) (row stride dz_ld) and db = its sums over the rows; dz or db may be NULL. activation TVB_ACT_NONE: dz = dy.
 struct LinearDz {

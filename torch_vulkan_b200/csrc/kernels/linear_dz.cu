@@ -54,7 +54,30 @@ __global__ void __launch_bounds__(kThreads) linear_dz_kernel(const LinearDz p) {
   cluster.sync();
 }
 
+// Rows that begin anywhere brought to rows that begin on 16 bytes: eight values per thread.
+__global__ void __launch_bounds__(kThreads) linear_pad_kernel(uint16_t* dst, int64_t dst_ld, const uint16_t* src, int64_t src_ld, int64_t rows,
+                                                               int64_t cols) {
+  const int64_t per_row = dst_ld / 8, total = rows * per_row;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; e < total; e += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t r = e / per_row, c = (e - r * per_row) * 8;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t lo = c + 2 * j < cols ? src[r * src_ld + c + 2 * j] : 0u, hi = c + 2 * j + 1 < cols ? src[r * src_ld + c + 2 * j + 1] : 0u;
+      w[j] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint4*>(dst + r * dst_ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 }  // namespace
+
+int linear_pad(int device, cudaStream_t stream, void* dst, int64_t dst_ld, const void* src, int64_t src_ld, int64_t rows, int64_t cols) {
+  const int64_t want = ceil_div(rows * (dst_ld / 8), kThreads), most = static_cast<int64_t>(sm_count(device)) * 16;
+  const int grid = static_cast<int>(std::min(want, most));
+  linear_pad_kernel<<<grid, kThreads, 0, stream>>>(static_cast<uint16_t*>(dst), dst_ld, static_cast<const uint16_t*>(src), src_ld, rows, cols);
+  return launched("linear_pad", dim3(grid), dim3(kThreads), 0, stream);
+}
 
 int linear_dz(int device, cudaStream_t stream, const LinearDz& p) {
   const int64_t strips = ceil_div(p.n, kStrip);

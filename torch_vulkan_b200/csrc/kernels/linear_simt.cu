@@ -1,4 +1,4 @@
-// The products of linear.h on the CUDA cores, for any strides: 64 x 64 tiles, float32 sums.
+// The products of linear.h in float32, on the CUDA cores, for any strides: 64 x 64 tiles, float32 sums.
 #include "../core/common.h"
 #include "linear.h"
 #include "linear_math.cuh"
@@ -9,7 +9,6 @@ namespace {
 
 constexpr int kTile = 64, kStep = 16;
 
-template <int DT>
 __global__ void __launch_bounds__(256) linear_simt_kernel(const LinearProduct p) {
   __shared__ float ps[kStep][kTile + 1], qs[kStep][kTile + 1];
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kTile, j0 = static_cast<int64_t>(blockIdx.y) * kTile;
@@ -20,10 +19,10 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinearProduct p)
     for (int u = 0; u < 4; u++) {
       // neighbouring threads read along whichever stride is 1
       const int e = threadIdx.x + 256 * u;
-      const int pi = p.p_sr == 1 ? e >> 4 : e & 63, pr = p.p_sr == 1 ? e & 15 : e >> 6;
-      const int qj = p.q_sr == 1 ? e >> 4 : e & 63, qr = p.q_sr == 1 ? e & 15 : e >> 6;
-      ps[pr][pi] = i0 + pi < p.I && r0 + pr < p.R ? load_float<DT>(p.p, (i0 + pi) * p.p_si + (r0 + pr) * p.p_sr) : 0.0f;
-      qs[qr][qj] = j0 + qj < p.J && r0 + qr < p.R ? load_float<DT>(p.q, (j0 + qj) * p.q_sj + (r0 + qr) * p.q_sr) : 0.0f;
+      const int pi = !p.p_mn ? e >> 4 : e & 63, pr = !p.p_mn ? e & 15 : e >> 6;
+      const int qj = !p.q_mn ? e >> 4 : e & 63, qr = !p.q_mn ? e & 15 : e >> 6;
+      ps[pr][pi] = i0 + pi < p.I && r0 + pr < p.R ? load_float<TVB_F32>(p.p, (i0 + pi) * p.p_si + (r0 + pr) * p.p_sr) : 0.0f;
+      qs[qr][qj] = j0 + qj < p.J && r0 + qr < p.R ? load_float<TVB_F32>(p.q, (j0 + qj) * p.q_sj + (r0 + qr) * p.q_sr) : 0.0f;
     }
     __syncthreads();
 #pragma unroll
@@ -50,11 +49,11 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinearProduct p)
       const int64_t i = i0 + tx + 16 * b;
       if (i >= p.I) continue;
       float z = acc[a][b];
-      if (p.bias != nullptr) z += load_float<DT>(p.bias, i);
-      if (p.preact != nullptr) store_float<DT>(p.preact, j * p.I + i, z);
-      float y = act_value<DT != TVB_F32>(z, p.activation);
-      if (p.residual != nullptr) y += load_float<DT>(p.residual, j * p.residual_ld + i);
-      store_float<DT>(p.out, j * p.I + i, y);
+      if (p.bias != nullptr) z += load_float<TVB_F32>(p.bias, i);
+      if (p.preact != nullptr) store_float<TVB_F32>(p.preact, j * p.I + i, z);
+      float y = act_value<false>(z, p.activation);
+      if (p.residual != nullptr) y += load_float<TVB_F32>(p.residual, j * p.residual_ld + i);
+      store_float<TVB_F32>(p.out, j * p.I + i, y);
     }
   }
 }
@@ -65,9 +64,7 @@ int linear_simt(cudaStream_t stream, const LinearProduct& p) {
   const int64_t rows = ceil_div(p.J, kTile);
   if (rows > 65535) return fail("tvb_linear: too many rows for one launch of the CUDA-core kernel (4194240)");
   const dim3 grid(static_cast<unsigned>(ceil_div(p.I, kTile)), static_cast<unsigned>(rows));
-  if (p.dtype == TVB_F32) linear_simt_kernel<TVB_F32><<<grid, 256, 0, stream>>>(p);
-  else if (p.dtype == TVB_F16) linear_simt_kernel<TVB_F16><<<grid, 256, 0, stream>>>(p);
-  else linear_simt_kernel<TVB_BF16><<<grid, 256, 0, stream>>>(p);
+  linear_simt_kernel<<<grid, 256, 0, stream>>>(p);
   return launched("linear_simt", grid, dim3(256), 0, stream);
 }
 

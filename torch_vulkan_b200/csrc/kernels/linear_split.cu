@@ -1,0 +1,301 @@
+// The 16-bit products of linear.h on tcgen05 when the output is small: few rows (decoding, short prompts), or gradients with few
+// tiles. Bound by the bytes of P (the weights) or by latency, so what counts is that every SM streams.
+//
+// One CTA multiplies a tile of 128 values of i (the MMA's 128 rows) by TN values of j (its columns; TN the smallest of 16 ...
+// 256 that holds the rows), over a slice of r; a cluster of S CTAs shares a tile, each with 1 / S of r. S is what makes a
+// product of 32 tiles fill 148 SMs. The CTAs leave their float32 sums in their own shared memory, and each adds up, in rank order,
+// 1 / S of the tile's columns of all S through distributed shared memory: no scratch in global memory, no counters and no
+// atomics, so a launch repeats its results bit for bit and launches share nothing.
+//   warp 4, one lane: TMA (128-byte swizzle) into a ring of stages of 64 values of r
+//   warp 5, one lane: tcgen05.mma (M = 128, N = TN, K = 16; float32 sums in TMEM); the warp owns the TMEM
+//   warps 0-3: TMEM -> shared memory; then all warps: sums, bias, activation, residual, store
+// An operand may be contiguous along r (K-major) or along i / j (MN-major: the transposed reads of the backward pass).
+// Up to TN = 128 the ring is kept under half of an SM's shared memory: two CTAs per SM, so that one streams while the other is
+// in its prologue or epilogue.
+#include <cuda.h>
+
+#include "../core/common.h"
+#include "../core/tensormap.h"
+#include "launch.h"
+#include "linear.h"
+#include "linear_epilogue.cuh"
+#include "ptx_pair.cuh"
+
+namespace tvb {
+namespace {
+
+constexpr int kRows = 128, kStepR = 64, kThreads = 192, kProducer = 4, kMma = 5;
+
+template <int TN>
+struct SplitCfg {
+  static constexpr int kStageP = kRows * 128, kStageQ = TN * 128, kStage = kStageP + kStageQ;
+  static constexpr int kBudget = TN <= 128 ? 100 * 1024 : 200 * 1024;
+  static constexpr int kStages = kBudget / kStage < 8 ? kBudget / kStage : 8;
+  static constexpr int kCtasPerSm = TN <= 128 ? 2 : 1;
+  static constexpr int kTmemCols = TN < 32 ? 32 : TN;
+  static constexpr int kSmemBytes = kStages * kStage + 1024 + 256;
+  static_assert(kRows * TN * 4 <= kStages * kStage, "the sums do not fit the ring");
+};
+
+struct SplitParams {
+  const void* bias;
+  const void* residual;
+  void* out;
+  void* preact;
+  int64_t residual_ld;
+  int I, J, blocks, tiles_j, activation, vector_ok;
+  uint32_t idesc;
+  int* status;
+};
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four neighbouring outputs (i ... i + 3, row j).
+template <bool BF16>
+__device__ __forceinline__ void finish4(const SplitParams& p, int64_t j, int i, float4 s) {
+  float z[4] = {s.x, s.y, s.z, s.w}, y[4];
+  const int64_t o = j * p.I + i;
+  if (p.vector_ok) {  // (I a multiple of 4, every pointer and row on 8 bytes)
+    if (p.bias != nullptr) {
+      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.bias) + i);
+      const float2 b0 = unpack16<BF16>(b.x), b1 = unpack16<BF16>(b.y);
+      z[0] += b0.x; z[1] += b0.y; z[2] += b1.x; z[3] += b1.y;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = act_value<true>(z[e], p.activation);
+    if (p.residual != nullptr) {
+      const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + j * p.residual_ld + i);
+      const float2 r0 = unpack16<BF16>(r.x), r1 = unpack16<BF16>(r.y);
+      y[0] += r0.x; y[1] += r0.y; y[2] += r1.x; y[3] += r1.y;
+    }
+    if (p.preact != nullptr)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.preact) + o) = make_uint2(pack16<BF16>(z[0], z[1]), pack16<BF16>(z[2], z[3]));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = make_uint2(pack16<BF16>(y[0], y[1]), pack16<BF16>(y[2], y[3]));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (i + e >= p.I) break;
+    if (p.bias != nullptr) z[e] += load16<BF16>(p.bias, i + e);
+    y[e] = act_value<true>(z[e], p.activation);
+    if (p.residual != nullptr) y[e] += load16<BF16>(p.residual, j * p.residual_ld + i + e);
+    if (p.preact != nullptr) store16<BF16>(p.preact, o + e, z[e]);
+    store16<BF16>(p.out, o + e, y[e]);
+  }
+}
+
+template <int TN, bool P_MN, bool Q_MN, bool BF16>
+__global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
+    linear_split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const SplitParams p) {
+  using Cfg = SplitCfg<TN>;
+  static_assert(!Q_MN || TN >= 64, "an MN-major operand comes in columns of 64 values");
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - ptx::smem_u32(smem_raw));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + Cfg::kStages * Cfg::kStage);
+  const uint32_t full0 = ptx::smem_u32(bars), empty0 = full0 + 8 * Cfg::kStages, tfull = empty0 + 8 * Cfg::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * Cfg::kStages + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t parts;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(parts));
+  const uint32_t part = ptx::cluster_ctarank();
+  const int tile = static_cast<int>(blockIdx.x / parts);
+  const int i0 = tile / p.tiles_j * kRows, j0 = tile % p.tiles_j * TN;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(p.blocks) * part / parts);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(p.blocks) * (part + 1) / parts);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::kStages; s++) {
+      ptx::mbar_init(full0 + 8 * s, 1);
+      ptx::mbar_init(empty0 + 8 * s, 1);
+    }
+    ptx::mbar_init(tfull, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == kProducer && lane == 0) {
+    ptx::prefetch_tensormap(&map_p);
+    ptx::prefetch_tensormap(&map_q);
+  }
+  if (warp == kMma) ptx::tmem_alloc(ptx::smem_u32(tmem_slot), Cfg::kTmemCols);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+
+  if (warp == kProducer) {
+    if (lane == 0) {
+      bool ok = true;
+      int it = 0;
+      for (int kb = kb0; kb < kb1; kb++, it++) {
+        const int s = it % Cfg::kStages;
+        ok = ptx::mbar_wait(empty0 + 8 * s, static_cast<uint32_t>((it / Cfg::kStages) & 1) ^ 1u, abort_flag);
+        if (!ok) break;
+        const uint32_t dst = base + s * Cfg::kStage, bar = full0 + 8 * s;
+        ptx::mbar_expect_tx(bar, Cfg::kStage);
+        if (P_MN) {
+          for (int c = 0; c < kRows / 64; c++) ptx::tma_load_2d(dst + c * 8192, &map_p, i0 + c * 64, kb * kStepR, bar);
+        } else {
+          ptx::tma_load_2d(dst, &map_p, kb * kStepR, i0, bar);
+        }
+        if (Q_MN) {
+          for (int c = 0; c < TN / 64; c++)
+            ptx::tma_load_2d(dst + Cfg::kStageP + c * 8192, &map_q, j0 + c * 64, kb * kStepR, bar);
+        } else {
+          ptx::tma_load_2d(dst + Cfg::kStageP, &map_q, kb * kStepR, j0, bar);
+        }
+      }
+      // no copy may still be in flight when the ring is used for the sums or released
+      for (int j = it > Cfg::kStages ? it - Cfg::kStages : 0; j < it; j++) {
+        volatile int never = 0;
+        ptx::mbar_wait(full0 + 8 * (j % Cfg::kStages), static_cast<uint32_t>((j / Cfg::kStages) & 1), &never);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMma) {
+    if (lane == 0) {
+      bool ok = true;
+      int it = 0;
+      for (int kb = kb0; kb < kb1; kb++, it++) {
+        const int s = it % Cfg::kStages;
+        ok = ptx::mbar_wait(full0 + 8 * s, static_cast<uint32_t>((it / Cfg::kStages) & 1), abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t at = base + s * Cfg::kStage;
+        const uint64_t pd = P_MN ? ptx::tc_smem_desc_sw128_mn(at) : ptx::tc_smem_desc_sw128(at);
+        const uint64_t qd = Q_MN ? ptx::tc_smem_desc_sw128_mn(at + Cfg::kStageP) : ptx::tc_smem_desc_sw128(at + Cfg::kStageP);
+#pragma unroll
+        for (int j = 0; j < kStepR / 16; j++)
+          ptx::tc_mma<2>(tmem, pd + (P_MN ? 128 : 2) * j, qd + (Q_MN ? 128 : 2) * j, p.idesc, (it | j) != 0 ? 1u : 0u);
+        ptx::tc_commit(empty0 + 8 * s);
+      }
+      if (ok && it != 0) ptx::tc_commit(tfull);
+    }
+    __syncwarp();
+  } else {
+    const bool empty = kb1 == kb0;  // no values of r here: sums of nothing
+    const bool ok = empty || ptx::mbar_wait(tfull, 0, abort_flag);
+    ptx::tc_fence_after();
+    const uint32_t dst = base + (warp * 32 + lane) * 4;
+    if (ok) {
+#pragma unroll 1
+      for (int c = 0; c < TN; c += 16) {
+        uint32_t r[16];
+        if (!empty) {
+          ptx::tmem_ld_32x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, r);
+          ptx::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (c + e) * (kRows * 4)), "r"(empty ? 0u : r[e]) : "memory");
+      }
+    }
+    ptx::tc_fence_before();
+  }
+  ptx::cluster_sync();  // every CTA's sums are in its shared memory
+  if (warp == kMma) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, Cfg::kTmemCols);
+  }
+  if (*abort_flag == 0) {
+    const int c0 = TN * static_cast<int>(part) / static_cast<int>(parts), c1 = TN * (static_cast<int>(part) + 1) / static_cast<int>(parts);
+    for (int e = threadIdx.x; e < (c1 - c0) * 32; e += kThreads) {
+      const int j = c0 + (e >> 5), i = (e & 31) * 4;
+      if (j0 + j >= p.J || i0 + i >= p.I) continue;
+      const uint32_t at = base + j * (kRows * 4) + i * 4;
+      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+      for (uint32_t g = 0; g < parts; g++) {
+        const float4 v = ld_cluster_f4(ptx::mapa(at, g));
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+      finish4<BF16>(p, j0 + j, i0 + i, s);
+    }
+  } else if (threadIdx.x == 0) {
+    atomicExch(p.status, 2);
+  }
+  ptx::cluster_sync();  // no CTA's shared memory is released while another may read it
+}
+
+// A map over one operand: `inner` contiguous values, `outer` rows.
+int operand_map(CUtensorMap* map, const void* base, int dtype, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
+  const CUtensorMapDataType dt = dtype == TVB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return make_tensor_map_2d(map, base, dt, inner, outer, ld * 2, 64, box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int TN, bool P_MN, bool Q_MN, bool BF16>
+int split_run(int device, cudaStream_t stream, const LinearProduct& lp, int parts) {
+  using Cfg = SplitCfg<TN>;
+  auto kernel = linear_split_kernel<TN, P_MN, Q_MN, BF16>;
+  static bool configured[64] = {};
+  if (!configured[device & 63]) {
+    TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
+    configured[device & 63] = true;
+  }
+  CUtensorMap map_p, map_q;
+  if (lp.R > 0) {
+    if (operand_map(&map_p, lp.p, lp.dtype, P_MN ? lp.I : lp.R, P_MN ? lp.R : lp.I, P_MN ? lp.p_sr : lp.p_si, P_MN ? kStepR : kRows) != 0 ||
+        operand_map(&map_q, lp.q, lp.dtype, Q_MN ? lp.J : lp.R, Q_MN ? lp.R : lp.J, Q_MN ? lp.q_sr : lp.q_sj, Q_MN ? kStepR : TN) != 0)
+      return -1;
+  } else {
+    map_p = map_q = CUtensorMap{};  // (a product over nothing: no box is ever loaded)
+  }
+  SplitParams p{};
+  p.bias = lp.bias;
+  p.residual = lp.residual;
+  p.out = lp.out;
+  p.preact = lp.preact;
+  p.residual_ld = lp.residual_ld;
+  p.I = static_cast<int>(lp.I);
+  p.J = static_cast<int>(lp.J);
+  p.blocks = static_cast<int>(ceil_div(lp.R, kStepR));
+  p.tiles_j = static_cast<int>(ceil_div(lp.J, TN));
+  p.activation = lp.activation;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(lp.out) | reinterpret_cast<uintptr_t>(lp.preact) | reinterpret_cast<uintptr_t>(lp.bias) |
+                        reinterpret_cast<uintptr_t>(lp.residual);
+  p.vector_ok = (all & 7u) == 0 && lp.I % 4 == 0 && (lp.residual == nullptr || lp.residual_ld % 4 == 0);
+  const uint32_t fmt = BF16 ? 1 : 0;
+  p.idesc = ptx::tc_instr_desc(1, fmt, fmt, kRows, TN) | (P_MN ? ptx::kTcAMajorMN : 0u) | (Q_MN ? ptx::kTcBMajorMN : 0u);
+  if (status_word(device, &p.status) != 0) return -1;
+  const int64_t grid = ceil_div(lp.I, kRows) * p.tiles_j * parts;
+  if (grid >= (int64_t(1) << 31)) return fail("tvb_linear: too many output tiles");
+  return launch_dependent_cluster("linear_split", kernel, parts, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg::kSmemBytes, stream,
+                                  map_p, map_q, p);
+}
+
+template <int TN, bool BF16>
+int split_orders(int device, cudaStream_t stream, const LinearProduct& lp, int parts) {
+  if (!lp.q_mn) return lp.p_mn ? split_run<TN, true, false, BF16>(device, stream, lp, parts) : split_run<TN, false, false, BF16>(device, stream, lp, parts);
+  if constexpr (TN >= 64) {
+    if (lp.p_mn) return split_run<TN, true, true, BF16>(device, stream, lp, parts);
+  }
+  return fail("tvb_linear: no kernel for this order of the operands");
+}
+
+}  // namespace
+
+int linear_split(int device, cudaStream_t stream, const LinearProduct& lp) {
+  int tn = lp.q_mn ? 64 : 16;
+  while (tn < 256 && tn < lp.J) tn *= 2;
+  const int64_t tiles = ceil_div(lp.I, kRows) * ceil_div(lp.J, tn), blocks = ceil_div(lp.R, kStepR);
+  const int64_t slots = static_cast<int64_t>(sm_count(device)) * (tn <= 128 ? 2 : 1);
+  int parts = 1;
+  while (parts < 8 && tiles * parts * 2 <= slots && blocks >= parts * 2 * 4) parts *= 2;
+  const bool bf16 = lp.dtype == TVB_BF16;
+  switch (tn) {
+    case 16: return bf16 ? split_orders<16, true>(device, stream, lp, parts) : split_orders<16, false>(device, stream, lp, parts);
+    case 32: return bf16 ? split_orders<32, true>(device, stream, lp, parts) : split_orders<32, false>(device, stream, lp, parts);
+    case 64: return bf16 ? split_orders<64, true>(device, stream, lp, parts) : split_orders<64, false>(device, stream, lp, parts);
+    case 128: return bf16 ? split_orders<128, true>(device, stream, lp, parts) : split_orders<128, false>(device, stream, lp, parts);
+    default: return bf16 ? split_orders<256, true>(device, stream, lp, parts) : split_orders<256, false>(device, stream, lp, parts);
+  }
+}
+
+}  // namespace tvb

@@ -273,6 +273,18 @@ __device__ __forceinline__ uint64_t tc_smem_desc_sw64(uint32_t smem_addr) {
   return d;
 }
 
+// The same for an operand tile whose contiguous direction is not k (MN-major, 128-byte swizzle): boxes of 64 rows of k x 128
+// bytes, groups of 8 rows of k 1024 bytes apart, and the next 128 bytes of the contiguous direction one box (8192 bytes) on. 16
+// values of k are 2048 bytes: +128 in the descriptor's 16-byte units.
+__device__ __forceinline__ uint64_t tc_smem_desc_sw128_mn(uint32_t smem_addr) {
+  uint64_t d = tc_smem_desc_sw128(smem_addr);
+  d |= static_cast<uint64_t>(8192u >> 4) << 16;  // stride between 128-byte columns of the contiguous direction
+  return d;
+}
+
+// Bits of the instruction descriptor: operand A / B is MN-major.
+constexpr uint32_t kTcAMajorMN = 1u << 15, kTcBMajorMN = 1u << 16;
+
 // Instruction descriptor: D format (1 float32, 2 int32), A / B formats (kind-specific codes),
 // both operands K-major, tile n x m.
 __host__ __device__ constexpr uint32_t tc_instr_desc(uint32_t d_fmt, uint32_t a_fmt, uint32_t b_fmt, uint32_t m, uint32_t n) {
