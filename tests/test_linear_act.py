@@ -110,3 +110,33 @@ def test_wrappers_refuse_what_they_cannot_pass_on():
     for bad in (lambda: cabi.linear(x.double(), w.double()), lambda: cabi.layer_norm(x.to(torch.int32))):
         with pytest.raises(TypeError):
             bad()
+
+
+@pytest.mark.parametrize("tiles,blocks,pairs", [((128, 896), (224, 32), 74), ((5, 40), (100, 7), 74), ((74, 74), (64, 64), 74), ((75, 3), (9, 9), 74),
+                                                ((1, 1), (3, 2), 2), ((500, 0), (8, 1), 74), ((30, 2000), (64, 3), 74), ((148, 10), (16, 16), 74)])
+def test_the_schedule_of_two_products_covers_every_tile_once(tiles, blocks, pairs):
+    """The same formulas as PairSchedule (csrc/kernels/linear_pair.cu): every tile of both products is one pair's, and no pair has
+    more than one tile's worth of work above an even share when there are tiles enough."""
+    a, b = blocks
+    extra = light_first = 0
+    rest = tiles[0] % pairs
+    if tiles[1] and rest:
+        extra = (2 * a + b) // (2 * b)
+        light_first = extra * b < a
+    light = pairs - rest if rest else 0
+    early = light * extra
+    seen, loads = set(), []
+    for pair in range(pairs):
+        mine = [(0, t) for t in range(pair, tiles[0], pairs)]
+        is_light = rest != 0 and pair >= rest
+        rank = pair - rest if is_light else pair
+        if is_light:
+            mine += [(1, t) for t in range(rank, min(early, tiles[1]), light)]
+        order = (rank if is_light else light + pair) if rest and light_first else pair
+        mine += [(1, t) for t in range(early + order, tiles[1], pairs)]
+        assert not seen & set(mine)
+        seen |= set(mine)
+        loads.append(sum(blocks[p] for p, _ in mine))
+    assert len(seen) == sum(tiles)
+    if tiles[1] >= 2 * early:
+        assert max(loads) <= sum(t * c for t, c in zip(tiles, blocks)) / pairs + 2 * b

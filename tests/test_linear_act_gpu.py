@@ -14,6 +14,10 @@ SIZES = [(1, 1, 1), (1, 8, 3), (3, 5, 7), (1, 64, 128), (2, 200, 129), (16, 128,
          (77, 1003, 517), (130, 328, 72), (200, 512, 300), (256, 64, 256), (257, 136, 520), (700, 96, 640), (5, 4104, 24)]
 
 
+# outputs large enough for the kernel of CTA pairs: whole tiles, ragged edges in both directions, widths of tile below 256
+LARGE = [(2048, 128, 2048), (1900, 200, 2600), (1024, 1032, 5000), (2001, 77, 1999), (4096, 64, 1024), (300, 520, 14336)]
+
+
 def cuda(*shape, seed, dtype, scale=1.0):
     return (torch.randn(*shape, generator=D.gen(seed)) * scale).to(dtype).cuda()
 
@@ -40,6 +44,31 @@ def test_forward_sizes(dtype, m, k, n):
     D.check("z", pre, z, ztol)
     want, tol, _, _ = D.linear64(x, w, None, None, "none")
     D.check("product", run(cabi.linear, x, w), want, tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,k,n", LARGE)
+def test_large_outputs(dtype, m, k, n):
+    x, w, b, r = operands(m, k, n, dtype, seed=15)
+    for act, bias, res in (("gelu_tanh", b, r), ("none", None, None)):
+        want, tol, z, ztol = D.linear64(x, w, bias, res, act)
+        y, pre = run(cabi.linear, x, w, bias, residual=res, activation=act, save_preactivation=True)
+        D.check("y", y, want, tol)
+        D.check("z", pre, z, ztol)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,k,n", [(2048, 2048, 2048), (1900, 2600, 2000), (2048, 4096, 1024), (4100, 1800, 1900), (2001, 1999, 2003)])
+def test_large_gradients(dtype, m, k, n):
+    """Both products of the backward pass in one launch, and each alone."""
+    x, w, b, dy = operands(m, k, n, dtype, seed=16)
+    z = (x.double() @ w.double().t() + b.double()).to(dtype)
+    want = D.linear_backward64(dy, x, w, z, "silu")
+    for need in ((True, True, True), (True, False, False), (False, True, False)):
+        got = run(cabi.linear_backward, dy, x, w, z, activation="silu", need=need)
+        for name, g, asked in zip(("dx", "dw", "db"), got, need):
+            if asked:
+                D.check((need, name), g, *want[name])
 
 
 @pytest.mark.parametrize("dtype", D.DTYPES)

@@ -44,8 +44,12 @@ int make_readable(int device, cudaStream_t stream, int dtype, const void** p, in
   return 0;
 }
 
+// Large outputs go to the kernel of CTA pairs, small ones to the one that splits r.
+bool large(const LinearProduct& p) { return p.R > 0 && p.J > 256 && p.I >= 256 && p.I * p.J >= int64_t(48) * 256 * 256; }
+
 int run_product(int device, cudaStream_t stream, const LinearProduct& p) {
-  return p.dtype == TVB_F32 ? linear_simt(stream, p) : linear_split(device, stream, p);
+  if (p.dtype == TVB_F32) return linear_simt(stream, p);
+  return large(p) ? linear_pair(device, stream, &p, 1) : linear_split(device, stream, p);
 }
 
 // dz needs a matrix of its own: there is an activation to differentiate, or TMA cannot read dy.
@@ -158,23 +162,26 @@ extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_
   }
   if (want_dw && make_readable(device, stream, dtype, &x, m, k, &x_sm, &at) != 0) return -1;
   if (want_dx && make_readable(device, stream, dtype, &w, n, k, &w_sn, &at) != 0) return -1;
+  LinearProduct p[2] = {};
+  int count = 0;
   if (want_dx) {
-    LinearProduct p{};
-    p.p = w; p.p_si = 1; p.p_sr = w_sn; p.p_mn = true;
-    p.q = dz; p.q_sj = dz_ld; p.q_sr = 1;
-    p.out = dx;
-    p.I = k; p.J = m; p.R = n;
-    p.dtype = dtype;
-    if (run_product(device, stream, p) != 0) return -1;
+    LinearProduct& d = p[count++];
+    d.p = w; d.p_si = 1; d.p_sr = w_sn; d.p_mn = true;
+    d.q = dz; d.q_sj = dz_ld; d.q_sr = 1;
+    d.out = dx;
+    d.I = k; d.J = m; d.R = n;
+    d.dtype = dtype;
   }
   if (want_dw) {
-    LinearProduct p{};
-    p.p = x; p.p_si = 1; p.p_sr = x_sm; p.p_mn = true;
-    p.q = dz; p.q_sj = 1; p.q_sr = dz_ld; p.q_mn = true;
-    p.out = dw;
-    p.I = k; p.J = n; p.R = m;
-    p.dtype = dtype;
-    if (run_product(device, stream, p) != 0) return -1;
+    LinearProduct& d = p[count++];
+    d.p = x; d.p_si = 1; d.p_sr = x_sm; d.p_mn = true;
+    d.q = dz; d.q_sj = 1; d.q_sr = dz_ld; d.q_mn = true;
+    d.out = dw;
+    d.I = k; d.J = n; d.R = m;
+    d.dtype = dtype;
   }
+  if (count == 2 && dtype != TVB_F32 && large(p[0]) && large(p[1])) return linear_pair(device, stream, p, 2);
+  for (int i = 0; i < count; i++)
+    if (run_product(device, stream, p[i]) != 0) return -1;
   return 0;
 }

@@ -31,6 +31,7 @@ struct LinearProduct {
 int linear_simt(cudaStream_t stream, const LinearProduct& p);  // float32
 // float16 and bfloat16, on the tensor cores; every operand begins on 16 bytes and its rows are a multiple of 16 bytes apart.
 int linear_split(int device, cudaStream_t stream, const LinearProduct& p);
+int linear_pair(int device, cudaStream_t stream, const LinearProduct* p, int count);  // one or two products, R > 0
 
 // Copies a 16-bit [rows, cols] matrix to rows dst_ld (a multiple of 8) apart.
 int linear_pad(int device, cudaStream_t stream, void* dst, int64_t dst_ld, const void* src, int64_t src_ld, int64_t rows, int64_t cols);
