@@ -452,7 +452,11 @@ TVB_API int tvb_addmm(int device, const void* a, int dtype, int64_t a_s0, int64_
  * tvb_linear_backward needs of a forward pass with an activation. y may be the residual itself (residual_sm == n); no other
  * output may overlap an operand. 16-bit products run on the tensor cores whatever their sizes; operands whose rows do not
  * begin on 16 bytes are first copied into the workspace (tvb_linear_workspace_bytes of them; 0 for aligned ones), which the
- * caller owns, 256-byte aligned, and which is free again when the queued work has run. float32 runs on the CUDA cores. */
+ * caller owns, 256-byte aligned, and which is free again when the queued work has run. float32 runs on the CUDA cores.
+ * stream (here and in the three calls below): NULL queues on the device's stream, as everything else does; any other stream of
+ * the device may be named instead (cudaStreamLegacy for the default one): these calls use none of the runtime's scratch, so
+ * calls on different streams need no ordering but that of their own operands. The calling thread's current device is
+ * `device` afterwards. */
 enum TvbActivation {
   TVB_ACT_NONE = 0,
   TVB_ACT_RELU = 1,
@@ -464,7 +468,7 @@ TVB_API uint64_t tvb_linear_workspace_bytes(int dtype, const void* x, int64_t x_
                                             int64_t k);
 TVB_API int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, const void* w, int64_t w_sn, const void* bias, int activation,
                        const void* residual, int64_t residual_sm, void* y, void* preact, int64_t m, int64_t n, int64_t k,
-                       void* workspace, uint64_t workspace_bytes);
+                       void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* The gradients of the layer above, given dy = dL/dy (rows dy_sm >= n apart) and the forward pass's preact (contiguous
  * [m, n]; may be NULL without an activation):
@@ -477,7 +481,7 @@ TVB_API uint64_t tvb_linear_backward_workspace_bytes(int dtype, const void* dy, 
                                                      int64_t w_sn, int activation, int want, int64_t m, int64_t n, int64_t k);
 TVB_API int tvb_linear_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* preact, const void* x, int64_t x_sm,
                                 const void* w, int64_t w_sn, int activation, void* dx, void* dw, void* db, int64_t m, int64_t n,
-                                int64_t k, void* workspace, uint64_t workspace_bytes);
+                                int64_t k, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* ---- layer norm over the last dimension: aten::native_layer_norm and its backward (what a model has between its Linears) ----
  * y = (x - mean) * rstd * weight + bias per row of d values; mean and rstd = 1 / sqrt(var + eps) of every row in float32 (var:
@@ -485,7 +489,7 @@ TVB_API int tvb_linear_backward(int device, const void* dy, int dtype, int64_t d
  * dtype or float32 (param_dtype), each may be NULL (1 and 0); mean and rstd may be NULL. With rows == 0 or d == 0 nothing is
  * written. No output may overlap an operand. */
 TVB_API int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm, const void* weight, const void* bias, int param_dtype,
-                           float eps, void* y, float* mean, float* rstd, int64_t rows, int64_t d);
+                           float eps, void* y, float* mean, float* rstd, int64_t rows, int64_t d, void* stream);
 /* With h = (x - mean) * rstd and u = dy * weight: dx = rstd * (u - <u> - h <u h>) (<.>: the mean over the row), dweight = sum
  * over the rows of dy h, dbias = sum of dy. Any of the three may be NULL; dweight and dbias are of param_dtype. The sums over
  * the rows are float32, in a fixed order (partial sums in the caller's workspace, 16-byte aligned; needed when dweight or
@@ -493,7 +497,7 @@ TVB_API int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm, c
 TVB_API uint64_t tvb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d);
 TVB_API int tvb_layer_norm_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* x, int64_t x_sm, const float* mean,
                                     const float* rstd, const void* weight, int param_dtype, void* dx, void* dweight, void* dbias,
-                                    int64_t rows, int64_t d, void* workspace, uint64_t workspace_bytes);
+                                    int64_t rows, int64_t d, void* workspace, uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -14,11 +14,11 @@ def refused(rc, *words):
 
 
 def linear(x=A, dtype=cabi.BF16, x_sm=64, w=B, w_sn=64, bias=None, act=0, res=None, res_sm=0, y=C, z=None, m=4, n=32, k=64, ws=None, nb=0):
-    return cabi.lib().tvb_linear(0, x, dtype, x_sm, w, w_sn, bias, act, res, res_sm, y, z, m, n, k, ws, nb)
+    return cabi.lib().tvb_linear(0, x, dtype, x_sm, w, w_sn, bias, act, res, res_sm, y, z, m, n, k, ws, nb, None)
 
 
 def backward(dy=A, dtype=cabi.BF16, dy_sm=32, z=None, x=B, x_sm=64, w=C, w_sn=64, act=0, dx=E, dw=F, db=G, m=4, n=32, k=64, ws=None, nb=0):
-    return cabi.lib().tvb_linear_backward(0, dy, dtype, dy_sm, z, x, x_sm, w, w_sn, act, dx, dw, db, m, n, k, ws, nb)
+    return cabi.lib().tvb_linear_backward(0, dy, dtype, dy_sm, z, x, x_sm, w, w_sn, act, dx, dw, db, m, n, k, ws, nb, None)
 
 
 def test_linear_refusals():
@@ -64,11 +64,11 @@ def test_layer_norm_refusals():
     so = cabi.lib()
 
     def fwd(x=A, dtype=cabi.BF16, x_sm=64, w=B, b=None, pdt=cabi.BF16, eps=1e-5, y=C, mean=E, rstd=F, rows=4, d=64):
-        return so.tvb_layer_norm(0, x, dtype, x_sm, w, b, pdt, eps, y, mean, rstd, rows, d)
+        return so.tvb_layer_norm(0, x, dtype, x_sm, w, b, pdt, eps, y, mean, rstd, rows, d, None)
 
     def bwd(dy=A, dtype=cabi.BF16, dy_sm=64, x=B, x_sm=64, mean=C, rstd=C + 4096, w=None, pdt=cabi.BF16, dx=E, dw=F, db=F + 4096, rows=4, d=64,
             ws=G, nb=1 << 20):
-        return so.tvb_layer_norm_backward(0, dy, dtype, dy_sm, x, x_sm, mean, rstd, w, pdt, dx, dw, db, rows, d, ws, nb)
+        return so.tvb_layer_norm_backward(0, dy, dtype, dy_sm, x, x_sm, mean, rstd, w, pdt, dx, dw, db, rows, d, ws, nb, None)
 
     refused(fwd(dtype=cabi.F64), "float32, float16 or bfloat16")
     refused(fwd(pdt=cabi.F16), "x's dtype or float32")

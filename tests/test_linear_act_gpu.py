@@ -117,7 +117,7 @@ def test_forward_written_over_the_residual(dtype, m):
     code = cabi._dtype_code(dtype)
     torch.cuda.synchronize()
     cabi.check(cabi.lib().tvb_linear(0, x.data_ptr(), code, k, w.data_ptr(), k, b.data_ptr(), cabi.ACTIVATIONS["relu"], r.data_ptr(), n,
-                                     r.data_ptr(), None, m, n, k, None, 0))
+                                     r.data_ptr(), None, m, n, k, None, 0, None))
     cabi.synchronize()
     D.check("y", r, want, tol)
 

@@ -9,6 +9,8 @@ no B200 is present, the calls raise.
 import ctypes
 import os
 
+from . import _native
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libtvb200.so")
 
@@ -120,12 +122,12 @@ SIGNATURES = {
     "tvb_scaled_mm": (_i, [_i, _vp, _i, _i64, _i64, _vp, _i, _i64, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i64, _i64,
                            _i64, _i]),
     "tvb_linear_workspace_bytes": (_u64, [_i, _vp, _i64, _vp, _i64, _i64, _i64, _i64]),
-    "tvb_linear": (_i, [_i, _vp, _i, _i64, _vp, _i64, _vp, _i, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _u64]),
+    "tvb_linear": (_i, [_i, _vp, _i, _i64, _vp, _i64, _vp, _i, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _u64, _vp]),
     "tvb_linear_backward_workspace_bytes": (_u64, [_i, _vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i64, _i64, _i64]),
-    "tvb_linear_backward": (_i, [_i, _vp, _i, _i64, _vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _u64]),
-    "tvb_layer_norm": (_i, [_i, _vp, _i, _i64, _vp, _vp, _i, _c.c_float, _vp, _vp, _vp, _i64, _i64]),
+    "tvb_linear_backward": (_i, [_i, _vp, _i, _i64, _vp, _vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _u64, _vp]),
+    "tvb_layer_norm": (_i, [_i, _vp, _i, _i64, _vp, _vp, _i, _c.c_float, _vp, _vp, _vp, _i64, _i64, _vp]),
     "tvb_layer_norm_backward_workspace_bytes": (_u64, [_i64, _i64]),
-    "tvb_layer_norm_backward": (_i, [_i, _vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i64, _vp, _u64]),
+    "tvb_layer_norm_backward": (_i, [_i, _vp, _i, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i64, _vp, _u64, _vp]),
 }
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # TvbActivation
@@ -370,41 +372,8 @@ def scaled_mm(a, b, scale_a, scale_b, bias=None, scale_result=None, out_dtype=No
     return out
 
 
-# ---- the fused Linear layer and layer norm. Like the wrappers above they take tensors in device memory (torch.cuda tensors, or
-# "vk" tensors), queue on the backend's stream (tvb_stream) and allocate their outputs on the operands' device: whoever mixes
-# them with other work on the same tensors orders that stream and theirs (tvb_set_stream, or a synchronize between).
-
-_FLOATS = None
-
-
-def _float_code(t):
-    global _FLOATS
-    if _FLOATS is None:
-        import torch
-
-        _FLOATS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    code = _FLOATS.get(t.dtype)
-    if code is None:
-        raise TypeError(f"float32, float16 or bfloat16 expected, got {t.dtype}")
-    return code
-
-
-def _matrix(fn, name, t, rows, cols, like):
-    """Checks a [rows, cols] operand with contiguous columns; returns its row stride in elements."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{fn}: {name} must be a {like.dtype} matrix [{rows}, {cols}] on {like.device}, got {t.dtype} "
-                         f"{list(t.shape)} on {t.device}")
-    s0, s1 = t.stride()
-    if (cols > 1 and s1 != 1) or (rows > 1 and s0 < cols):
-        raise ValueError(f"{fn}: {name} needs contiguous columns and rows that do not overlap (strides {(s0, s1)})")
-    return s0 if rows > 1 else cols
-
-
-def _vector(fn, name, t, n, like, dtypes=None):
-    if t.dim() != 1 or t.shape[0] != n or t.device != like.device or not t.is_contiguous() or t.dtype not in (dtypes or (like.dtype,)):
-        raise ValueError(f"{fn}: {name} must be a contiguous vector of {n} values on {like.device} of "
-                         f"{' or '.join(str(d) for d in (dtypes or (like.dtype,)))}, got {t.dtype} {list(t.shape)} on {t.device}")
-
+# ---- the fused Linear layer and layer norm. "vk" tensors: queued on the backend's stream, like every op of the device.
+# torch.cuda tensors: queued on torch's current stream, allocations included, like any CUDA op (and capturable with it).
 
 def _activation(fn, activation):
     code = ACTIVATIONS.get(activation)
@@ -413,122 +382,28 @@ def _activation(fn, activation):
     return code
 
 
-def _workspace(nbytes, like):
-    """(tensor to keep, its address or None)"""
-    if nbytes == 0:
-        return None, None
-    import torch
-
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    return ws, ws.data_ptr()
-
-
-def _out(t):
-    return t.data_ptr() if t is not None else None
-
-
 def linear(x, w, bias=None, residual=None, activation="none", save_preactivation=False):
-    """tvb_linear on device tensors: act(x @ w.t() + bias) + residual for x [m, k], w [n, k], bias [n], residual [m, n].
-    With save_preactivation returns (y, z), z being x @ w.t() + bias: what linear_backward takes for an activation."""
-    import torch
-
-    code, act = _float_code(x), _activation("linear", activation)
-    if x.dim() != 2 or w.dim() != 2:
-        raise ValueError("linear: x [m, k] and w [n, k] expected")
-    (m, k), n = x.shape, w.shape[0]
-    x_sm, w_sn = _matrix("linear", "x", x, m, k, x), _matrix("linear", "w", w, n, k, x)
-    if bias is not None:
-        _vector("linear", "bias", bias, n, x)
-    r_sm = _matrix("linear", "residual", residual, m, n, x) if residual is not None else 0
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    z = torch.empty((m, n), dtype=x.dtype, device=x.device) if save_preactivation else None
-    so, xp, wp = lib(), x.data_ptr(), w.data_ptr()
-    nbytes = so.tvb_linear_workspace_bytes(code, xp, x_sm, wp, w_sn, m, n, k)
-    ws, ws_ptr = _workspace(nbytes, x)
-    check(so.tvb_linear(_dev(x), xp, code, x_sm, wp, w_sn, _out(bias), act, _out(residual), r_sm, y.data_ptr(), _out(z), m, n, k,
-                        ws_ptr, nbytes))
+    """tvb_linear on device tensors: act(x @ w.t() + bias) + residual for x [m, k], w [n, k], bias [n], residual [m, n] of one
+    dtype (float32, float16, bfloat16), rows any distance apart, columns contiguous. With save_preactivation returns (y, z), z
+    being x @ w.t() + bias: what linear_backward takes for an activation."""
+    y, z = _native.linear_act(x, w, bias, residual, _activation("linear", activation), save_preactivation)
     return (y, z) if save_preactivation else y
 
 
 def linear_backward(dy, x, w, z=None, activation="none", need=(True, True, True)):
     """tvb_linear_backward on device tensors: (dx, dw, db), None where `need` is false. z: what linear saved (not needed
-    without an activation)."""
-    import torch
-
-    code, act = _float_code(x), _activation("linear_backward", activation)
-    if x.dim() != 2 or w.dim() != 2:
-        raise ValueError("linear_backward: x [m, k] and w [n, k] expected")
-    (m, k), n = x.shape, w.shape[0]
-    x_sm, w_sn = _matrix("linear_backward", "x", x, m, k, x), _matrix("linear_backward", "w", w, n, k, x)
-    dy_sm = _matrix("linear_backward", "dy", dy, m, n, x)
-    if z is not None:
-        _matrix("linear_backward", "z", z, m, n, x)
-        if not z.is_contiguous():
-            raise ValueError("linear_backward: z must be contiguous")
-    elif act != 0:
-        raise ValueError("linear_backward: an activation's gradient needs z, the values before it")
-    dx = torch.empty((m, k), dtype=x.dtype, device=x.device) if need[0] else None
-    dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need[1] else None
-    db = torch.empty((n,), dtype=x.dtype, device=x.device) if need[2] else None
-    so, dyp, xp, wp = lib(), dy.data_ptr(), x.data_ptr(), w.data_ptr()
+    without an activation). The residual's gradient is dy."""
     want = (WANT_DX if need[0] else 0) | (WANT_DW if need[1] else 0) | (WANT_DB if need[2] else 0)
-    nbytes = so.tvb_linear_backward_workspace_bytes(code, dyp, dy_sm, xp, x_sm, wp, w_sn, act, want, m, n, k)
-    ws, ws_ptr = _workspace(nbytes, x)
-    check(so.tvb_linear_backward(_dev(x), dyp, code, dy_sm, _out(z), xp, x_sm, wp, w_sn, act, _out(dx), _out(dw), _out(db), m, n, k,
-                                 ws_ptr, nbytes))
-    return dx, dw, db
-
-
-def _norm_params(fn, x, d, *params):
-    """The common dtype code of weight and bias (each may be None)."""
-    import torch
-
-    given = [(name, t) for name, t in params if t is not None]
-    for name, t in given:
-        _vector(fn, name, t, d, x, (x.dtype, torch.float32))
-    if len({t.dtype for _, t in given}) > 1:
-        raise ValueError(f"{fn}: weight and bias must have one dtype")
-    return _float_code(given[0][1]) if given else _float_code(x)
+    return _native.linear_act_backward(dy, x, w, z, _activation("linear_backward", activation), want)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
-    """tvb_layer_norm on device tensors: (y, mean, rstd) for x [rows, d], weight and bias [d] (of x's dtype or float32)."""
-    import torch
-
-    code = _float_code(x)
-    if x.dim() != 2:
-        raise ValueError("layer_norm: x [rows, d] expected")
-    rows, d = x.shape
-    x_sm = _matrix("layer_norm", "x", x, rows, d, x)
-    pcode = _norm_params("layer_norm", x, d, ("weight", weight), ("bias", bias))
-    y = torch.empty((rows, d), dtype=x.dtype, device=x.device)
-    mean = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    check(lib().tvb_layer_norm(_dev(x), x.data_ptr(), code, x_sm, _out(weight), _out(bias), pcode, eps, y.data_ptr(),
-                               mean.data_ptr(), rstd.data_ptr(), rows, d))
-    return y, mean, rstd
+    """tvb_layer_norm on device tensors: (y, mean, rstd) for x [rows, d] (float32, float16, bfloat16), weight and bias [d] of
+    x's dtype or float32; mean and rstd [rows] in float32."""
+    return _native.layer_norm(x, weight, bias, eps)
 
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True)):
     """tvb_layer_norm_backward on device tensors: (dx, dweight, dbias), None where `need` is false; mean and rstd [rows] as
     layer_norm returned them. dweight and dbias have weight's dtype (x's without a weight)."""
-    import torch
-
-    code = _float_code(x)
-    if x.dim() != 2:
-        raise ValueError("layer_norm_backward: x [rows, d] expected")
-    rows, d = x.shape
-    x_sm, dy_sm = _matrix("layer_norm_backward", "x", x, rows, d, x), _matrix("layer_norm_backward", "dy", dy, rows, d, x)
-    pcode = _norm_params("layer_norm_backward", x, d, ("weight", weight))
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _vector("layer_norm_backward", name, t, rows, x, (torch.float32,))
-    pdtype = weight.dtype if weight is not None else x.dtype
-    dx = torch.empty((rows, d), dtype=x.dtype, device=x.device) if need[0] else None
-    dg = torch.empty((d,), dtype=pdtype, device=x.device) if need[1] else None
-    db = torch.empty((d,), dtype=pdtype, device=x.device) if need[2] else None
-    so = lib()
-    nbytes = so.tvb_layer_norm_backward_workspace_bytes(rows, d) if need[1] or need[2] else 0
-    ws, ws_ptr = _workspace(nbytes, x)
-    check(so.tvb_layer_norm_backward(_dev(x), dy.data_ptr(), code, dy_sm, x.data_ptr(), x_sm, mean.data_ptr(), rstd.data_ptr(),
-                                     _out(weight), pcode, _out(dx), _out(dg), _out(db), rows, d, ws_ptr, nbytes))
-    return dx, dg, db
+    return _native.layer_norm_backward(dy, x, mean, rstd, weight, need[0], need[1], need[2])

@@ -46,6 +46,17 @@ void clear_weight_caches();
 at::Tensor int8_linear(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scales, const at::Tensor& bias,
                        const at::Tensor& residual);
 
+// The fused Linear layer and layer norm on "vk" or CUDA tensors (ops_dense.cpp); undefined tensors where nothing was asked for.
+std::tuple<at::Tensor, at::Tensor> linear_act(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
+                                              const std::optional<at::Tensor>& residual, int64_t activation, bool save);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_act_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w,
+                                                                   const std::optional<at::Tensor>& z, int64_t activation, int64_t want);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                                                          const std::optional<at::Tensor>& bias, double eps);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& mean,
+                                                                   const at::Tensor& rstd, const std::optional<at::Tensor>& weight,
+                                                                   bool need_x, bool need_weight, bool need_bias);
+
 void register_backend();
 void shutdown_backend();
 

@@ -77,5 +77,9 @@ PYBIND11_MODULE(_native, m) {
         return vkb::int8_linear(a, b, scales, bias.value_or(at::Tensor()), residual.value_or(at::Tensor()));
       },
       py::arg("a"), py::arg("b"), py::arg("scales"), py::arg("bias") = py::none(), py::arg("residual") = py::none());
+  m.def("linear_act", &vkb::linear_act, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_act_backward", &vkb::linear_act_backward, py::call_guard<py::gil_scoped_release>());
+  m.def("layer_norm", &vkb::layer_norm, py::call_guard<py::gil_scoped_release>());
+  m.def("layer_norm_backward", &vkb::layer_norm_backward, py::call_guard<py::gil_scoped_release>());
   m.def("shutdown", &vkb::shutdown_backend);
 }

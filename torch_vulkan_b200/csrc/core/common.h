@@ -20,6 +20,13 @@ int fail_cuda(const char* what, cudaError_t err);
 // message if the device does not exist or is not an sm_100 part.
 int enter(int device, cudaStream_t* stream);
 
+// The same for the launchers that take a stream of the caller's: NULL is the device's own.
+inline int enter_on(int device, void* caller_stream, cudaStream_t* stream) {
+  if (enter(device, stream) != 0) return -1;
+  if (caller_stream != nullptr) *stream = static_cast<cudaStream_t>(caller_stream);
+  return 0;
+}
+
 // Counts one kernel launch (tvb_dispatch_count) and, with TVB200_TRACE=1,
 // prints it and waits for it (as TORCH_VK_TRACE, ffi.rs:135-148).
 int launched(const char* name, dim3 grid, dim3 block, size_t smem, cudaStream_t stream);

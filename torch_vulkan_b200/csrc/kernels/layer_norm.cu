@@ -443,7 +443,7 @@ int check_sizes(const char* fn, int dtype, int param_dtype, int64_t rows, int64_
 using namespace tvb;
 
 extern "C" int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm, const void* weight, const void* bias, int param_dtype,
-                              float eps, void* y, float* mean, float* rstd, int64_t rows, int64_t d) {
+                              float eps, void* y, float* mean, float* rstd, int64_t rows, int64_t d, void* caller_stream) {
   if (check_sizes("tvb_layer_norm", dtype, param_dtype, rows, d) != 0) return -1;
   TVB_REQUIRE(eps >= 0.0f, "tvb_layer_norm: eps must not be negative");
   TVB_REQUIRE(rows <= 1 || x_sm >= d, "tvb_layer_norm: rows of x must be at least d apart");
@@ -455,7 +455,7 @@ extern "C" int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm
                   !overlap(y, y_bytes, weight, d * dtype_size(param_dtype)) && !overlap(y, y_bytes, bias, d * dtype_size(param_dtype)),
               "tvb_layer_norm: an output overlaps another operand");
   cudaStream_t stream;
-  if (enter(device, &stream) != 0) return -1;
+  if (enter_on(device, caller_stream, &stream) != 0) return -1;
   NormParams p{};
   p.x = x; p.weight = weight; p.bias = bias; p.y = y; p.mean = mean; p.rstd = rstd;
   p.x_ld = rows > 1 ? x_sm : d;
@@ -472,7 +472,8 @@ extern "C" uint64_t tvb_layer_norm_backward_workspace_bytes(int64_t rows, int64_
 
 extern "C" int tvb_layer_norm_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* x, int64_t x_sm,
                                        const float* mean, const float* rstd, const void* weight, int param_dtype, void* dx, void* dweight,
-                                       void* dbias, int64_t rows, int64_t d, void* workspace, uint64_t workspace_bytes) {
+                                       void* dbias, int64_t rows, int64_t d, void* workspace, uint64_t workspace_bytes,
+                                       void* caller_stream) {
   if (check_sizes("tvb_layer_norm_backward", dtype, param_dtype, rows, d) != 0) return -1;
   TVB_REQUIRE(rows <= 1 || (x_sm >= d && dy_sm >= d), "tvb_layer_norm_backward: rows of x and dy must be at least d apart");
   if (d == 0 || (dx == nullptr && dweight == nullptr && dbias == nullptr)) return 0;
@@ -494,7 +495,7 @@ extern "C" int tvb_layer_norm_backward(int device, const void* dy, int dtype, in
       TVB_REQUIRE(!overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]), "tvb_layer_norm_backward: two outputs overlap");
   }
   cudaStream_t stream;
-  if (enter(device, &stream) != 0) return -1;
+  if (enter_on(device, caller_stream, &stream) != 0) return -1;
   NormParams p{};
   p.x = x; p.dy = dy; p.weight = weight; p.y = dx;
   p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);

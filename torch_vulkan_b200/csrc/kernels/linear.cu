@@ -30,18 +30,20 @@ uint64_t copy_bytes(int dtype, const void* p, int64_t rows, int64_t cols, int64_
   return (static_cast<uint64_t>(rows) * static_cast<uint64_t>(round8(cols)) * 2 + 255) & ~uint64_t(255);
 }
 
-// The operand where TMA can read it: in place, or copied to the workspace at *at (which moves on).
-int make_readable(int device, cudaStream_t stream, int dtype, const void** p, int64_t rows, int64_t cols, int64_t* ld, uint8_t** at) {
+// One operand where TMA can read it: in place, or to be copied to the workspace at *at (which moves on).
+LinearCopy make_readable(int dtype, const void** p, int64_t rows, int64_t cols, int64_t* ld, uint8_t** at) {
+  LinearCopy c{};
+  c.dst_ld = 8;
   const uint64_t bytes = copy_bytes(dtype, *p, rows, cols, *ld);
   if (bytes != 0) {
-    if (linear_pad(device, stream, *at, round8(cols), *p, *ld, rows, cols) != 0) return -1;
+    c = LinearCopy{*at, *p, round8(cols), *ld, rows, cols};
     *p = *at;
     *ld = round8(cols);
     *at += bytes;
   } else if (rows <= 1) {
     *ld = round8(cols);  // (one row: the distance to the next is never used, but has to be a legal one)
   }
-  return 0;
+  return c;
 }
 
 // Large outputs go to the kernel of CTA pairs, small ones to the one that splits r.
@@ -71,7 +73,7 @@ extern "C" uint64_t tvb_linear_workspace_bytes(int dtype, const void* x, int64_t
 
 extern "C" int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, const void* w, int64_t w_sn, const void* bias,
                           int activation, const void* residual, int64_t residual_sm, void* y, void* preact, int64_t m, int64_t n,
-                          int64_t k, void* workspace, uint64_t workspace_bytes) {
+                          int64_t k, void* workspace, uint64_t workspace_bytes, void* caller_stream) {
   if (check_linear("tvb_linear", dtype, activation, m, n, k) != 0) return -1;
   TVB_REQUIRE((m <= 1 || x_sm >= k) && (n <= 1 || w_sn >= k), "tvb_linear: rows of x and w must be at least k apart");
   TVB_REQUIRE(residual == nullptr || m <= 1 || residual_sm >= n, "tvb_linear: rows of the residual must be at least n apart");
@@ -94,10 +96,10 @@ extern "C" int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, co
     for (int j = 0; j < i; j++) TVB_REQUIRE(!overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]), "tvb_linear: two outputs overlap");
   }
   cudaStream_t stream;
-  if (enter(device, &stream) != 0) return -1;
+  if (enter_on(device, caller_stream, &stream) != 0) return -1;
   uint8_t* at = static_cast<uint8_t*>(workspace);
-  if (make_readable(device, stream, dtype, &x, m, k, &x_sm, &at) != 0 || make_readable(device, stream, dtype, &w, n, k, &w_sn, &at) != 0)
-    return -1;
+  const LinearCopy cx = make_readable(dtype, &x, m, k, &x_sm, &at), cw = make_readable(dtype, &w, n, k, &w_sn, &at);
+  if (linear_copy(device, stream, cx, cw) != 0) return -1;
   LinearProduct p{};
   p.p = w; p.p_si = w_sn; p.p_sr = 1;
   p.q = x; p.q_sj = x_sm; p.q_sr = 1;
@@ -116,7 +118,7 @@ extern "C" uint64_t tvb_linear_backward_workspace_bytes(int dtype, const void* d
 
 extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* preact, const void* x, int64_t x_sm,
                                    const void* w, int64_t w_sn, int activation, void* dx, void* dw, void* db, int64_t m, int64_t n,
-                                   int64_t k, void* workspace, uint64_t workspace_bytes) {
+                                   int64_t k, void* workspace, uint64_t workspace_bytes, void* caller_stream) {
   if (check_linear("tvb_linear_backward", dtype, activation, m, n, k) != 0) return -1;
   TVB_REQUIRE((m <= 1 || (x_sm >= k && dy_sm >= n)) && (n <= 1 || w_sn >= k),
               "tvb_linear_backward: rows of x and w must be at least k apart, those of dy at least n");
@@ -143,7 +145,7 @@ extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_
       TVB_REQUIRE(!overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]), "tvb_linear_backward: two outputs overlap");
   }
   cudaStream_t stream;
-  if (enter(device, &stream) != 0) return -1;
+  if (enter_on(device, caller_stream, &stream) != 0) return -1;
   const void* dz = dy;
   int64_t dz_ld = m > 1 ? dy_sm : round8(n);
   uint8_t* at = static_cast<uint8_t*>(workspace);
@@ -160,8 +162,10 @@ extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_
     d.dtype = dtype; d.activation = activation;
     if (linear_dz(device, stream, d) != 0) return -1;
   }
-  if (want_dw && make_readable(device, stream, dtype, &x, m, k, &x_sm, &at) != 0) return -1;
-  if (want_dx && make_readable(device, stream, dtype, &w, n, k, &w_sn, &at) != 0) return -1;
+  LinearCopy cx{}, cw{};
+  if (want_dw) cx = make_readable(dtype, &x, m, k, &x_sm, &at);
+  if (want_dx) cw = make_readable(dtype, &w, n, k, &w_sn, &at);
+  if (linear_copy(device, stream, cx, cw) != 0) return -1;
   LinearProduct p[2] = {};
   int count = 0;
   if (want_dx) {

@@ -30,11 +30,17 @@ struct LinearProduct {
 
 int linear_simt(cudaStream_t stream, const LinearProduct& p);  // float32
 // float16 and bfloat16, on the tensor cores; every operand begins on 16 bytes and its rows are a multiple of 16 bytes apart.
+// `count`: one product, or two that share nothing but their launch.
 int linear_split(int device, cudaStream_t stream, const LinearProduct& p);
-int linear_pair(int device, cudaStream_t stream, const LinearProduct* p, int count);  // one or two products, R > 0
+int linear_pair(int device, cudaStream_t stream, const LinearProduct* p, int count);  // R > 0
 
-// Copies a 16-bit [rows, cols] matrix to rows dst_ld (a multiple of 8) apart.
-int linear_pad(int device, cudaStream_t stream, void* dst, int64_t dst_ld, const void* src, int64_t src_ld, int64_t rows, int64_t cols);
+// Copies 16-bit [rows, cols] matrices to rows dst_ld (a multiple of 8) apart: one or two (rows == 0: none) in one launch.
+struct LinearCopy {
+  void* dst;
+  const void* src;
+  int64_t dst_ld, src_ld, rows, cols;
+};
+int linear_copy(int device, cudaStream_t stream, const LinearCopy& a, const LinearCopy& b);
 
 // dz = dy * act'(z) (row stride dz_ld) and db = its sums over the rows; dz or db may be NULL. activation TVB_ACT_NONE: dz = dy.
 struct LinearDz {

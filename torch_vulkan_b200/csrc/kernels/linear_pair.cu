@@ -3,8 +3,7 @@
 // A cluster of two CTAs (the two SMs of a TPC) walks output tiles of 256 rows (j) x BN columns (i), BN a multiple of 32 up to 256.
 // Each CTA stages 128 rows of Q and BN / 2 rows of P per 64 values of r; one lane of CTA 0 issues tcgen05.mma.cta_group::2 for
 // both, and each CTA's TMEM receives its own 128 rows of the tile, in two buffers, so that a tile is read back under the next
-// tile's MMAs. BN is chosen per product so that the tiles fill the last round of pairs (2048 x 14336 outputs: 448 tiles of
-// 256 columns are 7 rounds of 74 pairs, 512 tiles of 224 columns 7 shorter ones).
+// tile's MMAs. BN is 256 unless narrower tiles put more pairs to work.
 //
 // A launch takes one product or two: the backward pass multiplies dz by w and by x at once. The tiles of the product with the
 // longer r come first; pairs that get one tile of it less than others start on the second product meanwhile, and the rest of its
@@ -387,14 +386,16 @@ int pair_product(const LinearProduct& lp, int bn, PairProduct* d) {
   return 0;
 }
 
-// Columns per tile for a product alone in its launch: the width whose rounds of tiles cost least.
+// Columns per tile for a product alone in its launch. A step of a tile costs its SM 128 rows of Q and bn / 2 of P from the L2,
+// which is what paces it (7 rounds of 256 columns: 215 us; 7 of 224: 218; 9 of 192: 249), so narrower tiles pay only where
+// they fill SMs that would have none.
 int pair_columns(const LinearProduct& lp, int pairs) {
   int best = 256;
   int64_t best_cost = -1;
   for (int bn = 256; bn >= 128; bn -= 32) {
     const int64_t tiles = ceil_div(lp.I, bn) * ceil_div(lp.J, kTileJ);
-    const int64_t cost = ceil_div(tiles, pairs) * bn;
-    if (best_cost < 0 || cost < best_cost) {
+    const int64_t cost = ceil_div(tiles, pairs) * (256 + bn);
+    if (best_cost < 0 || cost * 10 < best_cost * 9) {
       best = bn;
       best_cost = cost;
     }
