@@ -3,18 +3,21 @@
 //   dx = rstd (u - <u> - h <u h>),   u = dy g,  h = (x - mean) rstd
 //   dg = sum over rows of dy h,   db = sum over rows of dy
 //
-// Bound by memory: the forward pass reads and writes a row once, the backward pass reads two rows and writes one. A group of T
-// threads (8 or 32 of a warp, or a whole CTA) keeps its row in registers between the statistics and the result, so a row
-// is read once; the variance is taken from the centred values (two passes over registers, none over memory), which a
-// mean far from zero does not spoil. All statistics and sums are float32.
-// The backward pass keeps the sums of dg and db of its columns in registers over all rows that the group handles; one
-// partial row per CTA goes to the workspace and a second kernel adds those in a fixed order (no atomics: the gradients
-// repeat bit for bit).
+// Bound by memory: the forward pass reads and writes a row once, the backward pass reads two rows and writes one. All
+// statistics and sums are float32; the variance is taken from the centred values, which a mean far from zero does not spoil.
+//
+// Forward: a group of T threads (8 or 32 of a warp, or a CTA) keeps its row in registers between the statistics and the result.
+//
+// Backward: persistent CTAs (1024 threads per SM in all) stream their rows of x and dy through a ring in shared memory by bulk
+// copies, so the next rows are on their way whatever the CTA does with the present ones, and keep the sums of dg and db of their
+// columns in registers over all their rows. A cluster of two CTAs adds its sums through distributed shared memory and
+// leaves one partial row in the workspace; a second kernel adds those in a fixed order (no atomics: the gradients repeat bit for
+// bit). Rows that are short, or not whole 16-byte pieces, take the plain form of the kernel.
 #include "../core/common.h"
 #include "launch.h"
 #include "linear_math.cuh"
 #include "numerics.cuh"
-#include "ptx.cuh"
+#include "ptx_pair.cuh"
 
 namespace tvb {
 namespace {
@@ -55,6 +58,133 @@ __device__ __forceinline__ void load_vec(const void* base, int64_t i, float (&v)
   }
 }
 
+// Two neighbouring 16-bit values as a pair of float32 (one register pair, for the instructions that work on both halves at once:
+// with two bytes per value the kernels would be bound by their instructions, not by memory).
+template <int DT>
+__device__ __forceinline__ uint64_t pair16(uint32_t w) {
+  if constexpr (DT == TVB_BF16) return ptx::pack_f32x2(w << 16, w & 0xffff0000u);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return ptx::pack_f32x2(__float_as_uint(f.x), __float_as_uint(f.y));
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t round16(uint64_t v) {
+  float lo, hi;
+  ptx::unpack_f32x2(v, lo, hi);
+  if constexpr (DT == TVB_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four neighbouring values as two pairs: 8 bytes of 16-bit values, 16 of float32.
+template <int DT>
+__device__ __forceinline__ void load_pairs(const void* base, int64_t i, uint64_t (&v)[2]) {
+  if constexpr (DT == TVB_F32) {
+    const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const float*>(base) + i);
+    v[0] = ptx::pack_f32x2(t.x, t.y);
+    v[1] = ptx::pack_f32x2(t.z, t.w);
+  } else {
+    const uint2 t = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + i);
+    v[0] = pair16<DT>(t.x);
+    v[1] = pair16<DT>(t.y);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_pairs(void* base, int64_t i, const uint64_t (&v)[2]) {
+  if constexpr (DT == TVB_F32) {
+    float a, b, c, d;
+    ptx::unpack_f32x2(v[0], a, b);
+    ptx::unpack_f32x2(v[1], c, d);
+    *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = make_float4(a, b, c, d);
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + i) = make_uint2(round16<DT>(v[0]), round16<DT>(v[1]));
+  }
+}
+
+// 16 bytes of a row as pairs (VEC values), or one value.
+template <int DT, int VEC>
+struct Piece {
+  static constexpr int kPairs = VEC / 2;
+  uint64_t v[kPairs];
+  __device__ __forceinline__ void load(const uint8_t* at) {
+    if constexpr (DT == TVB_F32) {
+      load_pairs<DT>(at, 0, v);
+    } else {
+      const uint4 t = *reinterpret_cast<const uint4*>(at);
+      v[0] = pair16<DT>(t.x); v[1] = pair16<DT>(t.y); v[2] = pair16<DT>(t.z); v[3] = pair16<DT>(t.w);
+    }
+  }
+  // weight or bias: of the values' type, or (WIDE) float32 beside 16-bit values
+  template <bool WIDE>
+  __device__ __forceinline__ void load_param(const uint8_t* at) {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int e = 0; e < kPairs; e++) {
+        const uint2 t = *reinterpret_cast<const uint2*>(at + 8 * e);
+        v[e] = ptx::pack_f32x2(t.x, t.y);
+      }
+    } else {
+      load(at);
+    }
+  }
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int e = 0; e < kPairs; e++) v[e] = ptx::both_f32x2(f);
+  }
+  __device__ __forceinline__ void store(uint8_t* at) const {
+    if constexpr (DT == TVB_F32) store_pairs<DT>(at, 0, v);
+    else *reinterpret_cast<uint4*>(at) = make_uint4(round16<DT>(v[0]), round16<DT>(v[1]), round16<DT>(v[2]), round16<DT>(v[3]));
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < kPairs; e++) v[e] = 0;
+  }
+  __device__ __forceinline__ float sum() const {
+    uint64_t s = v[0];
+#pragma unroll
+    for (int e = 1; e < kPairs; e++) s = ptx::add_f32x2(s, v[e]);
+    return ptx::sum_f32x2(s);
+  }
+  // subtracts the mean; returns the sum of the squares
+  __device__ __forceinline__ float center(float mean) {
+    const uint64_t m = ptx::both_f32x2(-mean);
+    uint64_t s = 0;
+#pragma unroll
+    for (int e = 0; e < kPairs; e++) {
+      v[e] = ptx::add_f32x2(v[e], m);
+      s = ptx::fma_f32x2(v[e], v[e], s);
+    }
+    return ptx::sum_f32x2(s);
+  }
+  __device__ __forceinline__ void scale(float rstd, const Piece& g, const Piece& b) {
+    const uint64_t r = ptx::both_f32x2(rstd);
+#pragma unroll
+    for (int e = 0; e < kPairs; e++) v[e] = ptx::fma_f32x2(ptx::mul_f32x2(v[e], r), g.v[e], b.v[e]);
+  }
+};
+template <int DT>
+struct Piece<DT, 1> {
+  float v;
+  __device__ __forceinline__ void load(const uint8_t* at) { v = load_float<DT>(at, 0); }
+  template <bool WIDE>
+  __device__ __forceinline__ void load_param(const uint8_t* at) {
+    v = WIDE ? *reinterpret_cast<const float*>(at) : load_float<DT>(at, 0);
+  }
+  __device__ __forceinline__ void fill(float f) { v = f; }
+  __device__ __forceinline__ void store(uint8_t* at) const { store_float<DT>(at, 0, v); }
+  __device__ __forceinline__ void zero() { v = 0.0f; }
+  __device__ __forceinline__ float sum() const { return v; }
+  __device__ __forceinline__ float center(float mean) {
+    v -= mean;
+    return v * v;
+  }
+  __device__ __forceinline__ void scale(float rstd, const Piece& g, const Piece& b) { v = fmaf(v * rstd, g.v, b.v); }
+};
+
 template <int DT, int VEC>
 __device__ __forceinline__ void store_vec(void* base, int64_t i, const float (&v)[VEC]) {
   if constexpr (VEC == 1) {
@@ -91,25 +221,55 @@ __device__ __forceinline__ void load_param(const void* base, int param_dtype, in
   }
 }
 
-// Sums over the T threads of a group; every thread gets them. `slot` alternates between calls (two buffers: one barrier
-// per call is then enough).
-template <int T>
+// Two values summed over a warp: the first exchange leaves each half of the lanes one of them (five shuffles instead of ten).
+// Lanes 0-15 get the sum of a, lanes 16-31 that of b.
+__device__ __forceinline__ float fold2(float a, float b) {
+  const bool up = (threadIdx.x & 16) != 0;
+  float s = up ? b : a;
+  s += __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
+#pragma unroll
+  for (int x = 8; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+  return s;
+}
+
+// The same over a CTA of `warps` warps, every thread getting both. buf: room for `warps` pairs, another one at every second
+// call (a thread may still be reading one when the next call begins).
+__device__ __forceinline__ void cta_sum2(float& a, float& b, float2* buf, int warps) {
+  const int lane = threadIdx.x & 31;
+  float s = fold2(a, b);
+  if ((lane & 15) == 0) reinterpret_cast<float*>(buf + (threadIdx.x >> 5))[lane >> 4] = s;
+  __syncthreads();
+  const float2 v = lane < warps ? buf[lane] : make_float2(0.0f, 0.0f);
+  s = fold2(v.x, v.y);
+  a = __shfl_sync(0xffffffffu, s, 0);
+  b = __shfl_sync(0xffffffffu, s, 16);
+}
+
+// Sums of N (one or two) values over the T threads of a group (a power of two up to a warp, or the whole CTA); every thread gets
+// them.
+template <int T, int N = 2>
 __device__ __forceinline__ void group_sum(float& a, float& b, float2 (*buf)[32], int slot) {
+  if constexpr (T > 32 && N == 2) {
+    cta_sum2(a, b, buf[slot], T / 32);
+  } else {
 #pragma unroll
-  for (int s = (T < 32 ? T : 32) / 2; s > 0; s >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, s);
-    b += __shfl_xor_sync(0xffffffffu, b, s);
-  }
-  if constexpr (T > 32) {
-    if ((threadIdx.x & 31) == 0) buf[slot][threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    a = 0.0f;
-    b = 0.0f;
+    for (int s = (T < 32 ? T : 32) / 2; s > 0; s >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, s);
+      if constexpr (N == 2) b += __shfl_xor_sync(0xffffffffu, b, s);
+    }
+    if constexpr (T > 32) {
+      float* one = reinterpret_cast<float*>(buf[slot]);
+      if ((threadIdx.x & 31) == 0) one[threadIdx.x >> 5] = a;
+      __syncthreads();
+      a = 0.0f;
+      if constexpr (T <= 256) {
 #pragma unroll
-    for (int w = 0; w < T / 32; w++) {
-      const float2 v = buf[slot][w];
-      a += v.x;
-      b += v.y;
+        for (int w = 0; w < T / 32; w++) a += one[w];
+      } else {
+        a = (threadIdx.x & 31) < T / 32 ? one[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) a += __shfl_xor_sync(0xffffffffu, a, s);
+      }
     }
   }
 }
@@ -117,61 +277,84 @@ __device__ __forceinline__ void group_sum(float& a, float& b, float2 (*buf)[32],
 template <int T>
 constexpr int norm_threads() { return T < 128 ? 128 : T; }
 
-constexpr int kVals = 32;      // values of a row per thread, forward
-constexpr int kValsBwd = 16;   // backward (with two sums per value beside them)
+constexpr int kValsBwd = 16;   // values of a row per thread in the backward kernels (with two sums per value)
 
-template <int DT, int VEC, int T>
-__global__ void __launch_bounds__(norm_threads<T>()) layer_norm_kernel(const NormParams p) {
-  constexpr int kChunks = kVals / VEC, kGroups = norm_threads<T>() / T;
+// At least this many CTAs per SM: 1024 threads of 64 registers, but for 16-bit rows of up to 4096 values, where a few registers
+// more are worth more than the threads.
+template <int VEC, int T>
+constexpr int norm_ctas_per_sm() { return VEC == 8 && T < 512 ? 1 : 1024 / norm_threads<T>(); }
+
+// The weight's and bias's part of a row's result, with parameters of one width: x = (x rstd) g + b, stored.
+template <int DT, int VEC, int T, int VALS, int ROWS, bool WIDE>
+__device__ __forceinline__ void norm_finish(const NormParams& p, Piece<DT, VEC> (&x)[ROWS][VALS / VEC], const float (&rstd)[ROWS],
+                                            const bool (&live)[ROWS], int64_t row, int t) {
+  constexpr int kSize = DT == TVB_F32 ? 4 : 2, kWidth = WIDE ? 4 : kSize, kPieces = VALS / VEC;
+  const uint8_t* g_at = static_cast<const uint8_t*>(p.weight) + t * VEC * kWidth;
+  const uint8_t* b_at = static_cast<const uint8_t*>(p.bias) + t * VEC * kWidth;
+  uint8_t* y_at[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; k++) y_at[k] = static_cast<uint8_t*>(p.y) + ((row + k) * p.d + t * VEC) * kSize;
+#pragma unroll
+  for (int c = 0; c < kPieces; c++) {
+    if ((c * T + t) * VEC >= p.d) continue;
+    Piece<DT, VEC> g, b;
+    if (p.weight != nullptr) g.template load_param<WIDE>(g_at + c * T * VEC * kWidth);
+    else g.fill(1.0f);
+    if (p.bias != nullptr) b.template load_param<WIDE>(b_at + c * T * VEC * kWidth);
+    else b.fill(0.0f);
+#pragma unroll
+    for (int k = 0; k < ROWS; k++) {
+      x[k][c].scale(rstd[k], g, b);
+      if (live[k]) x[k][c].store(y_at[k] + c * T * VEC * kSize);
+    }
+  }
+}
+
+// VALS values of each of ROWS rows per thread: two rows share the loads and conversions of the parameters and the barriers.
+template <int DT, int VEC, int T, int VALS, int ROWS>
+__global__ void __launch_bounds__(norm_threads<T>(), norm_ctas_per_sm<VEC, T>()) layer_norm_kernel(const NormParams p) {
+  constexpr int kGroups = norm_threads<T>() / T, kPieces = VALS / VEC, kSize = DT == TVB_F32 ? 4 : 2;
   __shared__ float2 buf[2][32];
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const int t = threadIdx.x % T;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / T;
-  const bool live = row < p.rows;  // (every thread takes part in the shuffles)
-  float x[kChunks][VEC];
-  float sum = 0.0f, none = 0.0f;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / T) * ROWS;
+  Piece<DT, VEC> x[ROWS][kPieces];
+  float sum[2] = {}, sq[2] = {}, mean[ROWS], rstd[ROWS];
+  bool live[ROWS];  // (every thread takes part in the sums)
 #pragma unroll
-  for (int c = 0; c < kChunks; c++) {
-    const int col = (c * T + t) * VEC;
+  for (int k = 0; k < ROWS; k++) {
+    live[k] = row + k < p.rows;
+    const uint8_t* at = static_cast<const uint8_t*>(p.x) + ((row + k) * p.x_ld + t * VEC) * kSize;
 #pragma unroll
-    for (int j = 0; j < VEC; j++) x[c][j] = 0.0f;
-    if (live && col < p.d) load_vec<DT, VEC>(p.x, row * p.x_ld + col, x[c]);
-  }
-#pragma unroll
-  for (int c = 0; c < kChunks; c++)
-#pragma unroll
-    for (int j = 0; j < VEC; j++) sum += x[c][j];
-  group_sum<T>(sum, none, buf, 0);
-  const float mean = sum / static_cast<float>(p.d);
-  float sq = 0.0f;
-#pragma unroll
-  for (int c = 0; c < kChunks; c++)
-    if ((c * T + t) * VEC < p.d) {
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        x[c][j] -= mean;
-        sq = fmaf(x[c][j], x[c][j], sq);
-      }
+    for (int c = 0; c < kPieces; c++) {
+      if (live[k] && (c * T + t) * VEC < p.d) x[k][c].load(at + c * T * VEC * kSize);
+      else x[k][c].zero();
     }
-  group_sum<T>(sq, none, buf, 1);
-  const float rstd = 1.0f / sqrtf(sq / static_cast<float>(p.d) + p.eps);
-  if (!live) return;
-  if (t == 0) {
-    if (p.mean != nullptr) p.mean[row] = mean;
-    if (p.rstd != nullptr) p.rstd[row] = rstd;
   }
 #pragma unroll
-  for (int c = 0; c < kChunks; c++) {
-    const int col = (c * T + t) * VEC;
-    if (col >= p.d) continue;
-    float g[VEC], b[VEC];
-    load_param<DT, VEC>(p.weight, p.param_dtype, col, 1.0f, g);
-    load_param<DT, VEC>(p.bias, p.param_dtype, col, 0.0f, b);
+  for (int k = 0; k < ROWS; k++)
 #pragma unroll
-    for (int j = 0; j < VEC; j++) g[j] = fmaf(x[c][j] * rstd, g[j], b[j]);
-    store_vec<DT, VEC>(p.y, row * p.d + col, g);
+    for (int c = 0; c < kPieces; c++) sum[k] += x[k][c].sum();
+  group_sum<T, ROWS>(sum[0], sum[1], buf, 0);
+#pragma unroll
+  for (int k = 0; k < ROWS; k++) {
+    mean[k] = sum[k] / static_cast<float>(p.d);
+#pragma unroll
+    for (int c = 0; c < kPieces; c++)
+      if ((c * T + t) * VEC < p.d) sq[k] += x[k][c].center(mean[k]);
   }
+  group_sum<T, ROWS>(sq[0], sq[1], buf, 1);
+#pragma unroll
+  for (int k = 0; k < ROWS; k++) {
+    rstd[k] = 1.0f / sqrtf(sq[k] / static_cast<float>(p.d) + p.eps);
+    if (t == 0 && live[k]) {
+      if (p.mean != nullptr) p.mean[row + k] = mean[k];
+      if (p.rstd != nullptr) p.rstd[row + k] = rstd[k];
+    }
+  }
+  if (DT != TVB_F32 && p.param_dtype == TVB_F32) norm_finish<DT, VEC, T, VALS, ROWS, true>(p, x, rstd, live, row, t);
+  else norm_finish<DT, VEC, T, VALS, ROWS, false>(p, x, rstd, live, row, t);
 }
 
 // Rows too long for the registers of a CTA: three passes over the row (the second and third mostly from the L2).
@@ -294,6 +477,164 @@ __global__ void __launch_bounds__(norm_threads<T>()) layer_norm_backward_kernel(
   }
 }
 
+// Bytes from global memory into this CTA's shared memory (both on 16 bytes, a multiple of 16), counted at `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
+}
+
+constexpr int kRingCluster = 2;
+
+constexpr int kRingCols = 16;  // columns of a thread
+
+// The streamed form: `stages` slots of one row of x and one of dy each. Row number i of this CTA (row blockIdx.x + i *
+// gridDim.x) lies in slot i % stages; the slot of row i - 1 is refilled behind the barrier inside row i's sums, which every thread
+// reaches only after it is done with row i - 1. A row is read from shared memory twice (for the sums, for dx), and the
+// weights lie there too, which leaves the registers to the column sums.
+// Dynamic shared memory: the ring, the weights (as the values, or float32), two buffers for the sums over the warps.
+template <int DT>
+__global__ void __launch_bounds__(1024) layer_norm_backward_ring_kernel(const NormParams p, const int stages, int* status) {
+  constexpr int kSize = DT == TVB_F32 ? 4 : 2, kUnits = kRingCols / 4;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t bars[8];
+  __shared__ int abort_flag;
+  const int row_bytes = p.d * kSize, t = threadIdx.x, threads = blockDim.x, warps = threads >> 5;
+  const bool wide = DT != TVB_F32 && p.param_dtype == TVB_F32 && p.weight != nullptr;  // weights wider than the values
+  uint8_t* weights = ring + static_cast<size_t>(stages) * 2 * row_bytes;
+  float2* buf = reinterpret_cast<float2*>(weights + (wide ? 4 : kSize) * p.d);
+  const uint32_t ring0 = ptx::smem_u32(ring), bar0 = ptx::smem_u32(bars);
+  if (t == 0) {
+    for (int s = 0; s < stages; s++) ptx::mbar_init(bar0 + 8 * s, 1);
+    abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const int64_t step = gridDim.x;
+  const int count = blockIdx.x < p.rows ? static_cast<int>((p.rows - blockIdx.x + step - 1) / step) : 0;
+  const uint8_t* next_x = static_cast<const uint8_t*>(p.x) + blockIdx.x * p.x_ld * kSize;  // the next row to fetch (thread 0)
+  const uint8_t* next_dy = static_cast<const uint8_t*>(p.dy) + blockIdx.x * p.dy_ld * kSize;
+  int fetched = 0;
+  auto fetch = [&](int slot) {
+    const uint32_t dst = ring0 + 2 * slot * row_bytes, bar = bar0 + 8 * slot;
+    ptx::mbar_expect_tx(bar, 2 * row_bytes);
+    bulk_load(dst, next_x, row_bytes, bar);
+    bulk_load(dst + row_bytes, next_dy, row_bytes, bar);
+    next_x += step * p.x_ld * kSize;
+    next_dy += step * p.dy_ld * kSize;
+    fetched++;
+  };
+  if (t == 0)
+    while (fetched < count && fetched < stages) fetch(fetched);
+  uint64_t dg[kUnits][2] = {}, db[kUnits][2] = {};
+#pragma unroll
+  for (int c = 0; c < kUnits; c++) {  // (every thread reads back only what it wrote)
+    const int col = (c * threads + t) * 4;
+    if (col >= p.d) continue;
+    uint64_t g[2];
+    if (p.weight == nullptr) g[0] = g[1] = ptx::both_f32x2(1.0f);
+    else if (wide) load_pairs<TVB_F32>(p.weight, col, g);
+    else load_pairs<DT>(p.weight, col, g);
+    if (wide) store_pairs<TVB_F32>(weights, col, g);
+    else store_pairs<DT>(weights, col, g);
+  }
+  const float inv_d = 1.0f / static_cast<float>(p.d);
+  int64_t row = blockIdx.x;
+  float mean = count > 0 ? p.mean[row] : 0.0f, rstd = count > 0 ? p.rstd[row] : 0.0f;
+  int slot = 0, before = 0;
+  uint32_t phase = 0;
+  for (int i = 0; i < count; i++) {
+    float next_mean = 0.0f, next_rstd = 0.0f;  // the next row's statistics are asked for a row ahead
+    if (i + 1 < count) {
+      next_mean = p.mean[row + step];
+      next_rstd = p.rstd[row + step];
+    }
+    ptx::mbar_wait(bar0 + 8 * slot, phase, &abort_flag);  // (no early exit: barriers follow)
+    const uint8_t* xs = ring + 2 * slot * row_bytes;
+    const uint64_t m2 = ptx::both_f32x2(-mean), r2 = ptx::both_f32x2(rstd);
+    uint64_t su2 = 0, sux2 = 0;
+    int col = 4 * t;
+#pragma unroll
+    for (int c = 0; c < kUnits; c++, col += 4 * threads) {
+      if (col >= p.d) continue;
+      uint64_t x[2], dy[2], g[2];
+      load_pairs<DT>(xs, col, x);
+      load_pairs<DT>(xs + row_bytes, col, dy);
+      if (wide) load_pairs<TVB_F32>(weights, col, g);
+      else load_pairs<DT>(weights, col, g);
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        x[e] = ptx::add_f32x2(x[e], m2);
+        db[c][e] = ptx::add_f32x2(db[c][e], dy[e]);
+        dg[c][e] = ptx::fma_f32x2(ptx::mul_f32x2(x[e], r2), dy[e], dg[c][e]);
+        const uint64_t u = ptx::mul_f32x2(dy[e], g[e]);
+        su2 = ptx::add_f32x2(su2, u);
+        sux2 = ptx::fma_f32x2(u, x[e], sux2);
+      }
+    }
+    float su = ptx::sum_f32x2(su2), sux = ptx::sum_f32x2(sux2);
+    cta_sum2(su, sux, buf + (i & 1) * warps, warps);
+    if (t == 0 && i >= 1 && fetched < count) fetch(before);
+    if (p.y != nullptr) {
+      // dx = rstd u - rstd <u> - (x - mean) rstd^2 <u h>,  <u h> = rstd <u (x - mean)>
+      const uint64_t c0 = ptx::both_f32x2(-su * inv_d * rstd), c1 = ptx::both_f32x2(-(rstd * (rstd * sux * inv_d)) * rstd);
+      uint8_t* out = static_cast<uint8_t*>(p.y) + row * p.d * kSize;
+      col = 4 * t;
+#pragma unroll
+      for (int c = 0; c < kUnits; c++, col += 4 * threads) {
+        if (col >= p.d) continue;
+        uint64_t x[2], dy[2], g[2];
+        load_pairs<DT>(xs, col, x);
+        load_pairs<DT>(xs + row_bytes, col, dy);
+        if (wide) load_pairs<TVB_F32>(weights, col, g);
+        else load_pairs<DT>(weights, col, g);
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+          x[e] = ptx::fma_f32x2(ptx::add_f32x2(x[e], m2), c1, ptx::fma_f32x2(dy[e], ptx::mul_f32x2(g[e], r2), c0));
+        store_pairs<DT>(out, col, x);
+      }
+    }
+    mean = next_mean;
+    rstd = next_rstd;
+    row += step;
+    before = slot;
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  __syncthreads();
+  if (t == 0 && abort_flag != 0) atomicExch(status, 2);
+  if (p.partial == nullptr) return;
+  // the cluster's sums: each CTA leaves its own in shared memory (the ring is idle), and adds up half of the columns
+  float* sums = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int c = 0; c < kUnits; c++) {
+    const int col = (c * threads + t) * 4;
+    if (col >= p.d) continue;
+    store_pairs<TVB_F32>(sums, col, dg[c]);
+    store_pairs<TVB_F32>(sums, p.d + col, db[c]);
+  }
+  ptx::cluster_sync();
+  const uint32_t rank = ptx::cluster_ctarank();
+  float* out = p.partial + static_cast<int64_t>(blockIdx.x / kRingCluster) * 2 * p.d;
+  const int share = 2 * p.d / kRingCluster;
+  for (int e = t; e < share; e += threads) {
+    const int at = static_cast<int>(rank) * share + e;
+    float v = 0.0f;
+#pragma unroll
+    for (uint32_t r = 0; r < kRingCluster; r++) {
+      float w;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(ptx::mapa(ring0 + 4 * at, r)) : "memory");
+      v += w;
+    }
+    out[at] = v;
+  }
+  ptx::cluster_sync();  // no CTA's shared memory is released while another may read it
+}
+
 // Rows too long for the registers: dx in two passes over the row; the sums over the rows in a kernel of their own.
 template <int DT>
 __global__ void __launch_bounds__(1024) layer_norm_backward_long_kernel(const NormParams p) {
@@ -363,8 +704,8 @@ __global__ void __launch_bounds__(256) layer_norm_reduce_kernel(const float* par
   if (out != nullptr) store_float_rt(out, col < d ? col : col - d, param_dtype, s);
 }
 
-constexpr int kLongest = 32 * 1024;         // values of a row that the forward kernel keeps in registers
-constexpr int kLongestBwd = 16 * 1024;
+constexpr int kLongest = 32 * 1024;         // values of a row that the forward kernels keep in registers
+constexpr int kLongestBwd = 16 * 1024;      // and the plain backward kernel
 constexpr int64_t kLongSlices = 64;         // partial rows of layer_norm_columns_kernel, at most
 
 int norm_group(int64_t d, int vals) {
@@ -373,7 +714,31 @@ int norm_group(int64_t d, int vals) {
   return 1024;
 }
 
-// CTAs of the backward kernel (and partial rows of its sums).
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// The streamed backward kernel: rows of 512 to 16384 values that fit the shared memory at least twice; 1024 threads per SM, as
+// one CTA or several.
+struct Ring {
+  int threads, per_sm, stages;
+  size_t smem;
+};
+Ring ring_shape(int64_t d, int es, int weights_es) {
+  Ring r{};
+  if (d < 512 || d > 1024 * kRingCols || d % 4 != 0) return r;
+  r.threads = static_cast<int>(ceil_div(d, kRingCols * 32) * 32);
+  r.per_sm = std::min(1024 / r.threads, 16);
+  const int64_t rest = d * weights_es + r.threads / 2;  // weights, sums over the warps
+  // (228 KB per SM, of which every CTA takes 1 KB for itself and some for its barriers)
+  r.stages = static_cast<int>(std::min<int64_t>((228 * 1024 / r.per_sm - 1024 - 128 - rest) / (2 * d * es), 8));
+  if (r.stages < 2) return Ring{};
+  r.smem = static_cast<size_t>(std::max<int64_t>(r.stages * 2 * d * es + rest, 8 * d));  // (the sums of 2 d columns at the end)
+  return r;
+}
+
+// Its CTAs: whole clusters, at most what the GPU holds, no more than there are rows.
+int64_t ring_ctas(int64_t rows, const Ring& r) { return std::min(ceil_div(rows, kRingCluster) * kRingCluster, static_cast<int64_t>(148) * r.per_sm); }
+
+// CTAs of the plain backward kernel (and partial rows of its sums).
 int64_t norm_parts(int64_t rows, int64_t d) {
   if (d > kLongestBwd) return std::min<int64_t>(rows, kLongSlices);
   const int t = norm_group(d, kValsBwd);
@@ -382,15 +747,22 @@ int64_t norm_parts(int64_t rows, int64_t d) {
   return std::min(ceil_div(rows, groups), most);
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
+// The forward kernel's shape (bfloat16, us: 65536 x 768 with a warp per row 44, a CTA of 128 for two rows 76; 16384 x 4096 with 32 values
+// of one row per thread 54, 16 of two rows 56; 4096 x 16384: 93 and 77).
 template <int DT, int VEC>
 int forward_vec(cudaStream_t stream, const NormParams& p) {
-  const int t = norm_group(p.d, kVals);
-  const int64_t grid = t < 128 ? ceil_div(p.rows, 128 / t) : p.rows;
-  auto kernel = t == 8 ? layer_norm_kernel<DT, VEC, 8> : t == 32 ? layer_norm_kernel<DT, VEC, 32> : t == 128 ? layer_norm_kernel<DT, VEC, 128>
-              : t == 256 ? layer_norm_kernel<DT, VEC, 256> : t == 512 ? layer_norm_kernel<DT, VEC, 512> : layer_norm_kernel<DT, VEC, 1024>;
-  return launch_dependent("layer_norm", kernel, dim3(static_cast<unsigned>(grid)), dim3(t < 128 ? 128 : t), 0, stream, p);
+  auto run = [&](auto kernel, int t, int rows) {
+    const int64_t per_cta = (t < 128 ? 128 / t : 1) * rows;
+    return launch_dependent("layer_norm", kernel, dim3(static_cast<unsigned>(ceil_div(p.rows, per_cta))), dim3(t < 128 ? 128 : t), 0, stream, p);
+  };
+  if (p.d <= 16 * 8) return run(layer_norm_kernel<DT, VEC, 8, 16, 2>, 8, 2);
+  if (p.d <= 32 * 8) return run(layer_norm_kernel<DT, VEC, 8, 32, 1>, 8, 1);
+  if (p.d <= 32 * 32) return run(layer_norm_kernel<DT, VEC, 32, 32, 1>, 32, 1);
+  if (p.d <= 16 * 128) return run(layer_norm_kernel<DT, VEC, 128, 16, 2>, 128, 2);
+  if (p.d <= 32 * 128) return run(layer_norm_kernel<DT, VEC, 128, 32, 1>, 128, 1);
+  if (p.d <= 16 * 512) return run(layer_norm_kernel<DT, VEC, 512, 16, 2>, 512, 2);
+  if (p.d <= 16 * 1024) return run(layer_norm_kernel<DT, VEC, 1024, 16, 2>, 1024, 2);
+  return run(layer_norm_kernel<DT, VEC, 1024, 32, 1>, 1024, 1);
 }
 
 template <int DT, int VEC>
@@ -403,6 +775,20 @@ int backward_vec(cudaStream_t stream, const NormParams& p, int64_t parts) {
 }
 
 template <int DT>
+int backward_ring(int device, cudaStream_t stream, const NormParams& p, const Ring& r, int64_t ctas) {
+  auto kernel = layer_norm_backward_ring_kernel<DT>;
+  static bool configured[64] = {};
+  if (!configured[device & 63]) {
+    TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 128));
+    configured[device & 63] = true;
+  }
+  int* status = nullptr;
+  if (status_word(device, &status) != 0) return -1;
+  return launch_dependent_cluster("layer_norm_backward_ring", kernel, kRingCluster, dim3(static_cast<unsigned>(ctas)),
+                                  dim3(static_cast<unsigned>(r.threads)), r.smem, stream, p, r.stages, status);
+}
+
+template <int DT>
 int forward(cudaStream_t stream, const NormParams& p) {
   constexpr int kVec = DT == TVB_F32 ? 4 : 8;
   if (p.d > kLongest)
@@ -412,20 +798,28 @@ int forward(cudaStream_t stream, const NormParams& p) {
   return vec ? forward_vec<DT, kVec>(stream, p) : forward_vec<DT, 1>(stream, p);
 }
 
+// Queues the kernels of dx and of the partial sums; *parts receives the number of partial rows.
 template <int DT>
-int backward(cudaStream_t stream, const NormParams& p, int64_t parts) {
+int backward(int device, cudaStream_t stream, const NormParams& p, int64_t* parts) {
   constexpr int kVec = DT == TVB_F32 ? 4 : 8;
+  const bool vec = p.d % kVec == 0 && p.x_ld % kVec == 0 && p.dy_ld % kVec == 0 && aligned16(p.x) && aligned16(p.dy) &&
+                   aligned16(p.y) && aligned16(p.weight) && aligned16(p.partial);
+  const Ring ring = vec ? ring_shape(p.d, DT == TVB_F32 ? 4 : 2, p.param_dtype == TVB_F32 ? 4 : 2) : Ring{};
+  if (ring.stages != 0) {
+    const int64_t ctas = ring_ctas(p.rows, ring);
+    *parts = ctas / kRingCluster;
+    return backward_ring<DT>(device, stream, p, ring, ctas);
+  }
+  *parts = norm_parts(p.rows, p.d);
   if (p.d > kLongestBwd) {
     if (p.y != nullptr && launch_dependent("layer_norm_backward_long", layer_norm_backward_long_kernel<DT>,
                                            dim3(static_cast<unsigned>(p.rows)), dim3(1024), 0, stream, p) != 0)
       return -1;
     if (p.partial == nullptr) return 0;
     return launch_dependent("layer_norm_columns", layer_norm_columns_kernel<DT>,
-                            dim3(static_cast<unsigned>(ceil_div(p.d, 256)), static_cast<unsigned>(parts)), dim3(256), 0, stream, p);
+                            dim3(static_cast<unsigned>(ceil_div(p.d, 256)), static_cast<unsigned>(*parts)), dim3(256), 0, stream, p);
   }
-  const bool vec = p.d % kVec == 0 && p.x_ld % kVec == 0 && p.dy_ld % kVec == 0 && aligned16(p.x) && aligned16(p.dy) &&
-                   aligned16(p.y) && aligned16(p.weight);
-  return vec ? backward_vec<DT, kVec>(stream, p, parts) : backward_vec<DT, 1>(stream, p, parts);
+  return vec ? backward_vec<DT, kVec>(stream, p, *parts) : backward_vec<DT, 1>(stream, p, *parts);
 }
 
 int check_sizes(const char* fn, int dtype, int param_dtype, int64_t rows, int64_t d) {
@@ -467,7 +861,9 @@ extern "C" int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm
 
 extern "C" uint64_t tvb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d) {
   if (rows <= 0 || d <= 0) return 0;
-  return static_cast<uint64_t>(norm_parts(rows, d)) * 2 * static_cast<uint64_t>(d) * 4;
+  const Ring ring = ring_shape(d, 2, 2);  // (wider rows take as many CTAs or none)
+  const int64_t most = std::max(norm_parts(rows, d), ring.stages != 0 ? ring_ctas(rows, ring) / kRingCluster : 0);
+  return static_cast<uint64_t>(most) * 2 * static_cast<uint64_t>(d) * 4;
 }
 
 extern "C" int tvb_layer_norm_backward(int device, const void* dy, int dtype, int64_t dy_sm, const void* x, int64_t x_sm,
@@ -503,10 +899,11 @@ extern "C" int tvb_layer_norm_backward(int device, const void* dy, int dtype, in
   p.x_ld = rows > 1 ? x_sm : d;
   p.dy_ld = rows > 1 ? dy_sm : d;
   p.rows = rows; p.d = static_cast<int>(d); p.param_dtype = param_dtype;
-  const int64_t parts = rows > 0 ? norm_parts(rows, d) : 0;
+  int64_t parts = 0;
   if (rows > 0) {
-    const int rc = dtype == TVB_F32 ? backward<TVB_F32>(stream, p, parts) : dtype == TVB_F16 ? backward<TVB_F16>(stream, p, parts)
-                                                                                               : backward<TVB_BF16>(stream, p, parts);
+    const int rc = dtype == TVB_F32   ? backward<TVB_F32>(device, stream, p, &parts)
+                   : dtype == TVB_F16 ? backward<TVB_F16>(device, stream, p, &parts)
+                                      : backward<TVB_BF16>(device, stream, p, &parts);
     if (rc != 0) return -1;
   }
   if (!sums) return 0;

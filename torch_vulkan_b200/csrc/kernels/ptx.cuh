@@ -232,6 +232,22 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return d;
 }
 
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// The same value in both halves.
+__device__ __forceinline__ uint64_t both_f32x2(float v) { return pack_f32x2(__float_as_uint(v), __float_as_uint(v)); }
+
+// The sum of the two halves.
+__device__ __forceinline__ float sum_f32x2(uint64_t v) {
+  float lo, hi;
+  unpack_f32x2(v, lo, hi);
+  return lo + hi;
+}
+
 // ---------------------------------------------------------------- tcgen05 / tensor memory
 
 // One full warp allocates `cols` (a power of two >= 32) TMEM columns; the base address lands in shared memory.
