@@ -112,31 +112,64 @@ def test_wrappers_refuse_what_they_cannot_pass_on():
             bad()
 
 
-@pytest.mark.parametrize("tiles,blocks,pairs", [((128, 896), (224, 32), 74), ((5, 40), (100, 7), 74), ((74, 74), (64, 64), 74), ((75, 3), (9, 9), 74),
-                                                ((1, 1), (3, 2), 2), ((500, 0), (8, 1), 74), ((30, 2000), (64, 3), 74), ((148, 10), (16, 16), 74)])
-def test_the_schedule_of_two_products_covers_every_tile_once(tiles, blocks, pairs):
-    """The same formulas as PairSchedule (csrc/kernels/linear_pair.cu): every tile of both products is one pair's, and no pair has
-    more than one tile's worth of work above an even share when there are tiles enough."""
+@pytest.mark.parametrize("sizes,blocks,pairs", [(((2048, 4096), (14336, 4096)), (224, 32), 74), (((0, 0), (2048, 14336)), (0, 64), 74),
+                                                (((300, 600), (5000, 1100)), (100, 7), 74), (((1000, 1000), (1000, 1024)), (16, 16), 74),
+                                                (((513, 257), (511, 255)), (3, 2), 2), (((9000, 900), (700, 9000)), (9, 9), 74),
+                                                (((0, 0), (257, 300)), (0, 5), 74), (((2049, 2049), (8200, 2100)), (33, 32), 74)])
+def test_the_schedule_of_two_products_covers_every_output_once(sizes, blocks, pairs):
+    """The same formulas as PairSchedule and pair_run (csrc/kernels/linear_pair.cu): tiles of 512 rows x 256 columns, the last
+    ones cut; every 256 x 128 piece of both outputs belongs to one pair."""
+    def up(a, b):
+        return -(-a // b)
+
+    tj, ti = [up(j, 512) for j, _ in sizes], [up(i, 256) for _, i in sizes]
+    tiles = [a * b for a, b in zip(tj, ti)]
     a, b = blocks
-    extra = light_first = 0
-    rest = tiles[0] % pairs
-    if tiles[1] and rest:
+    extra = light_first = light = 0
+    if tiles[0] % pairs:
+        light = pairs - tiles[0] % pairs
         extra = (2 * a + b) // (2 * b)
         light_first = extra * b < a
-    light = pairs - rest if rest else 0
+    early = min(light * extra, tiles[1])
+    rest = (tiles[1] - early) % pairs
+    half, quarter = up(2 * rest, pairs) * 32, up(4 * rest, pairs) * 24
+    cut, whole = 256, tiles[1]
+    if rest and min(half, quarter) < 48:
+        whole -= rest
+        cut = 256 if half <= quarter else 128
+    pairs = min(pairs, tiles[0] + whole + (tiles[1] - whole) * (512 // cut))
+
+    def place(product, index):
+        band, r = divmod(index, 8 * ti[product])
+        rows = min(8, tj[product] - band * 8)
+        row, col = (band * 8 + r % rows) * 512, r // rows * 256
+        return row, col, 256, 2 if row + 256 < sizes[product][0] else 1
+
+    heavy = tiles[0] % pairs
+    light = pairs - heavy if heavy else 0
     early = light * extra
-    seen, loads = set(), []
+    seen = set()
     for pair in range(pairs):
-        mine = [(0, t) for t in range(pair, tiles[0], pairs)]
-        is_light = rest != 0 and pair >= rest
-        rank = pair - rest if is_light else pair
+        is_light = heavy != 0 and pair >= heavy
+        rank = pair - heavy if is_light else pair
+        order = (rank if is_light else pairs - heavy + pair) if heavy and light_first else pair
+        mine = [(0, *place(0, t)) for t in range(pair, tiles[0], pairs)]
         if is_light:
-            mine += [(1, t) for t in range(rank, min(early, tiles[1]), light)]
-        order = (rank if is_light else light + pair) if rest and light_first else pair
-        mine += [(1, t) for t in range(early + order, tiles[1], pairs)]
-        assert not seen & set(mine)
-        seen |= set(mine)
-        loads.append(sum(blocks[p] for p, _ in mine))
-    assert len(seen) == sum(tiles)
-    if tiles[1] >= 2 * early:
-        assert max(loads) <= sum(t * c for t, c in zip(tiles, blocks)) / pairs + 2 * b
+            mine += [(1, *place(1, t)) for t in range(rank, min(early, whole), light)]
+        mine += [(1, *place(1, t)) for t in range(early + order, whole, pairs)]
+        per_half = 256 // cut
+        for at in range(order, (tiles[1] - whole) * 2 * per_half, pairs):
+            row, col, _, _ = place(1, whole + at // (2 * per_half))
+            sub = at % (2 * per_half)
+            row, col = row + sub // per_half * 256, col + sub % per_half * cut
+            if row < sizes[1][0] and col < sizes[1][1]:
+                mine.append((1, row, col, cut, 1))
+        for product, row, col, cols, halves in mine:
+            for r in range(row, row + 256 * halves, 256):
+                for c in range(col, col + cols, 128):
+                    assert (product, r, c) not in seen
+                    seen.add((product, r, c))
+    for product, (j, i) in enumerate(sizes):
+        for r in range(0, j, 256):
+            for c in range(0, i, 128):
+                assert (product, r, c) in seen, (product, r, c)

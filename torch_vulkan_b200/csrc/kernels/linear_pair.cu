@@ -1,14 +1,18 @@
 // The 16-bit products of linear.h on tcgen05 when the output is large: bound by the tensor pipe.
 //
-// A cluster of two CTAs (the two SMs of a TPC) walks output tiles of 256 rows (j) x BN columns (i), BN a multiple of 32 up to 256.
-// Each CTA stages 128 rows of Q and BN / 2 rows of P per 64 values of r; one lane of CTA 0 issues tcgen05.mma.cta_group::2 for
-// both, and each CTA's TMEM receives its own 128 rows of the tile, in two buffers, so that a tile is read back under the next
-// tile's MMAs. BN is 256 unless narrower tiles put more pairs to work.
+// A cluster of two CTAs (the two SMs of a TPC) walks output tiles of 512 rows (j) x 256 columns (i): per 64 values of r each CTA
+// stages 256 rows of Q (two halves of 128) and 128 rows of P, 48 KB, and one lane of CTA 0 issues tcgen05.mma.cta_group::2 for both:
+// one instruction multiplies a half of both CTAs (256 rows) by the 256 columns. What paces such a kernel is the L2: with tiles of
+// 256 x 256 (32 KB per SM for half the work) every SM asks for a third more bytes per multiplication, and the steps took 690 clocks
+// where the tensor core needs 512. The two halves' sums fill the tensor memory, so a tile is read back while the halves are out of
+// step: the last steps of a tile multiply half 0 first, and the first steps of the next tile do too.
+// Tiles that do not fill a round of pairs are cut into smaller ones (256 rows, 256 or 128 columns), and so is a tile whose
+// second half lies beyond the last row.
 //
 // A launch takes one product or two: the backward pass multiplies dz by w and by x at once. The tiles of the product with the
 // longer r come first; pairs that get one tile of it less than others start on the second product meanwhile, and the rest of its
 // tiles are dealt out in turn. The schedule is computed from the sizes alone (no counters in memory), so launches share nothing.
-//   warps 0-7: epilogue (warp w reads TMEM lanes 32 (w % 4) ..., half w / 4 of the columns)
+//   warps 0-7: epilogue (warp w reads TMEM lanes 32 (w % 4) ..., every second 32 columns)
 //   warp 8, one lane: TMA; warp 9, one lane of CTA 0: MMA. All mbarrier waits are bounded.
 #include <cuda.h>
 
@@ -24,80 +28,106 @@
 namespace tvb {
 namespace {
 
-constexpr int kTileJ = 256, kRowsQ = 128, kStepR = 64;
-constexpr int kStageQ = kRowsQ * 128, kStageP = 128 * 128, kStage = kStageQ + kStageP, kStages = 6;
+constexpr int kHalfJ = 256, kTileJ = 2 * kHalfJ, kTileI = 256, kRowsQ = 128, kStepR = 64;
+constexpr int kBoxQ = kRowsQ * 128;  // bytes of one half's rows of Q in a stage
+constexpr int kStage = 2 * kBoxQ + 128 * 128, kStages = 4;
 constexpr int kEpiWarps = 8, kProducer = 8, kMma = 9, kThreads = 320, kTmemCols = 512;
 constexpr int kSmemBytes = kStages * kStage + 1024 + 256;
-constexpr int kBand = 16;  // tile rows per band of the tile order
+constexpr int kBand = 8;    // tile rows per band of the tile order
+constexpr int kAhead = 4;   // steps that half 0 is ahead at the beginning of a tile (at most kStages)
+constexpr int kBehind = 2;  // and at its end
 
 struct PairProduct {
-  CUtensorMap map_q, map_p;
+  CUtensorMap map_q, map_p;  // boxes of 64 values of r x 128 (Q) or 64 (P) rows, or 64 x 64 where r is not contiguous
   const void* bias;
   const void* residual;
   void* out;
   void* preact;
   int64_t residual_ld;
-  int I, J, blocks, tiles, tiles_i, tiles_j, bn, q_mn, p_mn, activation, vector_ok;
-  uint32_t idesc, stage_bytes;
+  int I, J, blocks, tiles, tiles_i, tiles_j, q_mn, p_mn, activation, vector_ok;
+  uint32_t fmt;  // instruction descriptor without the columns
 };
 
+// Product 0 may be empty (tiles == 0): a launch of one product has it as product 1.
 struct PairParams {
   PairProduct prod[2];
   int extra;        // tiles of product 1 that a pair with fewer tiles of product 0 takes first
   int light_first;  // which pairs come first when the rest of product 1 is dealt out
+  int whole;        // tiles of product 1 that are not cut; the others become cut tiles of 256 rows x cut_cols columns
+  int cut_cols;
   int* status;
 };
 
-// Walks the tiles of one pair: its tiles of product 0, its share of product 1.
-struct PairSchedule {
-  int pair, pairs, tile, heavy, is_light, rank_among, stage_of;
-  __device__ PairSchedule(const PairParams& p, int pair_, int pairs_) : pair(pair_), pairs(pairs_) {
-    const int rest = p.prod[0].tiles % pairs;
-    heavy = rest;                       // pairs 0 ... rest - 1 have one tile of product 0 more than the others
-    is_light = rest != 0 && pair >= rest;
-    rank_among = is_light ? pair - rest : pair;
-    stage_of = 0;
-    tile = pair;
-  }
-  // The next tile: which product, its index; false at the end.
-  __device__ bool next(const PairParams& p, int& product, int& index) {
-    if (stage_of == 0) {
-      if (tile < p.prod[0].tiles) {
-        product = 0;
-        index = tile;
-        tile += pairs;
-        return true;
-      }
-      stage_of = 1;
-      tile = rank_among;
-    }
-    product = 1;
-    const int light = heavy != 0 ? pairs - heavy : 0, early = light * p.extra;
-    if (stage_of == 1) {
-      if (is_light && tile < early && tile < p.prod[1].tiles) {
-        index = tile;
-        tile += light;
-        return true;
-      }
-      stage_of = 2;
-      int order = pair;
-      if (heavy != 0 && p.light_first) order = is_light ? rank_among : light + pair;
-      tile = early + order;
-    }
-    if (tile >= p.prod[1].tiles) return false;
-    index = tile;
-    tile += pairs;
-    return true;
-  }
+struct PairTile {
+  int product, row, col, cols, halves;
 };
 
-__device__ __forceinline__ void pair_tile_coords(const PairProduct& d, int tile, int& tj, int& ti) {
-  const int per_band = kBand * d.tiles_i, b = tile / per_band, first = b * kBand;
-  const int rows = d.tiles_j - first < kBand ? d.tiles_j - first : kBand;
-  const int r = tile - b * per_band;
-  tj = first + r % rows;
-  ti = r / rows;
-}
+// Walks the tiles of one pair: its tiles of product 0, its share of product 1, its share of what was cut.
+struct PairSchedule {
+  int pair, pairs, at, heavy, rank_among, order, stage;
+  bool is_light;
+  __device__ PairSchedule(const PairParams& p, int pair_, int pairs_) : pair(pair_), pairs(pairs_) {
+    heavy = p.prod[0].tiles % pairs;  // pairs 0 ... heavy - 1 have one tile of product 0 more than the others
+    is_light = heavy != 0 && pair >= heavy;
+    rank_among = is_light ? pair - heavy : pair;
+    order = heavy != 0 && p.light_first ? (is_light ? rank_among : pairs - heavy + pair) : pair;
+    stage = 0;
+    at = pair;
+  }
+  __device__ static void place(const PairProduct& d, int index, PairTile& t) {
+    const int per_band = kBand * d.tiles_i, b = index / per_band, first = b * kBand;
+    const int rows = d.tiles_j - first < kBand ? d.tiles_j - first : kBand;
+    const int r = index - b * per_band;
+    t.row = (first + r % rows) * kTileJ;
+    t.col = r / rows * kTileI;
+    t.cols = kTileI;
+    t.halves = t.row + kHalfJ < d.J ? 2 : 1;
+  }
+  __device__ bool next(const PairParams& p, PairTile& t) {
+    const int light = heavy != 0 ? pairs - heavy : 0, early = light * p.extra;
+    for (;;) {
+      if (stage == 0) {
+        if (at < p.prod[0].tiles) {
+          t.product = 0;
+          place(p.prod[0], at, t);
+          at += pairs;
+          return true;
+        }
+        stage = 1;
+        at = rank_among;
+      }
+      t.product = 1;
+      if (stage == 1) {
+        if (is_light && at < early && at < p.whole) {
+          place(p.prod[1], at, t);
+          at += light;
+          return true;
+        }
+        stage = 2;
+        at = early + order;
+      }
+      if (stage == 2) {
+        if (at < p.whole) {
+          place(p.prod[1], at, t);
+          at += pairs;
+          return true;
+        }
+        stage = 3;
+        at = order;
+      }
+      const int per_half = kTileI / p.cut_cols, per_tile = 2 * per_half;
+      const int index = p.whole + at / per_tile, sub = at % per_tile;
+      if (index >= p.prod[1].tiles) return false;
+      at += pairs;
+      place(p.prod[1], index, t);
+      t.row += sub / per_half * kHalfJ;
+      t.col += sub % per_half * p.cut_cols;
+      t.cols = p.cut_cols;
+      t.halves = 1;
+      if (t.row < p.prod[1].J && t.col < p.prod[1].I) return true;  // (a cut tile may lie outside altogether)
+    }
+  }
+};
 
 __device__ __forceinline__ void activate32(float (&v)[32], int act) {
   switch (act) {
@@ -211,37 +241,38 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
   ptx::grid_launch_dependents();
 
   PairSchedule sched(p, pair, pairs);
-  int which, tile;
+  PairTile t;
   if (warp == kProducer) {
     if (lane == 0) {
       long long it = 0;
       bool ok = true;
-      while (ok && sched.next(p, which, tile)) {
-        const PairProduct& d = p.prod[which];
-        int tj, ti;
-        pair_tile_coords(d, tile, tj, ti);
-        const int row_q = tj * kTileJ + static_cast<int>(rank) * kRowsQ, half = d.bn >> 1;
-        const int row_p = ti * d.bn + static_cast<int>(rank) * half;
-        const bool p_two = half > 64;  // (an MN-major operand comes in boxes of 64 columns)
+      while (ok && sched.next(p, t)) {
+        const PairProduct& d = p.prod[t.product];
+        const int row_q = t.row + static_cast<int>(rank) * kRowsQ, boxes_p = t.cols >> 7;
+        const int row_p = t.col + static_cast<int>(rank) * (t.cols >> 1);
+        const uint32_t bytes = 2u * (t.halves * kBoxQ + boxes_p * 8192);  // both CTAs' boxes of a stage
         for (int kb = 0; kb < d.blocks; kb++, it++) {
           const int s = static_cast<int>(it % kStages);
           ok = ptx::mbar_wait(empty0 + 8 * s, static_cast<uint32_t>((it / kStages) & 1) ^ 1u, abort_flag);
           if (!ok) break;
           const uint32_t dst = base + s * kStage;
-          if (rank == 0) ptx::mbar_expect_tx(full0 + 8 * s, 2 * d.stage_bytes);  // both CTAs' boxes of this stage
+          if (rank == 0) ptx::mbar_expect_tx(full0 + 8 * s, bytes);
           const uint32_t bar = ptx::mapa(full0 + 8 * s, 0);
           const int r = kb * kStepR;
-          if (d.q_mn) {
-            ptx::tma_load_2d_pair(dst, &d.map_q, row_q, r, bar);
-            ptx::tma_load_2d_pair(dst + 8192, &d.map_q, row_q + 64, r, bar);
-          } else {
-            ptx::tma_load_2d_pair(dst, &d.map_q, r, row_q, bar);
+          for (int h = 0; h < t.halves; h++) {
+            const uint32_t at = dst + h * kBoxQ;
+            const int row = row_q + h * kHalfJ;
+            if (d.q_mn) {
+              ptx::tma_load_2d_pair(at, &d.map_q, row, r, bar);
+              ptx::tma_load_2d_pair(at + 8192, &d.map_q, row + 64, r, bar);
+            } else {
+              ptx::tma_load_2d_pair(at, &d.map_q, r, row, bar);
+            }
           }
-          if (d.p_mn) {
-            ptx::tma_load_2d_pair(dst + kStageQ, &d.map_p, row_p, r, bar);
-            if (p_two) ptx::tma_load_2d_pair(dst + kStageQ + 8192, &d.map_p, row_p + 64, r, bar);
-          } else {
-            ptx::tma_load_2d_pair(dst + kStageQ, &d.map_p, r, row_p, bar);
+          for (int c = 0; c < boxes_p; c++) {
+            const uint32_t at = dst + 2 * kBoxQ + c * 8192;
+            if (d.p_mn) ptx::tma_load_2d_pair(at, &d.map_p, row_p + 64 * c, r, bar);
+            else ptx::tma_load_2d_pair(at, &d.map_p, r, row_p + 64 * c, bar);
           }
         }
       }
@@ -258,57 +289,115 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
   } else if (warp == kMma) {
     if (lane == 0 && rank == 0) {
       long long it = 0;
-      int n = 0;
+      uint32_t used0 = 0, used1 = 0;  // tiles (or halves) that each buffer of sums has held
+      int turn = 0;
       bool ok = true;
-      for (; ok && sched.next(p, which, tile); n++) {
-        const PairProduct& d = p.prod[which];
-        const int acc = n & 1;
-        ok = ptx::mbar_wait(tempty0 + 8 * acc, static_cast<uint32_t>((n >> 1) & 1) ^ 1u, abort_flag);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
+      while (ok && sched.next(p, t)) {
+        const PairProduct& d = p.prod[t.product];
         const uint64_t step_q = d.q_mn ? 128 : 2, step_p = d.p_mn ? 128 : 2;
-        for (int kb = 0; kb < d.blocks; kb++, it++) {
-          const int s = static_cast<int>(it % kStages);
-          ok = ptx::mbar_wait(full0 + 8 * s, static_cast<uint32_t>((it / kStages) & 1), abort_flag);
-          if (!ok) break;
+        const uint32_t idesc = d.fmt | (static_cast<uint32_t>(t.cols >> 3) << 17);
+        auto wait_full = [&](long long i) {
+          const bool there = ptx::mbar_wait(full0 + 8 * static_cast<int>(i % kStages), static_cast<uint32_t>((i / kStages) & 1), abort_flag);
           ptx::tc_fence_after();
-          const uint32_t at = base + s * kStage;
-          uint64_t qd = d.q_mn ? ptx::tc_smem_desc_sw128_mn(at) : ptx::tc_smem_desc_sw128(at);
-          uint64_t pd = d.p_mn ? ptx::tc_smem_desc_sw128_mn(at + kStageQ) : ptx::tc_smem_desc_sw128(at + kStageQ);
+          return there;
+        };
+        auto free_buffer = [&](int b) {
+          const bool there = ptx::mbar_wait(tempty0 + 8 * b, ((b ? used1 : used0) & 1u) ^ 1u, abort_flag);
+          ptx::tc_fence_after();
+          if (b) used1++;
+          else used0++;
+          return there;
+        };
+        auto multiply = [&](long long i, int half, int buffer, bool first) {
+          const uint32_t at_q = base + static_cast<int>(i % kStages) * kStage + half * kBoxQ;
+          const uint32_t at_p = base + static_cast<int>(i % kStages) * kStage + 2 * kBoxQ;
+          uint64_t qd = d.q_mn ? ptx::tc_smem_desc_sw128_mn(at_q) : ptx::tc_smem_desc_sw128(at_q);
+          uint64_t pd = d.p_mn ? ptx::tc_smem_desc_sw128_mn(at_p) : ptx::tc_smem_desc_sw128(at_p);
 #pragma unroll
           for (int j = 0; j < kStepR / 16; j++) {
-            ptx::tc_mma_pair<2>(d_tmem, qd, pd, d.idesc, (kb | j) != 0 ? 1u : 0u);
+            ptx::tc_mma_pair<2>(tmem_base + static_cast<uint32_t>(buffer * 256), qd, pd, idesc, first && j == 0 ? 0u : 1u);
             qd += step_q;
             pd += step_p;
           }
-          ptx::tc_commit_pair(empty0 + 8 * s);  // frees the stage in both CTAs
+        };
+        auto release = [&](long long i) { ptx::tc_commit_pair(empty0 + 8 * static_cast<int>(i % kStages)); };  // in both CTAs
+        if (t.halves == 1) {
+          ok = free_buffer(turn);
+          for (int kb = 0; ok && kb < d.blocks; kb++, it++) {
+            ok = wait_full(it);
+            if (!ok) break;
+            multiply(it, 0, turn, kb == 0);
+            release(it);
+          }
+          if (ok) ptx::tc_commit_pair(tfull0 + 8 * turn);
+          turn ^= 1;
+          continue;
         }
-        if (ok) ptx::tc_commit_pair(tfull0 + 8 * acc);
+        // two halves: half 0 ahead at the beginning (its buffer is read back first), and again at the end
+        const int ahead = d.blocks < kAhead ? d.blocks : kAhead;
+        const int behind = d.blocks - ahead < kBehind ? d.blocks - ahead : kBehind;
+        ok = free_buffer(0);
+        for (int kb = 0; ok && kb < ahead; kb++) {
+          ok = wait_full(it + kb);
+          if (ok) multiply(it + kb, 0, 0, kb == 0);
+        }
+        if (ok && behind == 0) ptx::tc_commit_pair(tfull0);
+        ok = ok && free_buffer(1);
+        for (int kb = 0; ok && kb < ahead; kb++) {
+          multiply(it + kb, 1, 1, kb == 0);
+          release(it + kb);
+        }
+        it += ahead;
+        for (int kb = ahead; ok && kb < d.blocks - behind; kb++, it++) {
+          ok = wait_full(it);
+          if (!ok) break;
+          multiply(it, 0, 0, false);
+          multiply(it, 1, 1, false);
+          release(it);
+        }
+        if (ok && behind != 0) {
+          for (int kb = 0; ok && kb < behind; kb++) {
+            ok = wait_full(it + kb);
+            if (ok) multiply(it + kb, 0, 0, false);
+          }
+          if (ok) ptx::tc_commit_pair(tfull0);
+          for (int kb = 0; ok && kb < behind; kb++) {
+            multiply(it + kb, 1, 1, false);
+            release(it + kb);
+          }
+          it += behind;
+        }
+        if (ok) ptx::tc_commit_pair(tfull0 + 8);
       }
     }
     __syncwarp();
   } else {
-    int n = 0;
-    for (; sched.next(p, which, tile); n++) {
-      const PairProduct& d = p.prod[which];
-      int tj, ti;
-      pair_tile_coords(d, tile, tj, ti);
-      const int acc = n & 1;
-      if (!ptx::mbar_wait(tfull0 + 8 * acc, static_cast<uint32_t>((n >> 1) & 1), abort_flag)) break;
-      ptx::tc_fence_after();
-      const int64_t row = static_cast<int64_t>(tj) * kTileJ + rank * kRowsQ + (warp & 3) * 32 + lane;
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(acc * 256);
+    uint32_t used0 = 0, used1 = 0;
+    int turn = 0;
+    bool ok = true;
+    while (ok && sched.next(p, t)) {
+      const PairProduct& d = p.prod[t.product];
+      for (int h = 0; h < t.halves; h++) {
+        const int b = t.halves == 2 ? h : turn;
+        ok = ptx::mbar_wait(tfull0 + 8 * b, (b ? used1 : used0) & 1u, abort_flag);
+        if (b) used1++;
+        else used0++;
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const int64_t row = static_cast<int64_t>(t.row) + h * kHalfJ + rank * kRowsQ + (warp & 3) * 32 + lane;
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(b * 256);
 #pragma unroll 1
-      for (int c = (warp >> 2) * 32; c < d.bn; c += 64) {
-        uint32_t r[32];
-        ptx::tmem_ld_32x32(taddr + c, r);
-        ptx::tmem_ld_wait();
-        finish32<BF16>(d, row, ti * d.bn + c, r);
+        for (int c = (warp >> 2) * 32; c < t.cols; c += 64) {
+          uint32_t r[32];
+          ptx::tmem_ld_32x32(taddr + c, r);
+          ptx::tmem_ld_wait();
+          finish32<BF16>(d, row, t.col + c, r);
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa(tempty0 + 8 * b, 0));
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa(tempty0 + 8 * acc, 0));
+      if (t.halves == 1) turn ^= 1;
     }
   }
   ptx::tc_fence_before();
@@ -356,10 +445,9 @@ int max_pairs(int device, int* out) {
   return 0;
 }
 
-int pair_product(const LinearProduct& lp, int bn, PairProduct* d) {
-  const int half = bn / 2;
+int pair_product(const LinearProduct& lp, PairProduct* d) {
   if (operand_map(&d->map_q, lp.q, lp.dtype, lp.q_mn, lp.J, lp.R, lp.q_mn ? lp.q_sr : lp.q_sj, kRowsQ) != 0 ||
-      operand_map(&d->map_p, lp.p, lp.dtype, lp.p_mn, lp.I, lp.R, lp.p_mn ? lp.p_sr : lp.p_si, half) != 0)
+      operand_map(&d->map_p, lp.p, lp.dtype, lp.p_mn, lp.I, lp.R, lp.p_mn ? lp.p_sr : lp.p_si, 64) != 0)
     return -1;
   d->bias = lp.bias;
   d->residual = lp.residual;
@@ -369,11 +457,10 @@ int pair_product(const LinearProduct& lp, int bn, PairProduct* d) {
   d->I = static_cast<int>(lp.I);
   d->J = static_cast<int>(lp.J);
   d->blocks = static_cast<int>(ceil_div(lp.R, kStepR));
-  d->tiles_i = static_cast<int>(ceil_div(lp.I, bn));
+  d->tiles_i = static_cast<int>(ceil_div(lp.I, kTileI));
   d->tiles_j = static_cast<int>(ceil_div(lp.J, kTileJ));
-  TVB_REQUIRE(static_cast<int64_t>(d->tiles_i) * d->tiles_j < (int64_t(1) << 30), "tvb_linear: too many output tiles");
+  TVB_REQUIRE(static_cast<int64_t>(d->tiles_i) * d->tiles_j < (int64_t(1) << 28), "tvb_linear: too many output tiles");
   d->tiles = d->tiles_i * d->tiles_j;
-  d->bn = bn;
   d->q_mn = lp.q_mn;
   d->p_mn = lp.p_mn;
   d->activation = lp.activation;
@@ -381,26 +468,8 @@ int pair_product(const LinearProduct& lp, int bn, PairProduct* d) {
                         reinterpret_cast<uintptr_t>(lp.residual);
   d->vector_ok = (all & 15u) == 0 && lp.I % 8 == 0 && (lp.residual == nullptr || lp.residual_ld % 8 == 0);
   const uint32_t fmt = lp.dtype == TVB_BF16 ? 1 : 0;
-  d->idesc = ptx::tc_instr_desc(1, fmt, fmt, kTileJ, bn) | (lp.q_mn ? ptx::kTcAMajorMN : 0u) | (lp.p_mn ? ptx::kTcBMajorMN : 0u);
-  d->stage_bytes = kStageQ + (lp.p_mn ? (half > 64 ? 16384 : 8192) : half * 128);
+  d->fmt = ptx::tc_instr_desc(1, fmt, fmt, kHalfJ, 0) | (lp.q_mn ? ptx::kTcAMajorMN : 0u) | (lp.p_mn ? ptx::kTcBMajorMN : 0u);
   return 0;
-}
-
-// Columns per tile for a product alone in its launch. A step of a tile costs its SM 128 rows of Q and bn / 2 of P from the L2,
-// which is what paces it (7 rounds of 256 columns: 215 us; 7 of 224: 218; 9 of 192: 249), so narrower tiles pay only where
-// they fill SMs that would have none.
-int pair_columns(const LinearProduct& lp, int pairs) {
-  int best = 256;
-  int64_t best_cost = -1;
-  for (int bn = 256; bn >= 128; bn -= 32) {
-    const int64_t tiles = ceil_div(lp.I, bn) * ceil_div(lp.J, kTileJ);
-    const int64_t cost = ceil_div(tiles, pairs) * (256 + bn);
-    if (best_cost < 0 || cost * 10 < best_cost * 9) {
-      best = bn;
-      best_cost = cost;
-    }
-  }
-  return best;
 }
 
 template <bool BF16>
@@ -408,19 +477,30 @@ int pair_run(int device, cudaStream_t stream, const LinearProduct* lp, int count
   int pairs = 0;
   if (max_pairs<BF16>(device, &pairs) != 0) return -1;
   PairParams p{};
-  if (count == 2 && lp[0].R < lp[1].R) {
-    const LinearProduct swapped[2] = {lp[1], lp[0]};
-    return pair_run<BF16>(device, stream, swapped, 2);
-  }
-  for (int k = 0; k < count; k++)
-    if (pair_product(lp[k], count == 1 ? pair_columns(lp[k], pairs) : 256, &p.prod[k]) != 0) return -1;
-  pairs = std::min(pairs, p.prod[0].tiles + p.prod[1].tiles);
-  if (count == 2 && p.prod[0].tiles % pairs != 0) {
+  const bool swap = count == 2 && lp[0].R < lp[1].R;  // the longer r first
+  if (count == 2 && pair_product(lp[swap ? 1 : 0], &p.prod[0]) != 0) return -1;
+  if (pair_product(lp[count == 2 && !swap ? 1 : 0], &p.prod[1]) != 0) return -1;
+  int light = 0;
+  if (p.prod[0].tiles % pairs != 0) {
     const int a = p.prod[0].blocks, b = p.prod[1].blocks;
+    light = pairs - p.prod[0].tiles % pairs;
     p.extra = (2 * a + b) / (2 * b);  // a / b, rounded
     p.light_first = p.extra * b < a;
   }
+  // Tiles of product 1 beyond whole rounds of pairs: a round of tiles as they are, or rounds of smaller ones. Relative costs of a
+  // step (512, 256 rows x 256 columns, 256 x 128), by the bytes an SM stages: 48, 32 and 24 KB.
+  const int early = std::min(light * p.extra, p.prod[1].tiles), rest = (p.prod[1].tiles - early) % pairs;
+  const int64_t tall = 48, half = ceil_div(2 * rest, pairs) * 32, quarter = ceil_div(4 * rest, pairs) * 24;
+  p.cut_cols = kTileI;
+  p.whole = p.prod[1].tiles;
+  if (rest != 0 && std::min(half, quarter) < tall) {
+    p.whole -= rest;
+    p.cut_cols = half <= quarter ? kTileI : kTileI / 2;
+  }
   if (status_word(device, &p.status) != 0) return -1;
+  const int per_cut = 2 * kTileI / p.cut_cols;
+  const int64_t tiles = static_cast<int64_t>(p.prod[0].tiles) + p.whole + static_cast<int64_t>(p.prod[1].tiles - p.whole) * per_cut;
+  pairs = static_cast<int>(std::min<int64_t>(pairs, tiles));
   return launch_dependent_cluster("linear_pair", linear_pair_kernel<BF16>, 2, dim3(2 * static_cast<unsigned>(pairs)), dim3(kThreads), kSmemBytes,
                                   stream, p);
 }
