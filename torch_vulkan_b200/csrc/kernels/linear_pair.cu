@@ -4,8 +4,9 @@
 // stages 256 rows of Q (two halves of 128) and 128 rows of P, 48 KB, and one lane of CTA 0 issues tcgen05.mma.cta_group::2 for both:
 // one instruction multiplies a half of both CTAs (256 rows) by the 256 columns. What paces such a kernel is the L2: with tiles of
 // 256 x 256 (32 KB per SM for half the work) every SM asks for a third more bytes per multiplication, and the steps took 690 clocks
-// where the tensor core needs 512. The two halves' sums fill the tensor memory, so a tile is read back while the halves are out of
-// step: the last steps of a tile multiply half 0 first, and the first steps of the next tile do too.
+// where the tensor core needs 512. The two halves' sums fill the tensor memory, so a tile's read-back is not overlapped; it is kept
+// short by leaving through shared memory and TMA stores. (Letting half 0 run ahead at the ends of a tile, to read one half back under
+// the other's multiplications, held the stages longer than it hid: 5 % slower.)
 // Tiles that do not fill a round of pairs are cut into smaller ones (256 rows, 256 or 128 columns), and so is a tile whose
 // second half lies beyond the last row.
 //
@@ -32,13 +33,13 @@ constexpr int kHalfJ = 256, kTileJ = 2 * kHalfJ, kTileI = 256, kRowsQ = 128, kSt
 constexpr int kBoxQ = kRowsQ * 128;  // bytes of one half's rows of Q in a stage
 constexpr int kStage = 2 * kBoxQ + 128 * 128, kStages = 4;
 constexpr int kEpiWarps = 8, kProducer = 8, kMma = 9, kThreads = 320, kTmemCols = 512;
-constexpr int kSmemBytes = kStages * kStage + 1024 + 256;
+constexpr int kOut = 32 * 128;  // a warp's outputs on their way out: 32 rows x 64 columns, 128-byte swizzle
+constexpr int kSmemBytes = kStages * kStage + kEpiWarps * kOut + 1024 + 256;
 constexpr int kBand = 8;    // tile rows per band of the tile order
-constexpr int kAhead = 4;   // steps that half 0 is ahead at the beginning of a tile (at most kStages)
-constexpr int kBehind = 2;  // and at its end
 
 struct PairProduct {
   CUtensorMap map_q, map_p;  // boxes of 64 values of r x 128 (Q) or 64 (P) rows, or 64 x 64 where r is not contiguous
+  CUtensorMap map_out, map_preact;  // boxes of 64 columns x 32 rows (where vector_ok)
   const void* bias;
   const void* residual;
   void* out;
@@ -167,16 +168,86 @@ __device__ __forceinline__ void add32(const void* src, int64_t at, float (&v)[32
   }
 }
 
+// 32 neighbouring outputs as 16 words, and those words into a row of the warp's staging tile (columns 32 q ...).
 template <bool BF16>
-__device__ __forceinline__ void put32(void* dst, int64_t at, const float (&v)[32]) {
-  uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + at);
+__device__ __forceinline__ void pack32(const float (&v)[32], uint32_t (&w)[16]) {
 #pragma unroll
-  for (int q = 0; q < 4; q++)
-    d[q] = make_uint4(pack16<BF16>(v[q * 8], v[q * 8 + 1]), pack16<BF16>(v[q * 8 + 2], v[q * 8 + 3]),
-                      pack16<BF16>(v[q * 8 + 4], v[q * 8 + 5]), pack16<BF16>(v[q * 8 + 6], v[q * 8 + 7]));
+  for (int e = 0; e < 16; e++) w[e] = pack16<BF16>(v[2 * e], v[2 * e + 1]);
+}
+__device__ __forceinline__ void stage32(uint32_t tile, int lane, int q, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + lane * 128 + (((4 * q + e) ^ (lane & 7)) << 4)), "r"(w[4 * e]),
+                 "r"(w[4 * e + 1]), "r"(w[4 * e + 2]), "r"(w[4 * e + 3])
+                 : "memory");
 }
 
-// 32 neighbouring sums of row j, from column i on.
+// The warp's staging tile to rows `row` ... and columns `col` ... of a matrix (what lies outside of it is not written).
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, uint32_t tile, int lane, int col, int row) {
+  ptx::fence_proxy_async();
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(col), "r"(row), "r"(tile)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+// The staging tile may be written again.
+__device__ __forceinline__ void wait_tile(int lane) {
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
+
+// Two times 32 sums (columns i ... i + 63 of this lane's row j; the warp's rows begin at row0), read from TMEM at `taddr`.
+template <bool BF16>
+__device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, uint32_t tile, int lane, int row0, int i) {
+  uint32_t y[2][16];
+  const bool live = row0 + lane < d.J;
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    uint32_t acc[32], w[16];
+    ptx::tmem_ld_32x32(taddr + 32 * q, acc);
+    ptx::tmem_ld_wait();
+    float v[32];
+#pragma unroll
+    for (int e = 0; e < 32; e++) v[e] = __uint_as_float(acc[e]);
+    const int at = i + 32 * q;
+    const bool inside = at + 32 <= d.I;  // (else the row's last columns: fewer than 32, a multiple of 8)
+    if (d.bias != nullptr) {
+      if (inside) {
+        add32<BF16>(d.bias, at, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          if (at + e < d.I) v[e] += load16<BF16>(d.bias, at + e);
+      }
+    }
+    if (d.preact != nullptr) {
+      pack32<BF16>(v, w);
+      if (q == 0) wait_tile(lane);
+      stage32(tile, lane, q, w);
+    }
+    activate32(v, d.activation);
+    if (d.residual != nullptr && live) {
+      const int64_t r = static_cast<int64_t>(row0 + lane) * d.residual_ld + at;
+      if (inside) {
+        add32<BF16>(d.residual, r, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          if (at + e < d.I) v[e] += load16<BF16>(d.residual, r + e);
+      }
+    }
+    pack32<BF16>(v, y[q]);
+  }
+  if (d.preact != nullptr) store_tile(&d.map_preact, tile, lane, i, row0);
+  wait_tile(lane);
+  stage32(tile, lane, 0, y[0]);
+  stage32(tile, lane, 1, y[1]);
+  store_tile(&d.map_out, tile, lane, i, row0);
+}
+
+// 32 neighbouring sums of row j, from column i on, where rows or operands do not begin on 16 bytes.
 template <bool BF16>
 __device__ __forceinline__ void finish32(const PairProduct& d, int64_t j, int i, const uint32_t (&acc)[32]) {
   if (j >= d.J || i >= d.I) return;
@@ -184,14 +255,6 @@ __device__ __forceinline__ void finish32(const PairProduct& d, int64_t j, int i,
 #pragma unroll
   for (int e = 0; e < 32; e++) v[e] = __uint_as_float(acc[e]);
   const int64_t o = j * d.I + i;
-  if (d.vector_ok && i + 32 <= d.I) {
-    if (d.bias != nullptr) add32<BF16>(d.bias, i, v);
-    if (d.preact != nullptr) put32<BF16>(d.preact, o, v);
-    activate32(v, d.activation);
-    if (d.residual != nullptr) add32<BF16>(d.residual, j * d.residual_ld + i, v);
-    put32<BF16>(d.out, o, v);
-    return;
-  }
 #pragma unroll
   for (int e = 0; e < 32; e++)
     if (i + e < d.I) {
@@ -212,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - ptx::smem_u32(smem_raw));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage + kEpiWarps * kOut);
   const uint32_t full0 = ptx::smem_u32(bars), empty0 = full0 + 8 * kStages, tfull0 = empty0 + 8 * kStages, tempty0 = tfull0 + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -320,54 +383,21 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
             pd += step_p;
           }
         };
-        auto release = [&](long long i) { ptx::tc_commit_pair(empty0 + 8 * static_cast<int>(i % kStages)); };  // in both CTAs
-        if (t.halves == 1) {
-          ok = free_buffer(turn);
-          for (int kb = 0; ok && kb < d.blocks; kb++, it++) {
-            ok = wait_full(it);
-            if (!ok) break;
-            multiply(it, 0, turn, kb == 0);
-            release(it);
-          }
-          if (ok) ptx::tc_commit_pair(tfull0 + 8 * turn);
-          turn ^= 1;
-          continue;
-        }
-        // two halves: half 0 ahead at the beginning (its buffer is read back first), and again at the end
-        const int ahead = d.blocks < kAhead ? d.blocks : kAhead;
-        const int behind = d.blocks - ahead < kBehind ? d.blocks - ahead : kBehind;
-        ok = free_buffer(0);
-        for (int kb = 0; ok && kb < ahead; kb++) {
-          ok = wait_full(it + kb);
-          if (ok) multiply(it + kb, 0, 0, kb == 0);
-        }
-        if (ok && behind == 0) ptx::tc_commit_pair(tfull0);
-        ok = ok && free_buffer(1);
-        for (int kb = 0; ok && kb < ahead; kb++) {
-          multiply(it + kb, 1, 1, kb == 0);
-          release(it + kb);
-        }
-        it += ahead;
-        for (int kb = ahead; ok && kb < d.blocks - behind; kb++, it++) {
+        const bool both = t.halves == 2;
+        const int buffer = both ? 0 : turn;  // (a single half takes the buffers in turn)
+        if (!both) turn ^= 1;
+        ok = free_buffer(buffer) && (!both || free_buffer(1));
+        for (int kb = 0; ok && kb < d.blocks; kb++, it++) {
           ok = wait_full(it);
           if (!ok) break;
-          multiply(it, 0, 0, false);
-          multiply(it, 1, 1, false);
-          release(it);
+          multiply(it, 0, buffer, kb == 0);
+          if (both) multiply(it, 1, 1, kb == 0);
+          ptx::tc_commit_pair(empty0 + 8 * static_cast<int>(it % kStages));  // frees the stage in both CTAs
         }
-        if (ok && behind != 0) {
-          for (int kb = 0; ok && kb < behind; kb++) {
-            ok = wait_full(it + kb);
-            if (ok) multiply(it + kb, 0, 0, false);
-          }
-          if (ok) ptx::tc_commit_pair(tfull0);
-          for (int kb = 0; ok && kb < behind; kb++) {
-            multiply(it + kb, 1, 1, false);
-            release(it + kb);
-          }
-          it += behind;
+        if (ok) {
+          ptx::tc_commit_pair(tfull0 + 8 * buffer);
+          if (both) ptx::tc_commit_pair(tfull0 + 8);
         }
-        if (ok) ptx::tc_commit_pair(tfull0 + 8);
       }
     }
     __syncwarp();
@@ -384,14 +414,23 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
         else used0++;
         if (!ok) break;
         ptx::tc_fence_after();
-        const int64_t row = static_cast<int64_t>(t.row) + h * kHalfJ + rank * kRowsQ + (warp & 3) * 32 + lane;
+        const int row0 = t.row + h * kHalfJ + static_cast<int>(rank) * kRowsQ + (warp & 3) * 32;
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(b * 256);
+        const uint32_t tile = base + kStages * kStage + warp * kOut;
 #pragma unroll 1
-        for (int c = (warp >> 2) * 32; c < t.cols; c += 64) {
-          uint32_t r[32];
-          ptx::tmem_ld_32x32(taddr + c, r);
-          ptx::tmem_ld_wait();
-          finish32<BF16>(d, row, t.col + c, r);
+        for (int c = (warp >> 2) * 64; c < t.cols; c += 128) {
+          if (row0 >= d.J || t.col + c >= d.I) break;  // (nothing of it is inside)
+          if (d.vector_ok) {
+            finish64<BF16>(d, taddr + c, tile, lane, row0, t.col + c);
+          } else {
+#pragma unroll 1
+            for (int q = 0; q < 64; q += 32) {
+              uint32_t r[32];
+              ptx::tmem_ld_32x32(taddr + c + q, r);
+              ptx::tmem_ld_wait();
+              finish32<BF16>(d, row0 + lane, t.col + c + q, r);
+            }
+          }
         }
         ptx::tc_fence_before();
         __syncwarp();
@@ -399,6 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
       }
       if (t.halves == 1) turn ^= 1;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the last stores have been made
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -467,6 +507,12 @@ int pair_product(const LinearProduct& lp, PairProduct* d) {
   const uintptr_t all = reinterpret_cast<uintptr_t>(lp.out) | reinterpret_cast<uintptr_t>(lp.preact) | reinterpret_cast<uintptr_t>(lp.bias) |
                         reinterpret_cast<uintptr_t>(lp.residual);
   d->vector_ok = (all & 15u) == 0 && lp.I % 8 == 0 && (lp.residual == nullptr || lp.residual_ld % 8 == 0);
+  if (d->vector_ok) {
+    const CUtensorMapDataType dt = lp.dtype == TVB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (make_tensor_map_2d(&d->map_out, lp.out, dt, lp.I, lp.J, lp.I * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) != 0) return -1;
+    if (lp.preact != nullptr && make_tensor_map_2d(&d->map_preact, lp.preact, dt, lp.I, lp.J, lp.I * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) != 0)
+      return -1;
+  }
   const uint32_t fmt = lp.dtype == TVB_BF16 ? 1 : 0;
   d->fmt = ptx::tc_instr_desc(1, fmt, fmt, kHalfJ, 0) | (lp.q_mn ? ptx::kTcAMajorMN : 0u) | (lp.p_mn ? ptx::kTcBMajorMN : 0u);
   return 0;
