@@ -270,6 +270,84 @@ __device__ __forceinline__ void finish32(const PairProduct& d, int64_t j, int i,
     }
 }
 
+// The roles' inner loops are run by one thread each, whose own instructions are the pace of everything (a copy instruction that
+// follows some hundred clocks of index arithmetic halves what the copies can move): a position in the ring is a counter and a
+// phase that step along, addresses and descriptors are sums, and the operands' orders are compile-time constants.
+struct RingAt {
+  uint32_t slot = 0, phase = 0, rounds = 0;
+  __device__ __forceinline__ void step() {
+    if (++slot == kStages) {
+      slot = 0;
+      phase ^= 1u;
+      rounds++;
+    }
+  }
+};
+
+// The boxes of one tile (both CTAs of the pair run this, each for its own rows; `bar`: the leader's barriers, `bytes`: both CTAs').
+template <bool Q_MN, bool P_MN>
+__device__ __forceinline__ bool load_tile(const PairProduct& d, const PairTile& t, uint32_t rank, RingAt& at, uint32_t base, uint32_t full0,
+                                          uint32_t empty0, uint32_t bar0, volatile int* abort_flag) {
+  const int row_q = t.row + static_cast<int>(rank) * kRowsQ, row_p = t.col + static_cast<int>(rank) * (t.cols >> 1);
+  const bool two = t.halves == 2, wide = t.cols == kTileI;
+  const uint32_t bytes = 2u * ((two ? 2 : 1) * kBoxQ + (wide ? 2 : 1) * 8192);
+  const int blocks = d.blocks;
+  int r = 0;
+#pragma unroll 1
+  for (int kb = 0; kb < blocks; kb++, r += kStepR, at.step()) {
+    if (!ptx::mbar_wait(empty0 + 8 * at.slot, at.phase ^ 1u, abort_flag)) return false;
+    const uint32_t dst = base + at.slot * kStage, bar = bar0 + 8 * at.slot;
+    if (rank == 0) ptx::mbar_expect_tx(full0 + 8 * at.slot, bytes);
+    if (Q_MN) {
+      ptx::tma_load_2d_pair(dst, &d.map_q, row_q, r, bar);
+      ptx::tma_load_2d_pair(dst + 8192, &d.map_q, row_q + 64, r, bar);
+      if (two) {
+        ptx::tma_load_2d_pair(dst + kBoxQ, &d.map_q, row_q + kHalfJ, r, bar);
+        ptx::tma_load_2d_pair(dst + kBoxQ + 8192, &d.map_q, row_q + kHalfJ + 64, r, bar);
+      }
+    } else {
+      ptx::tma_load_2d_pair(dst, &d.map_q, r, row_q, bar);
+      if (two) ptx::tma_load_2d_pair(dst + kBoxQ, &d.map_q, r, row_q + kHalfJ, bar);
+    }
+    if (P_MN) {
+      ptx::tma_load_2d_pair(dst + 2 * kBoxQ, &d.map_p, row_p, r, bar);
+      if (wide) ptx::tma_load_2d_pair(dst + 2 * kBoxQ + 8192, &d.map_p, row_p + 64, r, bar);
+    } else {
+      ptx::tma_load_2d_pair(dst + 2 * kBoxQ, &d.map_p, r, row_p, bar);
+      if (wide) ptx::tma_load_2d_pair(dst + 2 * kBoxQ + 8192, &d.map_p, r, row_p + 64, bar);
+    }
+  }
+  return true;
+}
+
+// The multiplications of one tile; half 0 into the sums at `d0`, half 1 (where there is one) into those at `d1`.
+template <bool Q_MN, bool P_MN>
+__device__ __forceinline__ bool multiply_tile(const PairProduct& d, const PairTile& t, RingAt& at, uint32_t base, uint32_t full0, uint32_t empty0,
+                                              uint32_t d0, uint32_t d1, volatile int* abort_flag) {
+  constexpr uint64_t kQ = Q_MN ? 128 : 2, kP = P_MN ? 128 : 2;  // 16 values of r, in the descriptors' units
+  const uint32_t idesc = d.fmt | (static_cast<uint32_t>(t.cols >> 3) << 17);
+  const uint64_t q0 = Q_MN ? ptx::tc_smem_desc_sw128_mn(base) : ptx::tc_smem_desc_sw128(base);
+  const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(base + 2 * kBoxQ) : ptx::tc_smem_desc_sw128(base + 2 * kBoxQ);
+  const bool two = t.halves == 2;
+  const int blocks = d.blocks;
+  uint32_t more = 0;  // (the first instruction of a tile overwrites the sums)
+#pragma unroll 1
+  for (int kb = 0; kb < blocks; kb++, at.step()) {
+    if (!ptx::mbar_wait(full0 + 8 * at.slot, at.phase, abort_flag)) return false;
+    ptx::tc_fence_after();
+    const uint64_t qd = q0 + at.slot * (kStage >> 4), pd = p0 + at.slot * (kStage >> 4);
+#pragma unroll
+    for (int j = 0; j < kStepR / 16; j++) ptx::tc_mma_pair<2>(d0, qd + kQ * j, pd + kP * j, idesc, j == 0 ? more : 1u);
+    if (two) {
+#pragma unroll
+      for (int j = 0; j < kStepR / 16; j++) ptx::tc_mma_pair<2>(d1, qd + (kBoxQ >> 4) + kQ * j, pd + kP * j, idesc, j == 0 ? more : 1u);
+    }
+    more = 1;
+    ptx::tc_commit_pair(empty0 + 8 * at.slot);  // frees the stage in both CTAs
+  }
+  return true;
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_constant__ PairParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -307,93 +385,46 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
   PairTile t;
   if (warp == kProducer) {
     if (lane == 0) {
-      long long it = 0;
+      RingAt at;
+      const uint32_t bar0 = ptx::mapa(full0, 0);  // the leader's barriers, from either CTA
       bool ok = true;
       while (ok && sched.next(p, t)) {
         const PairProduct& d = p.prod[t.product];
-        const int row_q = t.row + static_cast<int>(rank) * kRowsQ, boxes_p = t.cols >> 7;
-        const int row_p = t.col + static_cast<int>(rank) * (t.cols >> 1);
-        const uint32_t bytes = 2u * (t.halves * kBoxQ + boxes_p * 8192);  // both CTAs' boxes of a stage
-        for (int kb = 0; kb < d.blocks; kb++, it++) {
-          const int s = static_cast<int>(it % kStages);
-          ok = ptx::mbar_wait(empty0 + 8 * s, static_cast<uint32_t>((it / kStages) & 1) ^ 1u, abort_flag);
-          if (!ok) break;
-          const uint32_t dst = base + s * kStage;
-          if (rank == 0) ptx::mbar_expect_tx(full0 + 8 * s, bytes);
-          const uint32_t bar = ptx::mapa(full0 + 8 * s, 0);
-          const int r = kb * kStepR;
-          for (int h = 0; h < t.halves; h++) {
-            const uint32_t at = dst + h * kBoxQ;
-            const int row = row_q + h * kHalfJ;
-            if (d.q_mn) {
-              ptx::tma_load_2d_pair(at, &d.map_q, row, r, bar);
-              ptx::tma_load_2d_pair(at + 8192, &d.map_q, row + 64, r, bar);
-            } else {
-              ptx::tma_load_2d_pair(at, &d.map_q, r, row, bar);
-            }
-          }
-          for (int c = 0; c < boxes_p; c++) {
-            const uint32_t at = dst + 2 * kBoxQ + c * 8192;
-            if (d.p_mn) ptx::tma_load_2d_pair(at, &d.map_p, row_p + 64 * c, r, bar);
-            else ptx::tma_load_2d_pair(at, &d.map_p, r, row_p + 64 * c, bar);
-          }
-        }
+        ok = d.q_mn   ? load_tile<true, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
+             : d.p_mn ? load_tile<false, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
+                      : load_tile<false, false>(d, t, rank, at, base, full0, empty0, bar0, abort_flag);
       }
-      if (rank == 0) {
-        // no copy of either CTA may still be in flight when the pair's shared memory is released
-        const long long first = it > kStages ? it - kStages : 0;
-        for (long long j = first; j < it; j++) {
-          volatile int never = 0;
-          ptx::mbar_wait(full0 + 8 * static_cast<int>(j % kStages), static_cast<uint32_t>((j / kStages) & 1), &never);
-        }
+      // no copy of either CTA may still be in flight when the pair's shared memory is released: wait for the last filling of
+      // every slot (slots before at.slot were filled in this round, the others in the round before, if there was one)
+      for (uint32_t s = 0; rank == 0 && s < kStages; s++) {
+        volatile int never = 0;
+        if (s < at.slot) ptx::mbar_wait(full0 + 8 * s, at.phase, &never);
+        else if (at.rounds != 0) ptx::mbar_wait(full0 + 8 * s, at.phase ^ 1u, &never);
       }
     }
     __syncwarp();
   } else if (warp == kMma) {
     if (lane == 0 && rank == 0) {
-      long long it = 0;
+      RingAt at;
       uint32_t used0 = 0, used1 = 0;  // tiles (or halves) that each buffer of sums has held
       int turn = 0;
       bool ok = true;
       while (ok && sched.next(p, t)) {
         const PairProduct& d = p.prod[t.product];
-        const uint64_t step_q = d.q_mn ? 128 : 2, step_p = d.p_mn ? 128 : 2;
-        const uint32_t idesc = d.fmt | (static_cast<uint32_t>(t.cols >> 3) << 17);
-        auto wait_full = [&](long long i) {
-          const bool there = ptx::mbar_wait(full0 + 8 * static_cast<int>(i % kStages), static_cast<uint32_t>((i / kStages) & 1), abort_flag);
-          ptx::tc_fence_after();
-          return there;
-        };
-        auto free_buffer = [&](int b) {
-          const bool there = ptx::mbar_wait(tempty0 + 8 * b, ((b ? used1 : used0) & 1u) ^ 1u, abort_flag);
-          ptx::tc_fence_after();
-          if (b) used1++;
-          else used0++;
-          return there;
-        };
-        auto multiply = [&](long long i, int half, int buffer, bool first) {
-          const uint32_t at_q = base + static_cast<int>(i % kStages) * kStage + half * kBoxQ;
-          const uint32_t at_p = base + static_cast<int>(i % kStages) * kStage + 2 * kBoxQ;
-          uint64_t qd = d.q_mn ? ptx::tc_smem_desc_sw128_mn(at_q) : ptx::tc_smem_desc_sw128(at_q);
-          uint64_t pd = d.p_mn ? ptx::tc_smem_desc_sw128_mn(at_p) : ptx::tc_smem_desc_sw128(at_p);
-#pragma unroll
-          for (int j = 0; j < kStepR / 16; j++) {
-            ptx::tc_mma_pair<2>(tmem_base + static_cast<uint32_t>(buffer * 256), qd, pd, idesc, first && j == 0 ? 0u : 1u);
-            qd += step_q;
-            pd += step_p;
-          }
-        };
         const bool both = t.halves == 2;
         const int buffer = both ? 0 : turn;  // (a single half takes the buffers in turn)
         if (!both) turn ^= 1;
-        ok = free_buffer(buffer) && (!both || free_buffer(1));
-        for (int kb = 0; ok && kb < d.blocks; kb++, it++) {
-          ok = wait_full(it);
-          if (!ok) break;
-          multiply(it, 0, buffer, kb == 0);
-          if (both) multiply(it, 1, 1, kb == 0);
-          ptx::tc_commit_pair(empty0 + 8 * static_cast<int>(it % kStages));  // frees the stage in both CTAs
-        }
+        // the epilogues of both CTAs have read what the buffers held
+        ok = ptx::mbar_wait(tempty0 + 8 * buffer, ((buffer ? used1 : used0) & 1u) ^ 1u, abort_flag);
+        if (buffer) used1++;
+        else used0++;
+        if (ok && both) ok = ptx::mbar_wait(tempty0 + 8, (used1++ & 1u) ^ 1u, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t d0 = tmem_base + static_cast<uint32_t>(buffer * 256), d1 = tmem_base + 256;
+        ok = d.q_mn   ? multiply_tile<true, true>(d, t, at, base, full0, empty0, d0, d1, abort_flag)
+             : d.p_mn ? multiply_tile<false, true>(d, t, at, base, full0, empty0, d0, d1, abort_flag)
+                      : multiply_tile<false, false>(d, t, at, base, full0, empty0, d0, d1, abort_flag);
         if (ok) {
           ptx::tc_commit_pair(tfull0 + 8 * buffer);
           if (both) ptx::tc_commit_pair(tfull0 + 8);
