@@ -18,57 +18,47 @@ namespace {
 
 constexpr int kStrip = 64, kThreads = 256, kRowsPerStep = 32;
 
+// Eight neighbouring values as four pairs.
 template <int DT>
-__device__ __forceinline__ void load8(const void* base, int64_t i, float (&v)[8]) {
+__device__ __forceinline__ void load8(const void* base, int64_t i, uint64_t (&v)[4]) {
   if constexpr (DT == TVB_F32) {
-    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
-    const float4 a = s[0], b = s[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
-    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float2 f = unpack16<DT == TVB_BF16>(w[e]);
-      v[2 * e] = f.x;
-      v[2 * e + 1] = f.y;
-    }
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(void* base, int64_t i, const float (&v)[8]) {
-  if constexpr (DT == TVB_F32) {
-    float4* d = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
-    d[0] = make_float4(v[0], v[1], v[2], v[3]);
-    d[1] = make_float4(v[4], v[5], v[6], v[7]);
+    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + i);
+    const uint4 a = s[0], b = s[1];
+    v[0] = ptx::pack_f32x2(a.x, a.y); v[1] = ptx::pack_f32x2(a.z, a.w); v[2] = ptx::pack_f32x2(b.x, b.y); v[3] = ptx::pack_f32x2(b.z, b.w);
   } else {
     constexpr bool kB = DT == TVB_BF16;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + i) =
-        make_uint4(pack16<kB>(v[0], v[1]), pack16<kB>(v[2], v[3]), pack16<kB>(v[4], v[5]), pack16<kB>(v[6], v[7]));
+    const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
+    v[0] = unpack16<kB>(t.x); v[1] = unpack16<kB>(t.y); v[2] = unpack16<kB>(t.z); v[3] = unpack16<kB>(t.w);
   }
 }
 
-// v *= act'(z), the choice of activation made once for the eight.
-template <bool FAST>
-__device__ __forceinline__ void slopes8(float (&v)[8], const float (&z)[8], int act) {
-  switch (act) {
-    case TVB_ACT_RELU:
+template <int DT>
+__device__ __forceinline__ void store8(void* base, int64_t i, const uint64_t (&v)[4]) {
+  if constexpr (DT == TVB_F32) {
+    float f[8];
 #pragma unroll
-      for (int c = 0; c < 8; c++) v[c] *= act_slope<FAST>(z[c], TVB_ACT_RELU);
-      break;
-    case TVB_ACT_GELU:
+    for (int e = 0; e < 4; e++) ptx::unpack_f32x2(v[e], f[2 * e], f[2 * e + 1]);
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
+    d[0] = make_float4(f[0], f[1], f[2], f[3]);
+    d[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    constexpr bool kB = DT == TVB_BF16;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + i) = make_uint4(pack16<kB>(v[0]), pack16<kB>(v[1]), pack16<kB>(v[2]), pack16<kB>(v[3]));
+  }
+}
+
+// v *= act'(z)
+template <int DT>
+__device__ __forceinline__ void times_slope(uint64_t (&v)[4], const uint64_t (&z)[4], int act) {
+  if constexpr (DT == TVB_F32) {
 #pragma unroll
-      for (int c = 0; c < 8; c++) v[c] *= act_slope<FAST>(z[c], TVB_ACT_GELU);
-      break;
-    case TVB_ACT_GELU_TANH:
-#pragma unroll
-      for (int c = 0; c < 8; c++) v[c] *= act_slope<FAST>(z[c], TVB_ACT_GELU_TANH);
-      break;
-    default:
-#pragma unroll
-      for (int c = 0; c < 8; c++) v[c] *= act_slope<FAST>(z[c], TVB_ACT_SILU);
-      break;
+    for (int e = 0; e < 4; e++) {
+      float a, b;
+      ptx::unpack_f32x2(z[e], a, b);
+      v[e] = ptx::mul_f32x2(v[e], ptx::pack_f32x2(__float_as_uint(act_slope(a, act)), __float_as_uint(act_slope(b, act))));
+    }
+  } else {
+    times_slope_pairs(v, z, act);
   }
 }
 
@@ -83,38 +73,56 @@ __global__ void __launch_bounds__(kThreads) linear_dz_kernel(const LinearDz p) {
   const int64_t c0 = static_cast<int64_t>(blockIdx.x / parts) * kStrip + (threadIdx.x & 7) * 8;
   const int64_t r_begin = p.m * part / parts, r_end = p.m * (part + 1) / parts;
   const bool act = p.activation != TVB_ACT_NONE;
-  float sum[8] = {};
-  if (VEC) {
-    if (c0 < p.n) {
+  uint64_t sum[4] = {};
+  const int64_t c_end = p.n - c0;  // columns of this thread that exist
+  if (c_end > 0) {
 #pragma unroll 2
-      for (int64_t r = r_begin + (threadIdx.x >> 3); r < r_end; r += kRowsPerStep) {
-        float v[8], z[8];
-        load8<DT>(p.dy, r * p.dy_ld + c0, v);
-        if (act) {
-          load8<DT>(p.z, r * p.n + c0, z);
-          slopes8<DT != TVB_F32>(v, z, p.activation);
-        }
-#pragma unroll
-        for (int c = 0; c < 8; c++) sum[c] += v[c];
-        if (p.dz != nullptr) store8<DT>(p.dz, r * p.dz_ld + c0, v);
-      }
-    }
-  } else {
     for (int64_t r = r_begin + (threadIdx.x >> 3); r < r_end; r += kRowsPerStep) {
+      uint64_t v[4], z[4];
+      if (VEC) {
+        load8<DT>(p.dy, r * p.dy_ld + c0, v);
+        if (act) load8<DT>(p.z, r * p.n + c0, z);
+      } else {
 #pragma unroll
-      for (int c = 0; c < 8; c++) {
-        if (c0 + c >= p.n) break;
-        float v = load_float<DT>(p.dy, r * p.dy_ld + c0 + c);
-        if (act) v *= act_slope<DT != TVB_F32>(load_float<DT>(p.z, r * p.n + c0 + c), p.activation);
-        sum[c] += v;
-        if (p.dz != nullptr) store_float<DT>(p.dz, r * p.dz_ld + c0 + c, v);
+        for (int e = 0; e < 4; e++) {
+          float f[4] = {};
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            if (2 * e + h < c_end) {
+              f[h] = load_float<DT>(p.dy, r * p.dy_ld + c0 + 2 * e + h);
+              if (act) f[2 + h] = load_float<DT>(p.z, r * p.n + c0 + 2 * e + h);
+            }
+          v[e] = ptx::pack_f32x2(__float_as_uint(f[0]), __float_as_uint(f[1]));
+          z[e] = ptx::pack_f32x2(__float_as_uint(f[2]), __float_as_uint(f[3]));
+        }
+      }
+      if (act) times_slope<DT>(v, z, p.activation);
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum[e] = ptx::add_f32x2(sum[e], v[e]);
+      if (p.dz == nullptr) continue;
+      if (VEC) {
+        store8<DT>(p.dz, r * p.dz_ld + c0, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float f[2];
+          ptx::unpack_f32x2(v[e], f[0], f[1]);
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            if (2 * e + h < c_end) store_float<DT>(p.dz, r * p.dz_ld + c0 + 2 * e + h, f[h]);
+        }
       }
     }
   }
   __shared__ float part_sums[kRowsPerStep][kStrip];
   __shared__ float cta_sums[kStrip];
 #pragma unroll
-  for (int c = 0; c < 8; c++) part_sums[threadIdx.x >> 3][(threadIdx.x & 7) * 8 + c] = sum[c];
+  for (int e = 0; e < 4; e++) {
+    float lo, hi;
+    ptx::unpack_f32x2(sum[e], lo, hi);
+    part_sums[threadIdx.x >> 3][(threadIdx.x & 7) * 8 + 2 * e] = lo;
+    part_sums[threadIdx.x >> 3][(threadIdx.x & 7) * 8 + 2 * e + 1] = hi;
+  }
   __syncthreads();
   if (threadIdx.x < kStrip) {
     float s = 0.0f;

@@ -1,15 +1,13 @@
 // The 16-bit products of linear.h on tcgen05 when the output is large: bound by the tensor pipe.
 //
-// A cluster of two CTAs (the two SMs of a TPC) walks output tiles of 512 rows (j) x 256 columns (i): per 64 values of r each CTA
-// stages 256 rows of Q (two halves of 128) and 128 rows of P, 48 KB, and one lane of CTA 0 issues tcgen05.mma.cta_group::2 for both:
-// one instruction multiplies a half of both CTAs (256 rows) by the 256 columns. What paces such a kernel is the L2: with tiles of
-// 256 x 256 (32 KB per SM for half the work) every SM asks for a third more bytes per multiplication, and the steps took 690 clocks
-// where the tensor core needs 512. The two halves' sums fill the tensor memory, so a tile's read-back is not overlapped; it is kept
-// short by leaving through shared memory and TMA stores. (Letting half 0 run ahead at the ends of a tile, to read one half back under
-// the other's multiplications, held the stages longer than it hid: 5 % slower.)
-// Tiles that do not fill a round of pairs are cut into smaller ones (256 rows, 256 or 128 columns), and so is a tile whose
-// second half lies beyond the last row.
-//
+// A cluster of two CTAs (the two SMs of a TPC) walks output tiles of 256 rows (j) x 256 columns (i): per 64 values of r each CTA
+// stages 128 rows of Q and 128 rows of P, 32 KB, six stages deep, and one lane of CTA 0 issues tcgen05.mma.cta_group::2 for both.
+// Each CTA's TMEM receives its own 128 rows of the tile, in two buffers, so that a tile is read back under the next tile's
+// multiplications. With a long r tiles have 512 rows, in two halves that share P: 48 KB per stage for twice the work, so a third
+// less to move per multiplication; the halves' sums fill the TMEM, and a tile's read-back is not overlapped. Tiles that do not
+// fill a round of pairs are cut into smaller ones (256 rows, 256 or 128 columns).
+// Outputs leave through shared memory and TMA stores (a thread of the epilogue holds a row's 64 columns; stored from
+// registers they are 32 scattered pieces per instruction, and the read-back took four times as long).
 // A launch takes one product or two: the backward pass multiplies dz by w and by x at once. The tiles of the product with the
 // longer r come first; pairs that get one tile of it less than others start on the second product meanwhile, and the rest of its
 // tiles are dealt out in turn. The schedule is computed from the sizes alone (no counters in memory), so launches share nothing.
@@ -29,13 +27,22 @@
 namespace tvb {
 namespace {
 
-constexpr int kHalfJ = 256, kTileJ = 2 * kHalfJ, kTileI = 256, kRowsQ = 128, kStepR = 64;
+constexpr int kHalfJ = 256, kTileI = 256, kRowsQ = 128, kStepR = 64;
 constexpr int kBoxQ = kRowsQ * 128;  // bytes of one half's rows of Q in a stage
-constexpr int kStage = 2 * kBoxQ + 128 * 128, kStages = 4;
+// HALVES: 2 for tiles of 512 rows, 1 for tiles of 256.
+template <int HALVES>
+struct PairCfg {
+  static constexpr int kTileJ = HALVES * kHalfJ;
+  static constexpr int kP = HALVES * kBoxQ;  // where P begins in a stage
+  static constexpr int kStage = kP + 128 * 128;
+  static constexpr int kStages = HALVES == 2 ? 4 : 6;
+  static constexpr int kBand = 16 / HALVES;  // tile rows per band of the tile order
+};
+constexpr int kRing = 192 * 1024;
+static_assert(PairCfg<1>::kStages * PairCfg<1>::kStage == kRing && PairCfg<2>::kStages * PairCfg<2>::kStage == kRing, "the ring's size");
 constexpr int kEpiWarps = 8, kProducer = 8, kMma = 9, kThreads = 320, kTmemCols = 512;
 constexpr int kOut = 32 * 128;  // a warp's outputs on their way out: 32 rows x 64 columns, 128-byte swizzle
-constexpr int kSmemBytes = kStages * kStage + kEpiWarps * kOut + 1024 + 256;
-constexpr int kBand = 8;    // tile rows per band of the tile order
+constexpr int kSmemBytes = kRing + kEpiWarps * kOut + 1024 + 256;
 
 struct PairProduct {
   CUtensorMap map_q, map_p;  // boxes of 64 values of r x 128 (Q) or 64 (P) rows, or 64 x 64 where r is not contiguous
@@ -64,7 +71,9 @@ struct PairTile {
 };
 
 // Walks the tiles of one pair: its tiles of product 0, its share of product 1, its share of what was cut.
+template <int HALVES>
 struct PairSchedule {
+  using Cfg = PairCfg<HALVES>;
   int pair, pairs, at, heavy, rank_among, order, stage;
   bool is_light;
   __device__ PairSchedule(const PairParams& p, int pair_, int pairs_) : pair(pair_), pairs(pairs_) {
@@ -76,13 +85,13 @@ struct PairSchedule {
     at = pair;
   }
   __device__ static void place(const PairProduct& d, int index, PairTile& t) {
-    const int per_band = kBand * d.tiles_i, b = index / per_band, first = b * kBand;
-    const int rows = d.tiles_j - first < kBand ? d.tiles_j - first : kBand;
+    const int per_band = Cfg::kBand * d.tiles_i, b = index / per_band, first = b * Cfg::kBand;
+    const int rows = d.tiles_j - first < Cfg::kBand ? d.tiles_j - first : Cfg::kBand;
     const int r = index - b * per_band;
-    t.row = (first + r % rows) * kTileJ;
+    t.row = (first + r % rows) * Cfg::kTileJ;
     t.col = r / rows * kTileI;
     t.cols = kTileI;
-    t.halves = t.row + kHalfJ < d.J ? 2 : 1;
+    t.halves = HALVES == 2 && t.row + kHalfJ < d.J ? 2 : 1;
   }
   __device__ bool next(const PairParams& p, PairTile& t) {
     const int light = heavy != 0 ? pairs - heavy : 0, early = light * p.extra;
@@ -116,7 +125,7 @@ struct PairSchedule {
         stage = 3;
         at = order;
       }
-      const int per_half = kTileI / p.cut_cols, per_tile = 2 * per_half;
+      const int per_half = kTileI / p.cut_cols, per_tile = HALVES * per_half;
       const int index = p.whole + at / per_tile, sub = at % per_tile;
       if (index >= p.prod[1].tiles) return false;
       at += pairs;
@@ -130,49 +139,32 @@ struct PairSchedule {
   }
 };
 
-__device__ __forceinline__ void activate32(float (&v)[32], int act) {
-  switch (act) {
-    case TVB_ACT_RELU:
-#pragma unroll
-      for (int e = 0; e < 32; e++) v[e] = act_value<true>(v[e], TVB_ACT_RELU);
-      break;
-    case TVB_ACT_GELU:
-#pragma unroll
-      for (int e = 0; e < 32; e++) v[e] = act_value<true>(v[e], TVB_ACT_GELU);
-      break;
-    case TVB_ACT_GELU_TANH:
-#pragma unroll
-      for (int e = 0; e < 32; e++) v[e] = act_value<true>(v[e], TVB_ACT_GELU_TANH);
-      break;
-    case TVB_ACT_SILU:
-#pragma unroll
-      for (int e = 0; e < 32; e++) v[e] = act_value<true>(v[e], TVB_ACT_SILU);
-      break;
-    default: break;
-  }
-}
-
 template <bool BF16>
-__device__ __forceinline__ void add32(const void* src, int64_t at, float (&v)[32]) {  // (16-byte aligned)
+__device__ __forceinline__ void add32(const void* src, int64_t at, uint64_t (&v)[16]) {  // (16-byte aligned)
   const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at);
 #pragma unroll
   for (int q = 0; q < 4; q++) {
     const uint4 x = s[q];
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float2 f = unpack16<BF16>(w[e]);
-      v[q * 8 + 2 * e] += f.x;
-      v[q * 8 + 2 * e + 1] += f.y;
-    }
+    v[4 * q] = ptx::add_f32x2(v[4 * q], unpack16<BF16>(x.x));
+    v[4 * q + 1] = ptx::add_f32x2(v[4 * q + 1], unpack16<BF16>(x.y));
+    v[4 * q + 2] = ptx::add_f32x2(v[4 * q + 2], unpack16<BF16>(x.z));
+    v[4 * q + 3] = ptx::add_f32x2(v[4 * q + 3], unpack16<BF16>(x.w));
   }
+}
+
+__device__ __forceinline__ void load32(uint32_t taddr, uint64_t (&v)[16]) {
+  uint32_t acc[32];
+  ptx::tmem_ld_32x32(taddr, acc);
+  ptx::tmem_ld_wait();
+#pragma unroll
+  for (int e = 0; e < 16; e++) v[e] = ptx::pack_f32x2(acc[2 * e], acc[2 * e + 1]);
 }
 
 // 32 neighbouring outputs as 16 words, and those words into a row of the warp's staging tile (columns 32 q ...).
 template <bool BF16>
-__device__ __forceinline__ void pack32(const float (&v)[32], uint32_t (&w)[16]) {
+__device__ __forceinline__ void pack32(const uint64_t (&v)[16], uint32_t (&w)[16]) {
 #pragma unroll
-  for (int e = 0; e < 16; e++) w[e] = pack16<BF16>(v[2 * e], v[2 * e + 1]);
+  for (int e = 0; e < 16; e++) w[e] = pack16<BF16>(v[e]);
 }
 __device__ __forceinline__ void stage32(uint32_t tile, int lane, int q, const uint32_t (&w)[16]) {
 #pragma unroll
@@ -205,38 +197,25 @@ __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, u
   const bool live = row0 + lane < d.J;
 #pragma unroll
   for (int q = 0; q < 2; q++) {
-    uint32_t acc[32], w[16];
-    ptx::tmem_ld_32x32(taddr + 32 * q, acc);
-    ptx::tmem_ld_wait();
-    float v[32];
-#pragma unroll
-    for (int e = 0; e < 32; e++) v[e] = __uint_as_float(acc[e]);
+    uint32_t w[16];
+    uint64_t v[16];
+    load32(taddr + 32 * q, v);
     const int at = i + 32 * q;
     const bool inside = at + 32 <= d.I;  // (else the row's last columns: fewer than 32, a multiple of 8)
     if (d.bias != nullptr) {
-      if (inside) {
-        add32<BF16>(d.bias, at, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; e++)
-          if (at + e < d.I) v[e] += load16<BF16>(d.bias, at + e);
-      }
+      if (inside) add32<BF16>(d.bias, at, v);
+      else add_singly<BF16>(d.bias, at, d.I - at, v);
     }
     if (d.preact != nullptr) {
       pack32<BF16>(v, w);
       if (q == 0) wait_tile(lane);
       stage32(tile, lane, q, w);
     }
-    activate32(v, d.activation);
+    activate_pairs(v, d.activation);
     if (d.residual != nullptr && live) {
       const int64_t r = static_cast<int64_t>(row0 + lane) * d.residual_ld + at;
-      if (inside) {
-        add32<BF16>(d.residual, r, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; e++)
-          if (at + e < d.I) v[e] += load16<BF16>(d.residual, r + e);
-      }
+      if (inside) add32<BF16>(d.residual, r, v);
+      else add_singly<BF16>(d.residual, r, d.I - at, v);
     }
     pack32<BF16>(v, y[q]);
   }
@@ -249,34 +228,27 @@ __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, u
 
 // 32 neighbouring sums of row j, from column i on, where rows or operands do not begin on 16 bytes.
 template <bool BF16>
-__device__ __forceinline__ void finish32(const PairProduct& d, int64_t j, int i, const uint32_t (&acc)[32]) {
+__device__ __forceinline__ void finish32(const PairProduct& d, uint32_t taddr, int64_t j, int i) {
+  uint64_t v[16];
+  load32(taddr, v);
   if (j >= d.J || i >= d.I) return;
-  float v[32];
-#pragma unroll
-  for (int e = 0; e < 32; e++) v[e] = __uint_as_float(acc[e]);
+  const int count = d.I - i;
   const int64_t o = j * d.I + i;
-#pragma unroll
-  for (int e = 0; e < 32; e++)
-    if (i + e < d.I) {
-      if (d.bias != nullptr) v[e] += load16<BF16>(d.bias, i + e);
-      if (d.preact != nullptr) store16<BF16>(d.preact, o + e, v[e]);
-    }
-  activate32(v, d.activation);
-#pragma unroll
-  for (int e = 0; e < 32; e++)
-    if (i + e < d.I) {
-      if (d.residual != nullptr) v[e] += load16<BF16>(d.residual, j * d.residual_ld + i + e);
-      store16<BF16>(d.out, o + e, v[e]);
-    }
+  if (d.bias != nullptr) add_singly<BF16>(d.bias, i, count, v);
+  if (d.preact != nullptr) store_singly<BF16>(d.preact, o, count, v);
+  activate_pairs(v, d.activation);
+  if (d.residual != nullptr) add_singly<BF16>(d.residual, j * d.residual_ld + i, count, v);
+  store_singly<BF16>(d.out, o, count, v);
 }
 
 // The roles' inner loops are run by one thread each, whose own instructions are the pace of everything (a copy instruction that
 // follows some hundred clocks of index arithmetic halves what the copies can move): a position in the ring is a counter and a
 // phase that step along, addresses and descriptors are sums, and the operands' orders are compile-time constants.
+template <int STAGES>
 struct RingAt {
   uint32_t slot = 0, phase = 0, rounds = 0;
   __device__ __forceinline__ void step() {
-    if (++slot == kStages) {
+    if (++slot == STAGES) {
       slot = 0;
       phase ^= 1u;
       rounds++;
@@ -285,11 +257,12 @@ struct RingAt {
 };
 
 // The boxes of one tile (both CTAs of the pair run this, each for its own rows; `bar`: the leader's barriers, `bytes`: both CTAs').
-template <bool Q_MN, bool P_MN>
-__device__ __forceinline__ bool load_tile(const PairProduct& d, const PairTile& t, uint32_t rank, RingAt& at, uint32_t base, uint32_t full0,
+template <int HALVES, bool Q_MN, bool P_MN>
+__device__ __forceinline__ bool load_tile(const PairProduct& d, const PairTile& t, uint32_t rank, RingAt<PairCfg<HALVES>::kStages>& at, uint32_t base, uint32_t full0,
                                           uint32_t empty0, uint32_t bar0, volatile int* abort_flag) {
+  constexpr int kStage = PairCfg<HALVES>::kStage, kPAt = PairCfg<HALVES>::kP;
   const int row_q = t.row + static_cast<int>(rank) * kRowsQ, row_p = t.col + static_cast<int>(rank) * (t.cols >> 1);
-  const bool two = t.halves == 2, wide = t.cols == kTileI;
+  const bool two = HALVES == 2 && t.halves == 2, wide = t.cols == kTileI;
   const uint32_t bytes = 2u * ((two ? 2 : 1) * kBoxQ + (wide ? 2 : 1) * 8192);
   const int blocks = d.blocks;
   int r = 0;
@@ -310,25 +283,26 @@ __device__ __forceinline__ bool load_tile(const PairProduct& d, const PairTile& 
       if (two) ptx::tma_load_2d_pair(dst + kBoxQ, &d.map_q, r, row_q + kHalfJ, bar);
     }
     if (P_MN) {
-      ptx::tma_load_2d_pair(dst + 2 * kBoxQ, &d.map_p, row_p, r, bar);
-      if (wide) ptx::tma_load_2d_pair(dst + 2 * kBoxQ + 8192, &d.map_p, row_p + 64, r, bar);
+      ptx::tma_load_2d_pair(dst + kPAt, &d.map_p, row_p, r, bar);
+      if (wide) ptx::tma_load_2d_pair(dst + kPAt + 8192, &d.map_p, row_p + 64, r, bar);
     } else {
-      ptx::tma_load_2d_pair(dst + 2 * kBoxQ, &d.map_p, r, row_p, bar);
-      if (wide) ptx::tma_load_2d_pair(dst + 2 * kBoxQ + 8192, &d.map_p, r, row_p + 64, bar);
+      ptx::tma_load_2d_pair(dst + kPAt, &d.map_p, r, row_p, bar);
+      if (wide) ptx::tma_load_2d_pair(dst + kPAt + 8192, &d.map_p, r, row_p + 64, bar);
     }
   }
   return true;
 }
 
 // The multiplications of one tile; half 0 into the sums at `d0`, half 1 (where there is one) into those at `d1`.
-template <bool Q_MN, bool P_MN>
-__device__ __forceinline__ bool multiply_tile(const PairProduct& d, const PairTile& t, RingAt& at, uint32_t base, uint32_t full0, uint32_t empty0,
+template <int HALVES, bool Q_MN, bool P_MN>
+__device__ __forceinline__ bool multiply_tile(const PairProduct& d, const PairTile& t, RingAt<PairCfg<HALVES>::kStages>& at, uint32_t base, uint32_t full0, uint32_t empty0,
                                               uint32_t d0, uint32_t d1, volatile int* abort_flag) {
+  constexpr int kStage = PairCfg<HALVES>::kStage, kPAt = PairCfg<HALVES>::kP;
   constexpr uint64_t kQ = Q_MN ? 128 : 2, kP = P_MN ? 128 : 2;  // 16 values of r, in the descriptors' units
   const uint32_t idesc = d.fmt | (static_cast<uint32_t>(t.cols >> 3) << 17);
   const uint64_t q0 = Q_MN ? ptx::tc_smem_desc_sw128_mn(base) : ptx::tc_smem_desc_sw128(base);
-  const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(base + 2 * kBoxQ) : ptx::tc_smem_desc_sw128(base + 2 * kBoxQ);
-  const bool two = t.halves == 2;
+  const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(base + kPAt) : ptx::tc_smem_desc_sw128(base + kPAt);
+  const bool two = HALVES == 2 && t.halves == 2;
   const int blocks = d.blocks;
   uint32_t more = 0;  // (the first instruction of a tile overwrites the sums)
 #pragma unroll 1
@@ -348,12 +322,13 @@ __device__ __forceinline__ bool multiply_tile(const PairProduct& d, const PairTi
   return true;
 }
 
-template <bool BF16>
+template <int HALVES, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_constant__ PairParams p) {
+  constexpr int kStages = PairCfg<HALVES>::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - ptx::smem_u32(smem_raw));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kStages * kStage + kEpiWarps * kOut);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kRing + kEpiWarps * kOut);
   const uint32_t full0 = ptx::smem_u32(bars), empty0 = full0 + 8 * kStages, tfull0 = empty0 + 8 * kStages, tempty0 = tfull0 + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -381,18 +356,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
-  PairSchedule sched(p, pair, pairs);
+  PairSchedule<HALVES> sched(p, pair, pairs);
   PairTile t;
   if (warp == kProducer) {
     if (lane == 0) {
-      RingAt at;
+      RingAt<kStages> at;
       const uint32_t bar0 = ptx::mapa(full0, 0);  // the leader's barriers, from either CTA
       bool ok = true;
       while (ok && sched.next(p, t)) {
         const PairProduct& d = p.prod[t.product];
-        ok = d.q_mn   ? load_tile<true, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
-             : d.p_mn ? load_tile<false, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
-                      : load_tile<false, false>(d, t, rank, at, base, full0, empty0, bar0, abort_flag);
+        ok = d.q_mn   ? load_tile<HALVES, true, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
+             : d.p_mn ? load_tile<HALVES, false, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
+                      : load_tile<HALVES, false, false>(d, t, rank, at, base, full0, empty0, bar0, abort_flag);
       }
       // no copy of either CTA may still be in flight when the pair's shared memory is released: wait for the last filling of
       // every slot (slots before at.slot were filled in this round, the others in the round before, if there was one)
@@ -405,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
     __syncwarp();
   } else if (warp == kMma) {
     if (lane == 0 && rank == 0) {
-      RingAt at;
+      RingAt<kStages> at;
       uint32_t used0 = 0, used1 = 0;  // tiles (or halves) that each buffer of sums has held
       int turn = 0;
       bool ok = true;
@@ -422,9 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
         if (!ok) break;
         ptx::tc_fence_after();
         const uint32_t d0 = tmem_base + static_cast<uint32_t>(buffer * 256), d1 = tmem_base + 256;
-        ok = d.q_mn   ? multiply_tile<true, true>(d, t, at, base, full0, empty0, d0, d1, abort_flag)
-             : d.p_mn ? multiply_tile<false, true>(d, t, at, base, full0, empty0, d0, d1, abort_flag)
-                      : multiply_tile<false, false>(d, t, at, base, full0, empty0, d0, d1, abort_flag);
+        ok = d.q_mn   ? multiply_tile<HALVES, true, true>(d, t, at, base, full0, empty0, d0, d1, abort_flag)
+             : d.p_mn ? multiply_tile<HALVES, false, true>(d, t, at, base, full0, empty0, d0, d1, abort_flag)
+                      : multiply_tile<HALVES, false, false>(d, t, at, base, full0, empty0, d0, d1, abort_flag);
         if (ok) {
           ptx::tc_commit_pair(tfull0 + 8 * buffer);
           if (both) ptx::tc_commit_pair(tfull0 + 8);
@@ -447,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
         ptx::tc_fence_after();
         const int row0 = t.row + h * kHalfJ + static_cast<int>(rank) * kRowsQ + (warp & 3) * 32;
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + static_cast<uint32_t>(b * 256);
-        const uint32_t tile = base + kStages * kStage + warp * kOut;
+        const uint32_t tile = base + kRing + warp * kOut;
 #pragma unroll 1
         for (int c = (warp >> 2) * 64; c < t.cols; c += 128) {
           if (row0 >= d.J || t.col + c >= d.I) break;  // (nothing of it is inside)
@@ -455,12 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
             finish64<BF16>(d, taddr + c, tile, lane, row0, t.col + c);
           } else {
 #pragma unroll 1
-            for (int q = 0; q < 64; q += 32) {
-              uint32_t r[32];
-              ptx::tmem_ld_32x32(taddr + c + q, r);
-              ptx::tmem_ld_wait();
-              finish32<BF16>(d, row0 + lane, t.col + c + q, r);
-            }
+            for (int q = 0; q < 64; q += 32) finish32<BF16>(d, taddr + c + q, row0 + lane, t.col + c + q);
           }
         }
         ptx::tc_fence_before();
@@ -487,14 +457,14 @@ int operand_map(CUtensorMap* map, const void* base, int dtype, bool mn, int64_t 
 }
 
 // Pairs of CTAs that the device holds at once (asked of the runtime once per device).
-template <bool BF16>
+template <int HALVES, bool BF16>
 int max_pairs(int device, int* out) {
   static std::mutex mutex;
   static int known[64] = {};
   std::lock_guard<std::mutex> lock(mutex);
   int& n = known[device & 63];
   if (n == 0) {
-    auto kernel = linear_pair_kernel<BF16>;
+    auto kernel = linear_pair_kernel<HALVES, BF16>;
     TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
@@ -516,6 +486,7 @@ int max_pairs(int device, int* out) {
   return 0;
 }
 
+template <int HALVES>
 int pair_product(const LinearProduct& lp, PairProduct* d) {
   if (operand_map(&d->map_q, lp.q, lp.dtype, lp.q_mn, lp.J, lp.R, lp.q_mn ? lp.q_sr : lp.q_sj, kRowsQ) != 0 ||
       operand_map(&d->map_p, lp.p, lp.dtype, lp.p_mn, lp.I, lp.R, lp.p_mn ? lp.p_sr : lp.p_si, 64) != 0)
@@ -529,7 +500,7 @@ int pair_product(const LinearProduct& lp, PairProduct* d) {
   d->J = static_cast<int>(lp.J);
   d->blocks = static_cast<int>(ceil_div(lp.R, kStepR));
   d->tiles_i = static_cast<int>(ceil_div(lp.I, kTileI));
-  d->tiles_j = static_cast<int>(ceil_div(lp.J, kTileJ));
+  d->tiles_j = static_cast<int>(ceil_div(lp.J, PairCfg<HALVES>::kTileJ));
   TVB_REQUIRE(static_cast<int64_t>(d->tiles_i) * d->tiles_j < (int64_t(1) << 28), "tvb_linear: too many output tiles");
   d->tiles = d->tiles_i * d->tiles_j;
   d->q_mn = lp.q_mn;
@@ -549,14 +520,14 @@ int pair_product(const LinearProduct& lp, PairProduct* d) {
   return 0;
 }
 
-template <bool BF16>
+template <int HALVES, bool BF16>
 int pair_run(int device, cudaStream_t stream, const LinearProduct* lp, int count) {
   int pairs = 0;
-  if (max_pairs<BF16>(device, &pairs) != 0) return -1;
+  if (max_pairs<HALVES, BF16>(device, &pairs) != 0) return -1;
   PairParams p{};
   const bool swap = count == 2 && lp[0].R < lp[1].R;  // the longer r first
-  if (count == 2 && pair_product(lp[swap ? 1 : 0], &p.prod[0]) != 0) return -1;
-  if (pair_product(lp[count == 2 && !swap ? 1 : 0], &p.prod[1]) != 0) return -1;
+  if (count == 2 && pair_product<HALVES>(lp[swap ? 1 : 0], &p.prod[0]) != 0) return -1;
+  if (pair_product<HALVES>(lp[count == 2 && !swap ? 1 : 0], &p.prod[1]) != 0) return -1;
   int light = 0;
   if (p.prod[0].tiles % pairs != 0) {
     const int a = p.prod[0].blocks, b = p.prod[1].blocks;
@@ -565,27 +536,31 @@ int pair_run(int device, cudaStream_t stream, const LinearProduct* lp, int count
     p.light_first = p.extra * b < a;
   }
   // Tiles of product 1 beyond whole rounds of pairs: a round of tiles as they are, or rounds of smaller ones. Relative costs of a
-  // step (512, 256 rows x 256 columns, 256 x 128), by the bytes an SM stages: 48, 32 and 24 KB.
+  // step (512 or 256 rows x 256 columns, 256 x 128), by the bytes an SM stages: 48, 32 and 24 KB.
   const int early = std::min(light * p.extra, p.prod[1].tiles), rest = (p.prod[1].tiles - early) % pairs;
-  const int64_t tall = 48, half = ceil_div(2 * rest, pairs) * 32, quarter = ceil_div(4 * rest, pairs) * 24;
+  const int64_t uncut = HALVES == 2 ? 48 : 32, half = ceil_div(HALVES * rest, pairs) * 32, quarter = ceil_div(2 * HALVES * rest, pairs) * 24;
   p.cut_cols = kTileI;
   p.whole = p.prod[1].tiles;
-  if (rest != 0 && std::min(half, quarter) < tall) {
+  if (rest != 0 && std::min(half, quarter) < uncut) {
     p.whole -= rest;
     p.cut_cols = half <= quarter ? kTileI : kTileI / 2;
   }
   if (status_word(device, &p.status) != 0) return -1;
-  const int per_cut = 2 * kTileI / p.cut_cols;
+  const int per_cut = HALVES * kTileI / p.cut_cols;
   const int64_t tiles = static_cast<int64_t>(p.prod[0].tiles) + p.whole + static_cast<int64_t>(p.prod[1].tiles - p.whole) * per_cut;
   pairs = static_cast<int>(std::min<int64_t>(pairs, tiles));
-  return launch_dependent_cluster("linear_pair", linear_pair_kernel<BF16>, 2, dim3(2 * static_cast<unsigned>(pairs)), dim3(kThreads), kSmemBytes,
+  return launch_dependent_cluster("linear_pair", linear_pair_kernel<HALVES, BF16>, 2, dim3(2 * static_cast<unsigned>(pairs)), dim3(kThreads), kSmemBytes,
                                   stream, p);
 }
 
 }  // namespace
 
 int linear_pair(int device, cudaStream_t stream, const LinearProduct* lp, int count) {
-  return lp[0].dtype == TVB_BF16 ? pair_run<true>(device, stream, lp, count) : pair_run<false>(device, stream, lp, count);
+  // Tiles of 512 rows for a long r, whose sums are read back seldom enough (us, 512 / 256 rows: 8192^3 811 / 850, dx of 2048 x 4096 x
+  // 14336 with its 14336 values of r 185 / 199, y with 4096 208 / 198, dw with 2048 214 / 202, both gradients at once 395 / 383).
+  const bool tall = count == 1 && lp[0].R >= 8192;
+  if (tall) return lp[0].dtype == TVB_BF16 ? pair_run<2, true>(device, stream, lp, count) : pair_run<2, false>(device, stream, lp, count);
+  return lp[0].dtype == TVB_BF16 ? pair_run<1, true>(device, stream, lp, count) : pair_run<1, false>(device, stream, lp, count);
 }
 
 }  // namespace tvb

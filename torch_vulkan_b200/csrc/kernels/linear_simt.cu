@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) linear_simt_kernel(const LinearProduct p)
       float z = acc[a][b];
       if (p.bias != nullptr) z += load_float<TVB_F32>(p.bias, i);
       if (p.preact != nullptr) store_float<TVB_F32>(p.preact, j * p.I + i, z);
-      float y = act_value<false>(z, p.activation);
+      float y = act_value(z, p.activation);
       if (p.residual != nullptr) y += load_float<TVB_F32>(p.residual, j * p.residual_ld + i);
       store_float<TVB_F32>(p.out, j * p.I + i, y);
     }

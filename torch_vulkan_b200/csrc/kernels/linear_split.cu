@@ -56,36 +56,27 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 
 // Four neighbouring outputs (i ... i + 3, row j).
 template <bool BF16>
-__device__ __forceinline__ void finish4(const SplitParams& p, int64_t j, int i, float4 s) {
-  float z[4] = {s.x, s.y, s.z, s.w}, y[4];
-  const int64_t o = j * p.I + i;
-  if (p.vector_ok) {  // (I a multiple of 4, every pointer and row on 8 bytes)
-    if (p.bias != nullptr) {
-      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.bias) + i);
-      const float2 b0 = unpack16<BF16>(b.x), b1 = unpack16<BF16>(b.y);
-      z[0] += b0.x; z[1] += b0.y; z[2] += b1.x; z[3] += b1.y;
+__device__ __forceinline__ void finish4(const SplitParams& p, int64_t j, int i, uint64_t (&z)[2]) {
+  const int64_t o = j * p.I + i, r = j * p.residual_ld + i;
+  const int count = p.I - i;
+  auto add = [&](const void* src, int64_t at) {
+    if (p.vector_ok) {  // (I a multiple of 4, every pointer and row on 8 bytes)
+      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(src) + at);
+      z[0] = ptx::add_f32x2(z[0], unpack16<BF16>(b.x));
+      z[1] = ptx::add_f32x2(z[1], unpack16<BF16>(b.y));
+    } else {
+      add_singly<BF16>(src, at, count, z);
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = act_value<true>(z[e], p.activation);
-    if (p.residual != nullptr) {
-      const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + j * p.residual_ld + i);
-      const float2 r0 = unpack16<BF16>(r.x), r1 = unpack16<BF16>(r.y);
-      y[0] += r0.x; y[1] += r0.y; y[2] += r1.x; y[3] += r1.y;
-    }
-    if (p.preact != nullptr)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.preact) + o) = make_uint2(pack16<BF16>(z[0], z[1]), pack16<BF16>(z[2], z[3]));
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = make_uint2(pack16<BF16>(y[0], y[1]), pack16<BF16>(y[2], y[3]));
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    if (i + e >= p.I) break;
-    if (p.bias != nullptr) z[e] += load16<BF16>(p.bias, i + e);
-    y[e] = act_value<true>(z[e], p.activation);
-    if (p.residual != nullptr) y[e] += load16<BF16>(p.residual, j * p.residual_ld + i + e);
-    if (p.preact != nullptr) store16<BF16>(p.preact, o + e, z[e]);
-    store16<BF16>(p.out, o + e, y[e]);
-  }
+  };
+  auto put = [&](void* dst) {
+    if (p.vector_ok) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dst) + o) = make_uint2(pack16<BF16>(z[0]), pack16<BF16>(z[1]));
+    else store_singly<BF16>(dst, o, count, z);
+  };
+  if (p.bias != nullptr) add(p.bias, i);
+  if (p.preact != nullptr) put(p.preact);
+  activate_pairs(z, p.activation);
+  if (p.residual != nullptr) add(p.residual, r);
+  put(p.out);
 }
 
 template <int TN, bool P_MN, bool Q_MN, bool BF16>
@@ -210,11 +201,12 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
       const int j = c0 + (e >> 5), i = (e & 31) * 4;
       if (j0 + j >= p.J || i0 + i >= p.I) continue;
       const uint32_t at = base + j * (kRows * 4) + i * 4;
-      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      uint64_t s[2] = {0, 0};
 #pragma unroll 4
       for (uint32_t g = 0; g < parts; g++) {
         const float4 v = ld_cluster_f4(ptx::mapa(at, g));
-        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        s[0] = ptx::add_f32x2(s[0], ptx::pack_f32x2(__float_as_uint(v.x), __float_as_uint(v.y)));
+        s[1] = ptx::add_f32x2(s[1], ptx::pack_f32x2(__float_as_uint(v.z), __float_as_uint(v.w)));
       }
       finish4<BF16>(p, j0 + j, i0 + i, s);
     }
