@@ -48,35 +48,40 @@ struct SplitParams {
   int* status;
 };
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {  // (from mapa)
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
 
-// Four neighbouring outputs (i ... i + 3, row j).
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four neighbouring outputs (i ... i + 3, row j) from their sums; `bias`: those outputs' (0 where there is none).
 template <bool BF16>
-__device__ __forceinline__ void finish4(const SplitParams& p, int64_t j, int i, uint64_t (&z)[2]) {
-  const int64_t o = j * p.I + i, r = j * p.residual_ld + i;
-  const int count = p.I - i;
-  auto add = [&](const void* src, int64_t at) {
-    if (p.vector_ok) {  // (I a multiple of 4, every pointer and row on 8 bytes)
-      const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(src) + at);
-      z[0] = ptx::add_f32x2(z[0], unpack16<BF16>(b.x));
-      z[1] = ptx::add_f32x2(z[1], unpack16<BF16>(b.y));
-    } else {
-      add_singly<BF16>(src, at, count, z);
+__device__ __forceinline__ void finish4(const SplitParams& p, int64_t j, int i, const uint64_t (&bias)[2], uint64_t (&z)[2]) {
+  const int64_t o = j * p.I + i;
+  z[0] = ptx::add_f32x2(z[0], bias[0]);
+  z[1] = ptx::add_f32x2(z[1], bias[1]);
+  if (p.vector_ok) {  // (I a multiple of 4, every pointer and row on 8 bytes)
+    if (p.preact != nullptr) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.preact) + o) = make_uint2(pack16<BF16>(z[0]), pack16<BF16>(z[1]));
+    activate_pairs(z, p.activation);
+    if (p.residual != nullptr) {
+      const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + j * p.residual_ld + i);
+      z[0] = ptx::add_f32x2(z[0], unpack16<BF16>(r.x));
+      z[1] = ptx::add_f32x2(z[1], unpack16<BF16>(r.y));
     }
-  };
-  auto put = [&](void* dst) {
-    if (p.vector_ok) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(dst) + o) = make_uint2(pack16<BF16>(z[0]), pack16<BF16>(z[1]));
-    else store_singly<BF16>(dst, o, count, z);
-  };
-  if (p.bias != nullptr) add(p.bias, i);
-  if (p.preact != nullptr) put(p.preact);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = make_uint2(pack16<BF16>(z[0]), pack16<BF16>(z[1]));
+    return;
+  }
+  const int count = p.I - i;
+  if (p.preact != nullptr) store_singly<BF16>(p.preact, o, count, z);
   activate_pairs(z, p.activation);
-  if (p.residual != nullptr) add(p.residual, r);
-  put(p.out);
+  if (p.residual != nullptr) add_singly<BF16>(p.residual, j * p.residual_ld + i, count, z);
+  store_singly<BF16>(p.out, o, count, z);
 }
 
 template <int TN, bool P_MN, bool Q_MN, bool BF16>
@@ -121,53 +126,64 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
+  // (The two threads below set the pace of the whole kernel: no index arithmetic in their loops.)
   if (warp == kProducer) {
     if (lane == 0) {
-      bool ok = true;
-      int it = 0;
-      for (int kb = kb0; kb < kb1; kb++, it++) {
-        const int s = it % Cfg::kStages;
-        ok = ptx::mbar_wait(empty0 + 8 * s, static_cast<uint32_t>((it / Cfg::kStages) & 1) ^ 1u, abort_flag);
-        if (!ok) break;
-        const uint32_t dst = base + s * Cfg::kStage, bar = full0 + 8 * s;
+      uint32_t slot = 0, phase = 0;
+      int r = kb0 * kStepR;
+#pragma unroll 1
+      for (int kb = kb0; kb < kb1; kb++, r += kStepR) {
+        const uint32_t dst = base + slot * Cfg::kStage, bar = full0 + 8 * slot;
+        if (!ptx::mbar_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag)) break;
         ptx::mbar_expect_tx(bar, Cfg::kStage);
         if (P_MN) {
-          for (int c = 0; c < kRows / 64; c++) ptx::tma_load_2d(dst + c * 8192, &map_p, i0 + c * 64, kb * kStepR, bar);
+#pragma unroll
+          for (int c = 0; c < kRows / 64; c++) ptx::tma_load_2d(dst + c * 8192, &map_p, i0 + c * 64, r, bar);
         } else {
-          ptx::tma_load_2d(dst, &map_p, kb * kStepR, i0, bar);
+          ptx::tma_load_2d(dst, &map_p, r, i0, bar);
         }
         if (Q_MN) {
-          for (int c = 0; c < TN / 64; c++)
-            ptx::tma_load_2d(dst + Cfg::kStageP + c * 8192, &map_q, j0 + c * 64, kb * kStepR, bar);
+#pragma unroll
+          for (int c = 0; c < TN / 64; c++) ptx::tma_load_2d(dst + Cfg::kStageP + c * 8192, &map_q, j0 + c * 64, r, bar);
         } else {
-          ptx::tma_load_2d(dst + Cfg::kStageP, &map_q, kb * kStepR, j0, bar);
+          ptx::tma_load_2d(dst + Cfg::kStageP, &map_q, r, j0, bar);
+        }
+        if (++slot == Cfg::kStages) {
+          slot = 0;
+          phase ^= 1u;
         }
       }
-      // no copy may still be in flight when the ring is used for the sums or released
-      for (int j = it > Cfg::kStages ? it - Cfg::kStages : 0; j < it; j++) {
+      // no copy may still be in flight when the ring is used for the sums or released: the last filling of every slot
+      const int filled = (kb1 - kb0) < Cfg::kStages ? kb1 - kb0 : Cfg::kStages;
+      for (int s = 0; s < filled; s++) {
         volatile int never = 0;
-        ptx::mbar_wait(full0 + 8 * (j % Cfg::kStages), static_cast<uint32_t>((j / Cfg::kStages) & 1), &never);
+        ptx::mbar_wait(full0 + 8 * s, s < static_cast<int>(slot) ? phase : phase ^ 1u, &never);
       }
     }
     __syncwarp();
   } else if (warp == kMma) {
     if (lane == 0) {
-      bool ok = true;
-      int it = 0;
-      for (int kb = kb0; kb < kb1; kb++, it++) {
-        const int s = it % Cfg::kStages;
-        ok = ptx::mbar_wait(full0 + 8 * s, static_cast<uint32_t>((it / Cfg::kStages) & 1), abort_flag);
+      constexpr uint64_t kP = P_MN ? 128 : 2, kQ = Q_MN ? 128 : 2;  // 16 values of r, in the descriptors' units
+      const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(base) : ptx::tc_smem_desc_sw128(base);
+      const uint64_t q0 = Q_MN ? ptx::tc_smem_desc_sw128_mn(base + Cfg::kStageP) : ptx::tc_smem_desc_sw128(base + Cfg::kStageP);
+      uint32_t slot = 0, phase = 0, more = 0;
+      bool ok = kb1 > kb0;
+#pragma unroll 1
+      for (int kb = kb0; kb < kb1; kb++) {
+        ok = ptx::mbar_wait(full0 + 8 * slot, phase, abort_flag);
         if (!ok) break;
         ptx::tc_fence_after();
-        const uint32_t at = base + s * Cfg::kStage;
-        const uint64_t pd = P_MN ? ptx::tc_smem_desc_sw128_mn(at) : ptx::tc_smem_desc_sw128(at);
-        const uint64_t qd = Q_MN ? ptx::tc_smem_desc_sw128_mn(at + Cfg::kStageP) : ptx::tc_smem_desc_sw128(at + Cfg::kStageP);
+        const uint64_t pd = p0 + slot * (Cfg::kStage >> 4), qd = q0 + slot * (Cfg::kStage >> 4);
 #pragma unroll
-        for (int j = 0; j < kStepR / 16; j++)
-          ptx::tc_mma<2>(tmem, pd + (P_MN ? 128 : 2) * j, qd + (Q_MN ? 128 : 2) * j, p.idesc, (it | j) != 0 ? 1u : 0u);
-        ptx::tc_commit(empty0 + 8 * s);
+        for (int j = 0; j < kStepR / 16; j++) ptx::tc_mma<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
+        more = 1;
+        ptx::tc_commit(empty0 + 8 * slot);
+        if (++slot == Cfg::kStages) {
+          slot = 0;
+          phase ^= 1u;
+        }
       }
-      if (ok && it != 0) ptx::tc_commit(tfull);
+      if (ok) ptx::tc_commit(tfull);
     }
     __syncwarp();
   } else {
@@ -176,16 +192,30 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
     ptx::tc_fence_after();
     const uint32_t dst = base + (warp * 32 + lane) * 4;
     if (ok) {
-#pragma unroll 1
-      for (int c = 0; c < TN; c += 16) {
+      const uint32_t from = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+      if (empty) {
+#pragma unroll 4
+        for (int c = 0; c < TN; c++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + c * (kRows * 4)), "r"(0u) : "memory");
+      } else if constexpr (TN == 16) {
         uint32_t r[16];
-        if (!empty) {
-          ptx::tmem_ld_32x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + c, r);
-          ptx::tmem_ld_wait();
-        }
+        ptx::tmem_ld_32x16(from, r);
+        ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; e++)
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (c + e) * (kRows * 4)), "r"(empty ? 0u : r[e]) : "memory");
+        for (int e = 0; e < 16; e++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + e * (kRows * 4)), "r"(r[e]) : "memory");
+      } else {
+        constexpr int kAtOnce = TN < 64 ? TN : 64;
+#pragma unroll 1
+        for (int c = 0; c < TN; c += kAtOnce) {
+          uint32_t r[kAtOnce / 32][32];
+#pragma unroll
+          for (int h = 0; h < kAtOnce / 32; h++) ptx::tmem_ld_32x32(from + c + 32 * h, r[h]);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int h = 0; h < kAtOnce / 32; h++)
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + (c + 32 * h + e) * (kRows * 4)), "r"(r[h][e]) : "memory");
+        }
       }
     }
     ptx::tc_fence_before();
@@ -197,18 +227,38 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
   }
   if (*abort_flag == 0) {
     const int c0 = TN * static_cast<int>(part) / static_cast<int>(parts), c1 = TN * (static_cast<int>(part) + 1) / static_cast<int>(parts);
-    for (int e = threadIdx.x; e < (c1 - c0) * 32; e += kThreads) {
-      const int j = c0 + (e >> 5), i = (e & 31) * 4;
-      if (j0 + j >= p.J || i0 + i >= p.I) continue;
-      const uint32_t at = base + j * (kRows * 4) + i * 4;
-      uint64_t s[2] = {0, 0};
+    // A lane keeps its four values of i, a warp takes every sixth column; four columns at a time, because the sums come from
+    // other SMs and one after the other each would wait for a trip there.
+    constexpr int kAtOnce = 4, kWarps = kThreads / 32;
+    const int i = i0 + lane * 4, end = c1 < p.J - j0 ? c1 : p.J - j0;
+    if (i < p.I) {
+      uint64_t bias[2] = {};
+      if (p.bias != nullptr) add_singly<BF16>(p.bias, i, p.I - i, bias);
+      const uint32_t at = base + lane * 16;
+#pragma unroll 1
+      for (int j = c0 + warp; j < end; j += kAtOnce * kWarps) {
+        uint64_t s[kAtOnce][2] = {};
+        auto add = [&](int u, const float4& v) {
+          s[u][0] = ptx::add_f32x2(s[u][0], ptx::pack_f32x2(__float_as_uint(v.x), __float_as_uint(v.y)));
+          s[u][1] = ptx::add_f32x2(s[u][1], ptx::pack_f32x2(__float_as_uint(v.z), __float_as_uint(v.w)));
+        };
+        if (parts == 1) {  // (as an address of the cluster a CTA's own sums would take the trip all the same)
+#pragma unroll
+          for (int u = 0; u < kAtOnce; u++)
+            if (j + u * kWarps < end) add(u, ld_shared_f4(at + (j + u * kWarps) * (kRows * 4)));
+        } else {
 #pragma unroll 4
-      for (uint32_t g = 0; g < parts; g++) {
-        const float4 v = ld_cluster_f4(ptx::mapa(at, g));
-        s[0] = ptx::add_f32x2(s[0], ptx::pack_f32x2(__float_as_uint(v.x), __float_as_uint(v.y)));
-        s[1] = ptx::add_f32x2(s[1], ptx::pack_f32x2(__float_as_uint(v.z), __float_as_uint(v.w)));
+          for (uint32_t g = 0; g < parts; g++) {
+            const uint32_t there = ptx::mapa(at, g);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++)
+              if (j + u * kWarps < end) add(u, ld_cluster_f4(there + (j + u * kWarps) * (kRows * 4)));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++)
+          if (j + u * kWarps < end) finish4<BF16>(p, j0 + j + u * kWarps, i, bias, s[u]);
       }
-      finish4<BF16>(p, j0 + j, i0 + i, s);
     }
   } else if (threadIdx.x == 0) {
     atomicExch(p.status, 2);
