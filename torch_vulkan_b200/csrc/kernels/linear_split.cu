@@ -1,13 +1,15 @@
 // The 16-bit products of linear.h on tcgen05 when the output is small: few rows (decoding, short prompts), or gradients with few
-// tiles. Bound by the bytes of P (the weights) or by latency, so what counts is that every SM streams.
+// tiles. Bound by the bytes of P (the weights), by what the SMs can fetch from the L2, or by latency.
 //
-// One CTA multiplies a tile of 128 values of i (the MMA's 128 rows) by TN values of j (its columns; TN the smallest of 16 ...
-// 256 that holds the rows), over a slice of r; a cluster of S CTAs shares a tile, each with 1 / S of r. S is what makes a
-// product of 32 tiles fill 148 SMs. The CTAs leave their float32 sums in their own shared memory, and each adds up, in rank order,
-// 1 / S of the tile's columns of all S through distributed shared memory: no scratch in global memory, no counters and no
-// atomics, so a launch repeats its results bit for bit and launches share nothing.
+// One CTA multiplies a tile of 128 values of i (the MMA's 128 rows) by TN values of j (its columns; the rows of a decoding step
+// are 16 of them or more), over a slice of r; S slices in a cluster share a tile. S is what makes a product of 32 tiles fill 148
+// SMs. The CTAs leave their float32 sums in their own shared memory, and each adds up, in rank order, 1 / S of the tile's columns
+// of all S through distributed shared memory: no scratch in global memory, no counters and no atomics, so a launch repeats
+// its results bit for bit and launches share nothing.
+// From TN = 64 on two CTAs (the SMs of a TPC) work as a pair on 256 values of i (tcgen05 cta_group::2): each stages its 128 rows
+// of P and half of Q, so an SM fetches 32 KB per 64 values of r instead of 48 at TN = 256 (24 instead of 32 at 128).
 //   warp 4, one lane: TMA (128-byte swizzle) into a ring of stages of 64 values of r
-//   warp 5, one lane: tcgen05.mma (M = 128, N = TN, K = 16; float32 sums in TMEM); the warp owns the TMEM
+//   warp 5, one lane (of the pair's first CTA): tcgen05.mma, float32 sums in TMEM; the warp owns the TMEM
 //   warps 0-3: TMEM -> shared memory; then all warps: sums, bias, activation, residual, store
 // An operand may be contiguous along r (K-major) or along i / j (MN-major: the transposed reads of the backward pass).
 // Up to TN = 128 the ring is kept under half of an SM's shared memory: two CTAs per SM, so that one streams while the other is
@@ -28,7 +30,10 @@ constexpr int kRows = 128, kStepR = 64, kThreads = 192, kProducer = 4, kMma = 5;
 
 template <int TN>
 struct SplitCfg {
-  static constexpr int kStageP = kRows * 128, kStageQ = TN * 128, kStage = kStageP + kStageQ;
+  static constexpr bool kPair = TN >= 64;
+  static constexpr int kTileI = kPair ? 2 * kRows : kRows;  // of the pair
+  static constexpr int kRowsQ = kPair ? TN / 2 : TN;        // values of j that a CTA stages
+  static constexpr int kStageP = kRows * 128, kStageQ = kRowsQ * 128, kStage = kStageP + kStageQ;
   static constexpr int kBudget = TN <= 128 ? 100 * 1024 : 200 * 1024;
   static constexpr int kStages = kBudget / kStage < 8 ? kBudget / kStage : 8;
   static constexpr int kCtasPerSm = TN <= 128 ? 2 : 1;
@@ -60,35 +65,112 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
   return v;
 }
 
-// Four neighbouring outputs (i ... i + 3, row j) from their sums; `bias`: those outputs' (0 where there is none).
-template <bool BF16>
-__device__ __forceinline__ void finish4(const SplitParams& p, int64_t j, int i, const uint64_t (&bias)[2], uint64_t (&z)[2]) {
-  const int64_t o = j * p.I + i;
-  z[0] = ptx::add_f32x2(z[0], bias[0]);
-  z[1] = ptx::add_f32x2(z[1], bias[1]);
-  if (p.vector_ok) {  // (I a multiple of 4, every pointer and row on 8 bytes)
-    if (p.preact != nullptr) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.preact) + o) = make_uint2(pack16<BF16>(z[0]), pack16<BF16>(z[1]));
-    activate_pairs(z, p.activation);
-    if (p.residual != nullptr) {
-      const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.residual) + j * p.residual_ld + i);
-      z[0] = ptx::add_f32x2(z[0], unpack16<BF16>(r.x));
-      z[1] = ptx::add_f32x2(z[1], unpack16<BF16>(r.y));
+// How a warp finishes its columns of a tile. The sums of column j (of the tile) lie at `at` + j rows of shared memory in each of
+// the `parts` CTAs of ranks first_rank, first_rank + rank_step, ...
+struct Finish {
+  uint32_t at, parts, first_rank, rank_step;
+  int i;            // the lane's first output
+  int64_t row0;     // row of the output that column 0 is
+  uint64_t bias[2];
+};
+
+constexpr int kWarps = kThreads / 32;
+
+// U columns, j, j + kWarps, ...: four neighbouring outputs of each. There are few warps here and every instruction waits for the
+// one before it, so the U columns go through each step together, without branches between them (with a branch for each of four
+// columns, a tile of 256 took 11 us to leave).
+template <bool BF16, int ACT, int U>
+__device__ __forceinline__ void finish_columns(const SplitParams& p, const Finish& f, int j) {
+  uint64_t s[U][2] = {};
+  auto add = [&](int u, const float4& v) {
+    s[u][0] = ptx::add_f32x2(s[u][0], ptx::pack_f32x2(__float_as_uint(v.x), __float_as_uint(v.y)));
+    s[u][1] = ptx::add_f32x2(s[u][1], ptx::pack_f32x2(__float_as_uint(v.z), __float_as_uint(v.w)));
+  };
+  const uint32_t mine = f.at + j * (kRows * 4);
+  if (f.parts == 1) {  // (as an address of the cluster a CTA's own sums would take the trip all the same)
+#pragma unroll
+    for (int u = 0; u < U; u++) add(u, ld_shared_f4(mine + u * kWarps * (kRows * 4)));
+  } else {
+#pragma unroll 1
+    for (uint32_t g0 = 0; g0 < f.parts; g0 += 4) {  // (four CTAs' sums asked for at a time)
+      float4 v[4][U];
+#pragma unroll
+      for (uint32_t g = 0; g < 4; g++) {
+        const bool there = g0 + g < f.parts;
+        const uint32_t from = ptx::mapa(mine, f.first_rank + (there ? g0 + g : g0) * f.rank_step);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          v[g][u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (there) v[g][u] = ld_cluster_f4(from + u * kWarps * (kRows * 4));
+        }
+      }
+#pragma unroll
+      for (uint32_t g = 0; g < 4; g++)
+#pragma unroll
+        for (int u = 0; u < U; u++) add(u, v[g][u]);
     }
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = make_uint2(pack16<BF16>(z[0]), pack16<BF16>(z[1]));
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    s[u][0] = ptx::add_f32x2(s[u][0], f.bias[0]);
+    s[u][1] = ptx::add_f32x2(s[u][1], f.bias[1]);
+  }
+  const int64_t row = f.row0 + j, step = static_cast<int64_t>(kWarps) * p.I;
+  const int64_t o = row * p.I + f.i;
+  if (p.vector_ok) {  // (I a multiple of 4, every pointer and row on 8 bytes)
+    auto put = [&](void* dst) {
+      uint16_t* to = static_cast<uint16_t*>(dst) + o;
+#pragma unroll
+      for (int u = 0; u < U; u++, to += step) *reinterpret_cast<uint2*>(to) = make_uint2(pack16<BF16>(s[u][0]), pack16<BF16>(s[u][1]));
+    };
+    if (p.preact != nullptr) put(p.preact);
+#pragma unroll
+    for (int u = 0; u < U; u++) s[u][0] = act_pair<ACT>(s[u][0]), s[u][1] = act_pair<ACT>(s[u][1]);
+    if (p.residual != nullptr) {
+      const uint16_t* from = static_cast<const uint16_t*>(p.residual) + row * p.residual_ld + f.i;
+      uint2 r[U];
+#pragma unroll
+      for (int u = 0; u < U; u++, from += kWarps * p.residual_ld) r[u] = *reinterpret_cast<const uint2*>(from);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        s[u][0] = ptx::add_f32x2(s[u][0], unpack16<BF16>(r[u].x));
+        s[u][1] = ptx::add_f32x2(s[u][1], unpack16<BF16>(r[u].y));
+      }
+    }
+    put(p.out);
     return;
   }
-  const int count = p.I - i;
-  if (p.preact != nullptr) store_singly<BF16>(p.preact, o, count, z);
-  activate_pairs(z, p.activation);
-  if (p.residual != nullptr) add_singly<BF16>(p.residual, j * p.residual_ld + i, count, z);
-  store_singly<BF16>(p.out, o, count, z);
+  const int count = p.I - f.i;
+#pragma unroll 1
+  for (int u = 0; u < U; u++) {
+    uint64_t z[2] = {s[0][0], s[0][1]};
+#pragma unroll
+    for (int w = 1; w < U; w++)
+      if (u == w) z[0] = s[w][0], z[1] = s[w][1];
+    if (p.preact != nullptr) store_singly<BF16>(p.preact, o + u * step, count, z);
+    z[0] = act_pair<ACT>(z[0]);
+    z[1] = act_pair<ACT>(z[1]);
+    if (p.residual != nullptr) add_singly<BF16>(p.residual, (row + u * kWarps) * p.residual_ld + f.i, count, z);
+    store_singly<BF16>(p.out, o + u * step, count, z);
+  }
+}
+
+template <bool BF16, int ACT>
+__device__ __forceinline__ void finish_tile(const SplitParams& p, const Finish& f, int j, int end) {
+  constexpr int kAtOnce = 4;
+#pragma unroll 1
+  for (; j + (kAtOnce - 1) * kWarps < end; j += kAtOnce * kWarps) finish_columns<BF16, ACT, kAtOnce>(p, f, j);
+#pragma unroll 1
+  for (; j + kWarps < end; j += 2 * kWarps) finish_columns<BF16, ACT, 2>(p, f, j);
+  if (j < end) finish_columns<BF16, ACT, 1>(p, f, j);
 }
 
 template <int TN, bool P_MN, bool Q_MN, bool BF16>
 __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
     linear_split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const SplitParams p) {
   using Cfg = SplitCfg<TN>;
-  static_assert(!Q_MN || TN >= 64, "an MN-major operand comes in columns of 64 values");
+  static_assert(!Q_MN || Cfg::kRowsQ >= 64, "an MN-major operand comes in columns of 64 values");
+  constexpr bool kPair = Cfg::kPair;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - ptx::smem_u32(smem_raw));
@@ -98,11 +180,13 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint32_t parts;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(parts));
-  const uint32_t part = ptx::cluster_ctarank();
-  const int tile = static_cast<int>(blockIdx.x / parts);
-  const int i0 = tile / p.tiles_j * kRows, j0 = tile % p.tiles_j * TN;
+  uint32_t ctas;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
+  const uint32_t rank = ptx::cluster_ctarank();
+  // half: which CTA of its pair this is; the pair's first CTA (rank `first`) issues its MMAs
+  const uint32_t half = kPair ? rank & 1u : 0u, first = rank - half, part = kPair ? rank >> 1 : rank, parts = kPair ? ctas >> 1 : ctas;
+  const int tile = static_cast<int>(blockIdx.x / ctas);
+  const int i0 = tile / p.tiles_j * Cfg::kTileI + static_cast<int>(half) * kRows, j0 = tile % p.tiles_j * TN;
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.blocks) * part / parts);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.blocks) * (part + 1) / parts);
   if (threadIdx.x == 0) {
@@ -118,9 +202,13 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
     ptx::prefetch_tensormap(&map_p);
     ptx::prefetch_tensormap(&map_q);
   }
-  if (warp == kMma) ptx::tmem_alloc(ptx::smem_u32(tmem_slot), Cfg::kTmemCols);
+  if (warp == kMma) {
+    if (kPair) ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), Cfg::kTmemCols);
+    else ptx::tmem_alloc(ptx::smem_u32(tmem_slot), Cfg::kTmemCols);
+  }
   ptx::tc_fence_before();
   __syncthreads();
+  if (kPair) ptx::cluster_sync();  // both CTAs' barriers exist before either signals the other's
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   ptx::grid_dependency_wait();
@@ -131,22 +219,28 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
     if (lane == 0) {
       uint32_t slot = 0, phase = 0;
       int r = kb0 * kStepR;
+      const int row_q = j0 + static_cast<int>(half) * Cfg::kRowsQ;
+      const uint32_t bars0 = kPair ? ptx::mapa(full0, first) : full0;  // the barriers that count the boxes: the pair's first CTA's
+      auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+        if (kPair) ptx::tma_load_2d_pair(dst, map, x, y, bar);
+        else ptx::tma_load_2d(dst, map, x, y, bar);
+      };
 #pragma unroll 1
       for (int kb = kb0; kb < kb1; kb++, r += kStepR) {
-        const uint32_t dst = base + slot * Cfg::kStage, bar = full0 + 8 * slot;
+        const uint32_t dst = base + slot * Cfg::kStage, bar = bars0 + 8 * slot;
         if (!ptx::mbar_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag)) break;
-        ptx::mbar_expect_tx(bar, Cfg::kStage);
+        if (half == 0) ptx::mbar_expect_tx(full0 + 8 * slot, (kPair ? 2 : 1) * Cfg::kStage);
         if (P_MN) {
 #pragma unroll
-          for (int c = 0; c < kRows / 64; c++) ptx::tma_load_2d(dst + c * 8192, &map_p, i0 + c * 64, r, bar);
+          for (int c = 0; c < kRows / 64; c++) load(dst + c * 8192, &map_p, i0 + c * 64, r, bar);
         } else {
-          ptx::tma_load_2d(dst, &map_p, r, i0, bar);
+          load(dst, &map_p, r, i0, bar);
         }
         if (Q_MN) {
 #pragma unroll
-          for (int c = 0; c < TN / 64; c++) ptx::tma_load_2d(dst + Cfg::kStageP + c * 8192, &map_q, j0 + c * 64, r, bar);
+          for (int c = 0; c < Cfg::kRowsQ / 64; c++) load(dst + Cfg::kStageP + c * 8192, &map_q, row_q + c * 64, r, bar);
         } else {
-          ptx::tma_load_2d(dst + Cfg::kStageP, &map_q, r, j0, bar);
+          load(dst + Cfg::kStageP, &map_q, r, row_q, bar);
         }
         if (++slot == Cfg::kStages) {
           slot = 0;
@@ -155,14 +249,14 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
       }
       // no copy may still be in flight when the ring is used for the sums or released: the last filling of every slot
       const int filled = (kb1 - kb0) < Cfg::kStages ? kb1 - kb0 : Cfg::kStages;
-      for (int s = 0; s < filled; s++) {
+      for (int s = 0; half == 0 && s < filled; s++) {  // (a pair's second CTA stays until the sums are joined)
         volatile int never = 0;
         ptx::mbar_wait(full0 + 8 * s, s < static_cast<int>(slot) ? phase : phase ^ 1u, &never);
       }
     }
     __syncwarp();
   } else if (warp == kMma) {
-    if (lane == 0) {
+    if (lane == 0 && half == 0) {
       constexpr uint64_t kP = P_MN ? 128 : 2, kQ = Q_MN ? 128 : 2;  // 16 values of r, in the descriptors' units
       const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(base) : ptx::tc_smem_desc_sw128(base);
       const uint64_t q0 = Q_MN ? ptx::tc_smem_desc_sw128_mn(base + Cfg::kStageP) : ptx::tc_smem_desc_sw128(base + Cfg::kStageP);
@@ -175,15 +269,22 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
         ptx::tc_fence_after();
         const uint64_t pd = p0 + slot * (Cfg::kStage >> 4), qd = q0 + slot * (Cfg::kStage >> 4);
 #pragma unroll
-        for (int j = 0; j < kStepR / 16; j++) ptx::tc_mma<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
+        for (int j = 0; j < kStepR / 16; j++) {
+          if (kPair) ptx::tc_mma_pair<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
+          else ptx::tc_mma<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
+        }
         more = 1;
-        ptx::tc_commit(empty0 + 8 * slot);
+        if (kPair) ptx::tc_commit_pair_at(empty0 + 8 * slot, first);  // (in both CTAs)
+        else ptx::tc_commit(empty0 + 8 * slot);
         if (++slot == Cfg::kStages) {
           slot = 0;
           phase ^= 1u;
         }
       }
-      if (ok) ptx::tc_commit(tfull);
+      if (ok) {
+        if (kPair) ptx::tc_commit_pair_at(tfull, first);
+        else ptx::tc_commit(tfull);
+      }
     }
     __syncwarp();
   } else {
@@ -223,41 +324,29 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
   ptx::cluster_sync();  // every CTA's sums are in its shared memory
   if (warp == kMma) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, Cfg::kTmemCols);
+    if (kPair) ptx::tmem_dealloc_pair(tmem, Cfg::kTmemCols);
+    else ptx::tmem_dealloc(tmem, Cfg::kTmemCols);
   }
   if (*abort_flag == 0) {
     const int c0 = TN * static_cast<int>(part) / static_cast<int>(parts), c1 = TN * (static_cast<int>(part) + 1) / static_cast<int>(parts);
-    // A lane keeps its four values of i, a warp takes every sixth column; four columns at a time, because the sums come from
-    // other SMs and one after the other each would wait for a trip there.
-    constexpr int kAtOnce = 4, kWarps = kThreads / 32;
-    const int i = i0 + lane * 4, end = c1 < p.J - j0 ? c1 : p.J - j0;
-    if (i < p.I) {
-      uint64_t bias[2] = {};
-      if (p.bias != nullptr) add_singly<BF16>(p.bias, i, p.I - i, bias);
-      const uint32_t at = base + lane * 16;
-#pragma unroll 1
-      for (int j = c0 + warp; j < end; j += kAtOnce * kWarps) {
-        uint64_t s[kAtOnce][2] = {};
-        auto add = [&](int u, const float4& v) {
-          s[u][0] = ptx::add_f32x2(s[u][0], ptx::pack_f32x2(__float_as_uint(v.x), __float_as_uint(v.y)));
-          s[u][1] = ptx::add_f32x2(s[u][1], ptx::pack_f32x2(__float_as_uint(v.z), __float_as_uint(v.w)));
-        };
-        if (parts == 1) {  // (as an address of the cluster a CTA's own sums would take the trip all the same)
-#pragma unroll
-          for (int u = 0; u < kAtOnce; u++)
-            if (j + u * kWarps < end) add(u, ld_shared_f4(at + (j + u * kWarps) * (kRows * 4)));
-        } else {
-#pragma unroll 4
-          for (uint32_t g = 0; g < parts; g++) {
-            const uint32_t there = ptx::mapa(at, g);
-#pragma unroll
-            for (int u = 0; u < kAtOnce; u++)
-              if (j + u * kWarps < end) add(u, ld_cluster_f4(there + (j + u * kWarps) * (kRows * 4)));
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < kAtOnce; u++)
-          if (j + u * kWarps < end) finish4<BF16>(p, j0 + j + u * kWarps, i, bias, s[u]);
+    // a lane keeps its four values of i, a warp takes every sixth column
+    Finish f;
+    f.at = base + lane * 16;
+    f.parts = parts;
+    f.first_rank = kPair ? half : 0;
+    f.rank_step = kPair ? 2 : 1;
+    f.i = i0 + lane * 4;
+    f.row0 = j0;
+    const int j = c0 + warp, end = c1 < p.J - j0 ? c1 : p.J - j0;
+    if (f.i < p.I) {
+      f.bias[0] = f.bias[1] = 0;
+      if (p.bias != nullptr) add_singly<BF16>(p.bias, f.i, p.I - f.i, f.bias);
+      switch (p.activation) {
+        case TVB_ACT_RELU: finish_tile<BF16, TVB_ACT_RELU>(p, f, j, end); break;
+        case TVB_ACT_GELU: finish_tile<BF16, TVB_ACT_GELU>(p, f, j, end); break;
+        case TVB_ACT_GELU_TANH: finish_tile<BF16, TVB_ACT_GELU_TANH>(p, f, j, end); break;
+        case TVB_ACT_SILU: finish_tile<BF16, TVB_ACT_SILU>(p, f, j, end); break;
+        default: finish_tile<BF16, TVB_ACT_NONE>(p, f, j, end); break;
       }
     }
   } else if (threadIdx.x == 0) {
@@ -284,7 +373,7 @@ int split_run(int device, cudaStream_t stream, const LinearProduct& lp, int part
   CUtensorMap map_p, map_q;
   if (lp.R > 0) {
     if (operand_map(&map_p, lp.p, lp.dtype, P_MN ? lp.I : lp.R, P_MN ? lp.R : lp.I, P_MN ? lp.p_sr : lp.p_si, P_MN ? kStepR : kRows) != 0 ||
-        operand_map(&map_q, lp.q, lp.dtype, Q_MN ? lp.J : lp.R, Q_MN ? lp.R : lp.J, Q_MN ? lp.q_sr : lp.q_sj, Q_MN ? kStepR : TN) != 0)
+        operand_map(&map_q, lp.q, lp.dtype, Q_MN ? lp.J : lp.R, Q_MN ? lp.R : lp.J, Q_MN ? lp.q_sr : lp.q_sj, Q_MN ? kStepR : Cfg::kRowsQ) != 0)
       return -1;
   } else {
     map_p = map_q = CUtensorMap{};  // (a product over nothing: no box is ever loaded)
@@ -304,18 +393,19 @@ int split_run(int device, cudaStream_t stream, const LinearProduct& lp, int part
                         reinterpret_cast<uintptr_t>(lp.residual);
   p.vector_ok = (all & 7u) == 0 && lp.I % 4 == 0 && (lp.residual == nullptr || lp.residual_ld % 4 == 0);
   const uint32_t fmt = BF16 ? 1 : 0;
-  p.idesc = ptx::tc_instr_desc(1, fmt, fmt, kRows, TN) | (P_MN ? ptx::kTcAMajorMN : 0u) | (Q_MN ? ptx::kTcBMajorMN : 0u);
+  p.idesc = ptx::tc_instr_desc(1, fmt, fmt, Cfg::kTileI, TN) | (P_MN ? ptx::kTcAMajorMN : 0u) | (Q_MN ? ptx::kTcBMajorMN : 0u);
   if (status_word(device, &p.status) != 0) return -1;
-  const int64_t grid = ceil_div(lp.I, kRows) * p.tiles_j * parts;
+  const int ctas = Cfg::kPair ? 2 * parts : parts;
+  const int64_t grid = ceil_div(lp.I, Cfg::kTileI) * p.tiles_j * ctas;
   if (grid >= (int64_t(1) << 31)) return fail("tvb_linear: too many output tiles");
-  return launch_dependent_cluster("linear_split", kernel, parts, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg::kSmemBytes, stream,
+  return launch_dependent_cluster("linear_split", kernel, ctas, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg::kSmemBytes, stream,
                                   map_p, map_q, p);
 }
 
 template <int TN, bool BF16>
 int split_orders(int device, cudaStream_t stream, const LinearProduct& lp, int parts) {
   if (!lp.q_mn) return lp.p_mn ? split_run<TN, true, false, BF16>(device, stream, lp, parts) : split_run<TN, false, false, BF16>(device, stream, lp, parts);
-  if constexpr (TN >= 64) {
+  if constexpr (TN >= 128) {
     if (lp.p_mn) return split_run<TN, true, true, BF16>(device, stream, lp, parts);
   }
   return fail("tvb_linear: no kernel for this order of the operands");
@@ -324,12 +414,13 @@ int split_orders(int device, cudaStream_t stream, const LinearProduct& lp, int p
 }  // namespace
 
 int linear_split(int device, cudaStream_t stream, const LinearProduct& lp) {
-  int tn = lp.q_mn ? 64 : 16;
+  int tn = lp.q_mn ? 128 : 16;
   while (tn < 256 && tn < lp.J) tn *= 2;
-  const int64_t tiles = ceil_div(lp.I, kRows) * ceil_div(lp.J, tn), blocks = ceil_div(lp.R, kStepR);
+  const bool pair = tn >= 64;
+  const int64_t tiles = ceil_div(lp.I, pair ? 2 * kRows : kRows) * ceil_div(lp.J, tn) * (pair ? 2 : 1), blocks = ceil_div(lp.R, kStepR);
   const int64_t slots = static_cast<int64_t>(sm_count(device)) * (tn <= 128 ? 2 : 1);
   int parts = 1;
-  while (parts < 8 && tiles * parts * 2 <= slots && blocks >= parts * 2 * 4) parts *= 2;
+  while (parts < (pair ? 4 : 8) && tiles * parts * 2 <= slots && blocks >= parts * 2 * 4) parts *= 2;
   const bool bf16 = lp.dtype == TVB_BF16;
   switch (tn) {
     case 16: return bf16 ? split_orders<16, true>(device, stream, lp, parts) : split_orders<16, false>(device, stream, lp, parts);

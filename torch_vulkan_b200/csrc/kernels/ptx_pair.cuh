@@ -57,6 +57,13 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
                : "memory");
 }
 
+// The same for a pair within a larger cluster, whose ranks are `first` and first + 1.
+__device__ __forceinline__ void tc_commit_pair_at(uint32_t bar, uint32_t first) {
+  const uint16_t mask = static_cast<uint16_t>(3u << first);
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask)
+               : "memory");
+}
+
 // KIND 0: kind::f8f6f4, 2: kind::f16. One instruction over the 256 rows of A and the n rows of B that the pair holds (each
 // CTA half of both, at the same shared-memory offsets); issued by one thread of the pair's CTA 0.
 template <int KIND>
