@@ -46,12 +46,9 @@ LinearCopy make_readable(int dtype, const void** p, int64_t rows, int64_t cols, 
   return c;
 }
 
-// Large outputs go to the kernel of CTA pairs, small ones to the one that splits r.
-bool large(const LinearProduct& p) { return p.R > 0 && p.J > 256 && p.I >= 256 && p.I * p.J >= int64_t(48) * 256 * 256; }
-
 int run_product(int device, cudaStream_t stream, const LinearProduct& p) {
   if (p.dtype == TVB_F32) return linear_simt(stream, p);
-  return large(p) ? linear_pair(device, stream, &p, 1) : linear_split(device, stream, p);
+  return linear_large(p) ? linear_pair(device, stream, &p, 1) : linear_split(device, stream, p);
 }
 
 // dz needs a matrix of its own: there is an activation to differentiate, or TMA cannot read dy.
@@ -184,7 +181,7 @@ extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_
     d.I = k; d.J = n; d.R = m;
     d.dtype = dtype;
   }
-  if (count == 2 && dtype != TVB_F32 && large(p[0]) && large(p[1])) return linear_pair(device, stream, p, 2);
+  if (count == 2 && dtype != TVB_F32 && linear_large(p[0]) && linear_large(p[1])) return linear_pair(device, stream, p, 2);
   for (int i = 0; i < count; i++)
     if (run_product(device, stream, p[i]) != 0) return -1;
   return 0;

@@ -16,6 +16,8 @@
 // in its prologue or epilogue.
 #include <cuda.h>
 
+#include <algorithm>
+
 #include "../core/common.h"
 #include "../core/tensormap.h"
 #include "launch.h"
@@ -411,18 +413,65 @@ int split_orders(int device, cudaStream_t stream, const LinearProduct& lp, int p
   return fail("tvb_linear: no kernel for this order of the operands");
 }
 
+// The shape of a launch: which TN and S, and whether the kernel of CTA pairs (linear_pair.cu) is faster. The rule is a model of
+// the time in us, fitted to 1137 measurements of both kernels (1 to 2048 rows, matrices from 512 x 512 to 4096 x 14336, every TN
+// and S): its choices are 2 % slower than the best of each shape on average, 30 % at worst (333 x 4096 x 6144). What it
+// says: a step (64 values of r) takes longer as more SMs ask the L2 at once, and as two CTAs share an SM; a tile's way out takes
+// its time by its columns, more when sums are joined; a second round of CTAs is dear; clusters of more than four CTAs start
+// late, and clusters of whole SMs do not all fit. From 74 tiles of 256 x 256 on (one for every pair of SMs) the pairs' kernel is
+// taken whatever the model says: there the GPU is bound by its power, and fetching less counts for more than in a short run
+// (2048 x 4096 x 14336 with gelu: 215 us against 255).
+struct Shape {
+  int tn, parts;
+  double us;
+};
+
+double split_cost(const LinearProduct& lp, int tn, int parts) {
+  const bool pair = tn >= 64;
+  const double ctas = static_cast<double>(ceil_div(lp.I, pair ? 2 * kRows : kRows) * ceil_div(lp.J, tn) * parts * (pair ? 2 : 1));
+  const double per_sm = tn <= 128 ? 2 : 1, load = ctas / 148, rounds = std::max(1.0, load / per_sm);
+  const double alone = tn <= 32 ? 0.297 : tn == 64 ? 0.264 : tn == 128 ? 0.322 : 0.294;
+  double step = alone * (1 + 0.417 * std::min(1.0, load)) * (1 + 0.678 * std::max(0.0, std::min(load, per_sm) - 1));
+  if (tn == 256 && parts >= 3) step *= 1.792;
+  double us = 2.11 + 0.00994 * tn + rounds * static_cast<double>(ceil_div(ceil_div(lp.R, kStepR), parts)) * step + 6.36 * (rounds - 1);
+  if (parts > 1) us += 0.309 + 0.0116 * tn / parts;
+  if (parts * (pair ? 2 : 1) > 4) us += 1.07;
+  return us;
+}
+
+int64_t pair_tiles(const LinearProduct& lp) { return ceil_div(lp.I, 256) * ceil_div(lp.J, 256); }
+
+double pair_cost(const LinearProduct& lp) {  // (fewer tiles than pairs)
+  return 1.64 + static_cast<double>(ceil_div(lp.R, kStepR)) * (0.486 + 0.0706 * static_cast<double>(pair_tiles(lp)) / 74) + 2.49;
+}
+
+Shape split_shape(const LinearProduct& lp) {
+  const int least = lp.q_mn ? 128 : 16;
+  int fits = least;  // the smallest TN that holds the rows
+  while (fits < 256 && fits < lp.J) fits *= 2;
+  const int64_t blocks = ceil_div(lp.R, kStepR);
+  Shape best{fits, 1, split_cost(lp, fits, 1)};
+  for (int tn = fits; tn >= least && tn * 4 >= fits && tn * 8 >= lp.J; tn /= 2)
+    for (int parts : {1, 2, 3, 4, 6, 8}) {
+      if (parts > 1 && (parts > blocks || (tn >= 64 && parts > 4))) break;
+      const double us = split_cost(lp, tn, parts);
+      if (us < 0.96 * best.us) best = Shape{tn, parts, us};  // (a finer split has to be worth it)
+    }
+  return best;
+}
+
 }  // namespace
 
+bool linear_large(const LinearProduct& lp) {
+  if (lp.R == 0 || lp.J <= 64) return false;
+  return pair_tiles(lp) >= 74 || pair_cost(lp) < split_shape(lp).us;
+}
+
 int linear_split(int device, cudaStream_t stream, const LinearProduct& lp) {
-  int tn = lp.q_mn ? 128 : 16;
-  while (tn < 256 && tn < lp.J) tn *= 2;
-  const bool pair = tn >= 64;
-  const int64_t tiles = ceil_div(lp.I, pair ? 2 * kRows : kRows) * ceil_div(lp.J, tn) * (pair ? 2 : 1), blocks = ceil_div(lp.R, kStepR);
-  const int64_t slots = static_cast<int64_t>(sm_count(device)) * (tn <= 128 ? 2 : 1);
-  int parts = 1;
-  while (parts < (pair ? 4 : 8) && tiles * parts * 2 <= slots && blocks >= parts * 2 * 4) parts *= 2;
+  const Shape s = split_shape(lp);
+  const int parts = s.parts;
   const bool bf16 = lp.dtype == TVB_BF16;
-  switch (tn) {
+  switch (s.tn) {
     case 16: return bf16 ? split_orders<16, true>(device, stream, lp, parts) : split_orders<16, false>(device, stream, lp, parts);
     case 32: return bf16 ? split_orders<32, true>(device, stream, lp, parts) : split_orders<32, false>(device, stream, lp, parts);
     case 64: return bf16 ? split_orders<64, true>(device, stream, lp, parts) : split_orders<64, false>(device, stream, lp, parts);
