@@ -93,7 +93,9 @@ TVB_API void tvb_shutdown(void);
  * (cudaMemcpyAsync semantics otherwise); device->device is stream-ordered. */
 /* Capture of the device's stream into a CUDA graph (for launch-bound loops such as a decoding step): every launcher
  * called between begin and end is recorded instead of run; tvb_graph_launch replays the recording on the stream.
- * Warm every shape once before capturing (first calls allocate scratch and set kernel attributes). */
+ * Warm every shape once before capturing (first calls allocate scratch and set kernel attributes). Memory of the pool that
+ * was allocated, or given back, between begin and end stays with the recording until tvb_graph_destroy: temporaries of the
+ * recorded step are never another tensor's memory while it can be replayed. */
 TVB_API int tvb_graph_begin(int device);
 TVB_API int tvb_graph_end(int device, void** graph_exec);
 TVB_API int tvb_graph_launch(int device, void* graph_exec);

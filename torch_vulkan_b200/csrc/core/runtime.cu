@@ -29,6 +29,7 @@ struct Block {
   void* ptr;
   uint64_t size;
   int device;
+  uint64_t recording;  // the recording (tvb_graph_begin) during which it was allocated, or 0
 };
 
 struct DeviceState {
@@ -50,6 +51,20 @@ struct DeviceState {
   cudaStream_t copy_stream = nullptr;
   cudaEvent_t fork_event = nullptr, join_event = nullptr;
   bool copies_pending = false;
+  // While the stream is being recorded: the recording's number, blocks that were allocated in it and are free again (the rest of
+  // the recording may use them: its kernels run in order), and older blocks that were freed meanwhile (nobody may: a replay
+  // reads them as they are).
+  uint64_t recording = 0;
+  std::multimap<uint64_t, void*> recording_free;
+  std::vector<std::pair<uint64_t, void*>> recording_held;
+};
+
+// What a finished recording keeps out of the pool for as long as it can be replayed: its kernels write to blocks whose tensors
+// are gone (temporaries of the recorded step), and a block given to another tensor meanwhile would be overwritten.
+struct Recording {
+  int device;
+  uint64_t number;
+  std::vector<std::pair<uint64_t, void*>> blocks;
 };
 
 std::mutex g_mutex;
@@ -58,6 +73,8 @@ bool g_counted = false;
 bool g_shutdown = false;
 int g_count = 0;
 uint64_t g_dispatches = 0;
+uint64_t g_recordings = 0;
+std::map<void*, Recording> g_graphs;  // by executable graph
 
 bool env_flag(const char* name) {
   const char* v = std::getenv(name);
@@ -261,13 +278,16 @@ int tvb_alloc(int device, uint64_t nbytes, TvbAlloc* out) {
   if (state_locked(device, &d) != 0) return -1;
   uint64_t size = round_size(nbytes);
   void* ptr = nullptr;
-  // best fit among cached blocks, not wasting more than a quarter of the block
-  auto it = d->free_blocks.lower_bound(size);
-  if (it != d->free_blocks.end() && it->first <= size + size / 4 + 4096) {
+  // best fit among cached blocks, not wasting more than a quarter of the block; in a recording its own free blocks first
+  auto take = [&](std::multimap<uint64_t, void*>& from) {
+    auto it = from.lower_bound(size);
+    if (it == from.end() || it->first > size + size / 4 + 4096) return false;
     size = it->first;
     ptr = it->second;
-    d->free_blocks.erase(it);
-  } else {
+    from.erase(it);
+    return true;
+  };
+  if (!(d->recording != 0 && take(d->recording_free)) && !take(d->free_blocks)) {
     TVB_CUDA(cudaSetDevice(device));
     cudaError_t err = cudaMalloc(&ptr, size);
     if (err == cudaErrorMemoryAllocation) {  // (trim and retry, as memory.rs:171-179)
@@ -284,7 +304,7 @@ int tvb_alloc(int device, uint64_t nbytes, TvbAlloc* out) {
     d->blocks += 1;
   }
   d->allocated += size;
-  Block* b = new Block{ptr, size, device};
+  Block* b = new Block{ptr, size, device, d->recording};
   out->handle = b;
   out->ptr = ptr;
   out->size = size;
@@ -300,8 +320,15 @@ void tvb_free(void* handle) {
     std::lock_guard<std::mutex> lock(g_mutex);
     if (!g_shutdown && b->device < static_cast<int>(g_devices.size())) {
       DeviceState& d = g_devices[b->device];
-      // Later users of the block are queued on the same stream, so reuse is ordered after the last use.
-      d.free_blocks.emplace(b->size, b->ptr);
+      // Later users of the block are queued on the same stream, so reuse is ordered after the last use. What a recording uses
+      // stays with it.
+      Recording* owner = nullptr;
+      for (auto& g : g_graphs)
+        if (b->recording != 0 && g.second.device == b->device && g.second.number == b->recording) owner = &g.second;
+      if (d.recording != 0 && b->recording == d.recording) d.recording_free.emplace(b->size, b->ptr);
+      else if (owner != nullptr) owner->blocks.emplace_back(b->size, b->ptr);
+      else if (d.recording != 0) d.recording_held.emplace_back(b->size, b->ptr);
+      else d.free_blocks.emplace(b->size, b->ptr);
       d.allocated -= b->size;
     }
   }
@@ -505,6 +532,8 @@ int tvb_graph_begin(int device) {
   cudaStream_t s;
   if (enter(device, &s) != 0) return -1;
   TVB_CUDA(cudaStreamBeginCapture(s, cudaStreamCaptureModeRelaxed));
+  std::lock_guard<std::mutex> lock(g_mutex);
+  g_devices[device].recording = ++g_recordings;
   return 0;
 }
 
@@ -512,13 +541,30 @@ int tvb_graph_end(int device, void** graph_exec) {
   TVB_REQUIRE(graph_exec != nullptr, "tvb_graph_end: NULL pointer");
   cudaStream_t s;
   if (enter(device, &s) != 0) return -1;
-  if (tvb_join_copies(device) != 0) return -1;  // a recording cannot end with the copy-out lane still forked off
+  const int joined = tvb_join_copies(device);  // a recording cannot end with the copy-out lane still forked off
   cudaGraph_t graph = nullptr;
-  TVB_CUDA(cudaStreamEndCapture(s, &graph));
   cudaGraphExec_t exec = nullptr;
-  cudaError_t err = cudaGraphInstantiate(&exec, graph, 0);
-  cudaGraphDestroy(graph);
-  if (err != cudaSuccess) return fail_cuda("cudaGraphInstantiate", err);
+  const char* what = "cudaStreamEndCapture";
+  cudaError_t err = joined == 0 ? cudaStreamEndCapture(s, &graph) : cudaSuccess;
+  if (joined == 0 && err == cudaSuccess) {
+    what = "cudaGraphInstantiate";
+    err = cudaGraphInstantiate(&exec, graph, 0);
+    cudaGraphDestroy(graph);
+  }
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    DeviceState& d = g_devices[device];
+    Recording r{device, d.recording, std::move(d.recording_held)};
+    r.blocks.insert(r.blocks.end(), d.recording_free.begin(), d.recording_free.end());
+    d.recording_held.clear();
+    d.recording_free.clear();
+    d.recording = 0;
+    if (joined == 0 && err == cudaSuccess) g_graphs.emplace(exec, std::move(r));
+    else
+      for (auto& b : r.blocks) d.free_blocks.emplace(b.first, b.second);
+  }
+  if (joined != 0) return -1;
+  if (err != cudaSuccess) return fail_cuda(what, err);
   *graph_exec = exec;
   return 0;
 }
@@ -532,7 +578,17 @@ int tvb_graph_launch(int device, void* graph_exec) {
 }
 
 void tvb_graph_destroy(void* graph_exec) {
-  if (graph_exec != nullptr && cudaGraphExecDestroy(static_cast<cudaGraphExec_t>(graph_exec)) != cudaSuccess) cudaGetLastError();
+  if (graph_exec == nullptr) return;
+  {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    auto it = g_graphs.find(graph_exec);
+    if (it != g_graphs.end()) {
+      if (!g_shutdown)  // (replays that are still queued run before whatever takes these blocks next: one stream)
+        for (auto& b : it->second.blocks) g_devices[it->second.device].free_blocks.emplace(b.first, b.second);
+      g_graphs.erase(it);
+    }
+  }
+  if (cudaGraphExecDestroy(static_cast<cudaGraphExec_t>(graph_exec)) != cudaSuccess) cudaGetLastError();
 }
 
 // ---- sharing device memory between the ranks of one node (one process per GPU)

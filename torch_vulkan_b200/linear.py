@@ -13,10 +13,16 @@ which is how the logic is tested without a GPU) and both can hold one rank's sli
 sharded over the GPUs of a node (`shard(rank, world)`): the forward then assembles the full output on every rank.
 `swap_linears` replaces the nn.Linear modules of a model in place; `save` / `load` keep the quantised form on disk so
 that a restart skips the quantisation.
+
+The layers that stay in 16 or 32 bits have a form of their own: `linear_act` (and the module LinearAct) is a Linear with its
+activation and the residual stream it joins in one call, act(x @ weight.T + bias) + residual, with gradients; `fuse_linears`
+puts it in place of the Linear / activation pairs of a model.
 """
 
 import torch
+import torch.nn.functional as F
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import shard as _shard
 
@@ -164,10 +170,126 @@ class DynInt4Linear(nn.Module, _ShardedMixin):
                 + (f", rows {self.rank}/{self.world}" if self.world > 1 else ""))
 
 
+def _rows(t, cols):
+    """A [rows, cols] form of t that the kernels can read: contiguous columns, rows that do not overlap (a copy where there is
+    none, for instance of an expanded gradient)."""
+    t = t.reshape(-1, cols)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+class _LinearAct(torch.autograd.Function):
+    """cabi.linear and cabi.linear_backward as one differentiable operation. Keeps x, the weight and, with an activation, the
+    values before it; only where something needs a gradient."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        from . import cabi
+
+        n, k = weight.shape
+        x2 = _rows(x, k)
+        w2 = _rows(weight, k)
+        r2 = None if residual is None else _rows(residual, n)
+        keep = activation != "none" and any(ctx.needs_input_grad[:3])
+        y = cabi.linear(x2, w2, bias, residual=r2, activation=activation, save_preactivation=keep)
+        y, z = y if keep else (y, None)
+        ctx.save_for_backward(x2, w2, z)
+        ctx.activation, ctx.x_shape = activation, x.shape
+        return y.view(*x.shape[:-1], n)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        from . import cabi
+
+        x2, w2, z = ctx.saved_tensors
+        need = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        if any(need):
+            dx, dw, db = cabi.linear_backward(_rows(dy, w2.shape[0]), x2, w2, z, activation=ctx.activation, need=need)
+        return (None if dx is None else dx.view(ctx.x_shape)), dw, db, (dy if ctx.needs_input_grad[3] else None), None
+
+
+def linear_act(x, weight, bias=None, activation="none", residual=None):
+    """act(x @ weight.T + bias) + residual: x [..., in], weight [out, in], bias [out], residual [..., out], all of one dtype
+    (float32, float16 or bfloat16). activation: "none", "relu", "gelu" (by erf), "gelu_tanh" or "silu". Differentiable (once)
+    in every operand. On "vk" one kernel computes it (tvb_linear; the gradients: tvb_linear_backward); on the CPU PyTorch's own
+    operations do. CUDA tensors take the kernel too, without gradients: PyTorch's autograd engine serves one accelerator per
+    process, and here that is "vk" (cabi.linear_backward computes them when called)."""
+    from . import cabi
+
+    if activation not in cabi.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(cabi.ACTIVATIONS)}, got {activation!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x of shape {tuple(x.shape)} does not go with a weight of shape {tuple(weight.shape)}")
+    if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
+        raise ValueError(f"residual of shape {tuple(residual.shape)} for an output of shape {(*x.shape[:-1], weight.shape[0])}")
+    if x.device.type == "cpu":
+        y = F.linear(x, weight, bias)
+        y = {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"),
+             "silu": F.silu}[activation](y)
+        return y if residual is None else y + residual
+    return _LinearAct.apply(x, weight, bias if bias is None or bias.is_contiguous() else bias.contiguous(), residual, activation)
+
+
+class LinearAct(nn.Linear):
+    """nn.Linear (its parameters, its state dict) with an activation and, in the call, a residual: `linear_act` as a module."""
+
+    def __init__(self, in_features, out_features, bias=True, activation="none", device=None, dtype=None):
+        from . import cabi
+
+        if activation not in cabi.ACTIVATIONS:
+            raise ValueError(f"activation must be one of {', '.join(cabi.ACTIVATIONS)}, got {activation!r}")
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        self.activation = activation
+
+    @classmethod
+    def from_float(cls, linear, activation="none"):
+        """The same layer (it shares `linear`'s parameters) followed by `activation`."""
+        out = cls(linear.in_features, linear.out_features, bias=linear.bias is not None, activation=activation, device="meta")
+        out.weight, out.bias = linear.weight, linear.bias
+        return out.train(linear.training)
+
+    def forward(self, x, residual=None):
+        return linear_act(x, self.weight, self.bias, self.activation, residual)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", activation={self.activation}"
+
+
+def _activation_name(module):
+    """What LinearAct calls an activation module, or None."""
+    if type(module) is nn.ReLU:
+        return "relu"
+    if type(module) is nn.GELU:
+        return "gelu" if module.approximate == "none" else "gelu_tanh"
+    return "silu" if type(module) is nn.SiLU else None
+
+
+def fuse_linears(model):
+    """Replaces, in every nn.Sequential under `model` (in place), an nn.Linear that is followed by ReLU, GELU or SiLU with one
+    LinearAct that shares its parameters, and the activation with nn.Identity (so that the other layers keep their names).
+    Returns the names of the layers it replaced."""
+    replaced = []
+    for name, module in list(model.named_modules()):
+        if not isinstance(module, nn.Sequential):
+            continue
+        children = list(module.named_children())
+        for (first, linear), (second, act) in zip(children, children[1:]):
+            activation = _activation_name(act)
+            if type(linear) is not nn.Linear or activation is None:
+                continue
+            setattr(module, first, LinearAct.from_float(linear, activation))
+            setattr(module, second, nn.Identity())
+            replaced.append(f"{name}.{first}" if name else first)
+    return replaced
+
+
 def swap_linears(model, kind="int8", dtype=torch.bfloat16, block_size=32, device=None, skip=None):
     """Replaces every nn.Linear under `model` (in place) with its quantised counterpart, quantising on the CPU and moving
-    the result to `device`. kind: "int8" (Int8Linear) or "dyn4" (DynInt4Linear). `skip(name, module)` keeps a layer as is.
-    Returns the names of the layers it replaced."""
+    the result to `device`. kind: "int8" (Int8Linear) or "dyn4" (DynInt4Linear). `skip(name, module)` keeps a layer as is; a
+    LinearAct with an activation is kept too (the quantised layers have none). Returns the names of the layers it replaced."""
     if kind not in ("int8", "dyn4"):
         raise ValueError("kind must be 'int8' or 'dyn4'")
     replaced = []
@@ -175,6 +297,8 @@ def swap_linears(model, kind="int8", dtype=torch.bfloat16, block_size=32, device
         for child_name, child in list(module.named_children()):
             full = f"{name}.{child_name}" if name else child_name
             if not isinstance(child, nn.Linear) or (skip is not None and skip(full, child)):
+                continue
+            if isinstance(child, LinearAct) and child.activation != "none":
                 continue
             if kind == "int8":
                 new = Int8Linear.from_float(child, dtype=dtype)
