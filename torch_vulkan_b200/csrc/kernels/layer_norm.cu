@@ -490,19 +490,21 @@ constexpr int kRingCols = 16;  // columns of a thread
 
 // The streamed form: `stages` slots of one row of x and one of dy each. Row number i of this CTA (row blockIdx.x + i *
 // gridDim.x) lies in slot i % stages; the slot of row i - 1 is refilled behind the barrier inside row i's sums, which every thread
-// reaches only after it is done with row i - 1. A row is read from shared memory twice (for the sums, for dx), and the
-// weights lie there too, which leaves the registers to the column sums.
-// Dynamic shared memory: the ring, the weights (as the values, or float32), two buffers for the sums over the warps.
-template <int DT>
-__global__ void __launch_bounds__(1024) layer_norm_backward_ring_kernel(const NormParams p, const int stages, int* status) {
-  constexpr int kSize = DT == TVB_F32 ? 4 : 2, kUnits = kRingCols / 4;
+// reaches only after it is done with row i - 1. A row is read from shared memory twice (for the sums, for dx), which leaves the
+// registers to the column sums and, where they are 16-bit, the weights; others (WIDE: float32) lie in shared memory.
+// With 16-bit rows the instructions are what bounds it (two thirds of the issue slots; they were twice as many with the
+// number of threads a variable, most of them addresses).
+// Dynamic shared memory: the ring, the weights (WIDE), two buffers for the sums over the warps.
+template <int DT, int T, bool WIDE>
+__global__ void __launch_bounds__(T, T > 512 ? 1 : 512 / T) layer_norm_backward_ring_kernel(const NormParams p, const int stages, int* status) {
+  constexpr int kSize = DT == TVB_F32 ? 4 : 2, kUnits = kRingCols / 4, threads = T, warps = T / 32;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t bars[8];
   __shared__ int abort_flag;
-  const int row_bytes = p.d * kSize, t = threadIdx.x, threads = blockDim.x, warps = threads >> 5;
-  const bool wide = DT != TVB_F32 && p.param_dtype == TVB_F32 && p.weight != nullptr;  // weights wider than the values
-  uint8_t* weights = ring + static_cast<size_t>(stages) * 2 * row_bytes;
-  float2* buf = reinterpret_cast<float2*>(weights + (wide ? 4 : kSize) * p.d);
+  const int d = p.d, row_bytes = d * kSize, t = threadIdx.x;
+  const int left = d - 4 * t;  // unit c of this thread (columns 4 (c T + t) ...) exists if left > 4 c T
+  float* weights = reinterpret_cast<float*>(ring + static_cast<size_t>(stages) * 2 * row_bytes);
+  float2* buf = reinterpret_cast<float2*>(weights + (WIDE ? d : 0));
   const uint32_t ring0 = ptx::smem_u32(ring), bar0 = ptx::smem_u32(bars);
   if (t == 0) {
     for (int s = 0; s < stages; s++) ptx::mbar_init(bar0 + 8 * s, 1);
@@ -529,41 +531,58 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_ring_kernel(const No
   if (t == 0)
     while (fetched < count && fetched < stages) fetch(fetched);
   uint64_t dg[kUnits][2] = {}, db[kUnits][2] = {};
+  uint2 kept[kUnits];  // !WIDE: the weights as they are
 #pragma unroll
-  for (int c = 0; c < kUnits; c++) {  // (every thread reads back only what it wrote)
-    const int col = (c * threads + t) * 4;
-    if (col >= p.d) continue;
-    uint64_t g[2];
-    if (p.weight == nullptr) g[0] = g[1] = ptx::both_f32x2(1.0f);
-    else if (wide) load_pairs<TVB_F32>(p.weight, col, g);
-    else load_pairs<DT>(p.weight, col, g);
-    if (wide) store_pairs<TVB_F32>(weights, col, g);
-    else store_pairs<DT>(weights, col, g);
+  for (int c = 0; c < kUnits; c++) {
+    kept[c] = make_uint2(0, 0);
+    if (left <= 4 * c * T) continue;
+    const int col = 4 * (c * T + t);
+    if constexpr (WIDE) {  // (every thread reads back only what it wrote)
+      *reinterpret_cast<float4*>(weights + col) = p.weight != nullptr ? *reinterpret_cast<const float4*>(static_cast<const float*>(p.weight) + col)
+                                                                      : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    } else {
+      const uint32_t one = DT == TVB_BF16 ? 0x3f803f80u : 0x3c003c00u;
+      kept[c] = p.weight != nullptr ? *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.weight) + col) : make_uint2(one, one);
+    }
   }
-  const float inv_d = 1.0f / static_cast<float>(p.d);
-  int64_t row = blockIdx.x;
-  float mean = count > 0 ? p.mean[row] : 0.0f, rstd = count > 0 ? p.rstd[row] : 0.0f;
+  auto weight = [&](int c, uint64_t (&g)[2]) {
+    if constexpr (WIDE) {
+      load_pairs<TVB_F32>(weights, 4 * (c * T + t), g);
+    } else {
+      g[0] = pair16<DT>(kept[c].x);
+      g[1] = pair16<DT>(kept[c].y);
+    }
+  };
+  const float inv_d = 1.0f / static_cast<float>(d);
+  const float* mean_at = p.mean + blockIdx.x;
+  const float* rstd_at = p.rstd + blockIdx.x;
+  uint8_t* y_at = p.y == nullptr ? nullptr : static_cast<uint8_t*>(p.y) + static_cast<int64_t>(blockIdx.x) * row_bytes + t * 4 * kSize;
+  const int64_t y_step = step * row_bytes;
+  float mean = count > 0 ? *mean_at : 0.0f, rstd = count > 0 ? *rstd_at : 0.0f;
   int slot = 0, before = 0;
   uint32_t phase = 0;
+  const uint8_t* mine = ring + t * 4 * kSize;  // this thread's first unit of the row of x in the present slot
+#pragma unroll 1
   for (int i = 0; i < count; i++) {
     float next_mean = 0.0f, next_rstd = 0.0f;  // the next row's statistics are asked for a row ahead
+    mean_at += step;
+    rstd_at += step;
     if (i + 1 < count) {
-      next_mean = p.mean[row + step];
-      next_rstd = p.rstd[row + step];
+      next_mean = *mean_at;
+      next_rstd = *rstd_at;
     }
     ptx::mbar_wait(bar0 + 8 * slot, phase, &abort_flag);  // (no early exit: barriers follow)
-    const uint8_t* xs = ring + 2 * slot * row_bytes;
+    const uint8_t* xs = mine;
+    const uint8_t* ds = mine + row_bytes;
     const uint64_t m2 = ptx::both_f32x2(-mean), r2 = ptx::both_f32x2(rstd);
     uint64_t su2 = 0, sux2 = 0;
-    int col = 4 * t;
 #pragma unroll
-    for (int c = 0; c < kUnits; c++, col += 4 * threads) {
-      if (col >= p.d) continue;
+    for (int c = 0; c < kUnits; c++) {
+      if (left <= 4 * c * T) continue;
       uint64_t x[2], dy[2], g[2];
-      load_pairs<DT>(xs, col, x);
-      load_pairs<DT>(xs + row_bytes, col, dy);
-      if (wide) load_pairs<TVB_F32>(weights, col, g);
-      else load_pairs<DT>(weights, col, g);
+      load_pairs<DT>(xs, 4 * c * T, x);
+      load_pairs<DT>(ds, 4 * c * T, dy);
+      weight(c, g);
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         x[e] = ptx::add_f32x2(x[e], m2);
@@ -577,32 +596,31 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_ring_kernel(const No
     float su = ptx::sum_f32x2(su2), sux = ptx::sum_f32x2(sux2);
     cta_sum2(su, sux, buf + (i & 1) * warps, warps);
     if (t == 0 && i >= 1 && fetched < count) fetch(before);
-    if (p.y != nullptr) {
+    if (y_at != nullptr) {
       // dx = rstd u - rstd <u> - (x - mean) rstd^2 <u h>,  <u h> = rstd <u (x - mean)>
       const uint64_t c0 = ptx::both_f32x2(-su * inv_d * rstd), c1 = ptx::both_f32x2(-(rstd * (rstd * sux * inv_d)) * rstd);
-      uint8_t* out = static_cast<uint8_t*>(p.y) + row * p.d * kSize;
-      col = 4 * t;
 #pragma unroll
-      for (int c = 0; c < kUnits; c++, col += 4 * threads) {
-        if (col >= p.d) continue;
+      for (int c = 0; c < kUnits; c++) {
+        if (left <= 4 * c * T) continue;
         uint64_t x[2], dy[2], g[2];
-        load_pairs<DT>(xs, col, x);
-        load_pairs<DT>(xs + row_bytes, col, dy);
-        if (wide) load_pairs<TVB_F32>(weights, col, g);
-        else load_pairs<DT>(weights, col, g);
+        load_pairs<DT>(xs, 4 * c * T, x);
+        load_pairs<DT>(ds, 4 * c * T, dy);
+        weight(c, g);
 #pragma unroll
         for (int e = 0; e < 2; e++)
           x[e] = ptx::fma_f32x2(ptx::add_f32x2(x[e], m2), c1, ptx::fma_f32x2(dy[e], ptx::mul_f32x2(g[e], r2), c0));
-        store_pairs<DT>(out, col, x);
+        store_pairs<DT>(y_at, 4 * c * T, x);
       }
+      y_at += y_step;
     }
     mean = next_mean;
     rstd = next_rstd;
-    row += step;
     before = slot;
+    mine += 2 * row_bytes;
     if (++slot == stages) {
       slot = 0;
       phase ^= 1u;
+      mine = ring + t * 4 * kSize;
     }
   }
   __syncthreads();
@@ -612,10 +630,10 @@ __global__ void __launch_bounds__(1024) layer_norm_backward_ring_kernel(const No
   float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
   for (int c = 0; c < kUnits; c++) {
-    const int col = (c * threads + t) * 4;
-    if (col >= p.d) continue;
+    if (left <= 4 * c * T) continue;
+    const int col = 4 * (c * T + t);
     store_pairs<TVB_F32>(sums, col, dg[c]);
-    store_pairs<TVB_F32>(sums, p.d + col, db[c]);
+    store_pairs<TVB_F32>(sums, d + col, db[c]);
   }
   ptx::cluster_sync();
   const uint32_t rank = ptx::cluster_ctarank();
@@ -716,18 +734,19 @@ int norm_group(int64_t d, int vals) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// The streamed backward kernel: rows of 512 to 16384 values that fit the shared memory at least twice; 1024 threads per SM, as
-// one CTA or several.
+// The streamed backward kernel: rows of 512 to 16384 values that fit the shared memory at least twice; up to 1024 threads per
+// SM, as one CTA or several. (A few numbers of threads, so that they can be constants of the kernel.)
 struct Ring {
   int threads, per_sm, stages;
   size_t smem;
 };
-Ring ring_shape(int64_t d, int es, int weights_es) {
+Ring ring_shape(int64_t d, int es, bool wide) {
   Ring r{};
   if (d < 512 || d > 1024 * kRingCols || d % 4 != 0) return r;
-  r.threads = static_cast<int>(ceil_div(d, kRingCols * 32) * 32);
-  r.per_sm = std::min(1024 / r.threads, 16);
-  const int64_t rest = d * weights_es + r.threads / 2;  // weights, sums over the warps
+  for (int t : {64, 128, 192, 256, 384, 512, 768, 1024})
+    if (r.threads == 0 && d <= t * kRingCols) r.threads = t;
+  r.per_sm = std::max(512 / r.threads, 1);
+  const int64_t rest = (wide ? d * 4 : 0) + r.threads / 2;  // weights, sums over the warps
   // (228 KB per SM, of which every CTA takes 1 KB for itself and some for its barriers)
   r.stages = static_cast<int>(std::min<int64_t>((228 * 1024 / r.per_sm - 1024 - 128 - rest) / (2 * d * es), 8));
   if (r.stages < 2) return Ring{};
@@ -774,9 +793,9 @@ int backward_vec(cudaStream_t stream, const NormParams& p, int64_t parts) {
   return launch_dependent("layer_norm_backward", kernel, dim3(static_cast<unsigned>(parts)), dim3(t < 128 ? 128 : t), 0, stream, p);
 }
 
-template <int DT>
+template <int DT, int T, bool WIDE>
 int backward_ring(int device, cudaStream_t stream, const NormParams& p, const Ring& r, int64_t ctas) {
-  auto kernel = layer_norm_backward_ring_kernel<DT>;
+  auto kernel = layer_norm_backward_ring_kernel<DT, T, WIDE>;
   static bool configured[64] = {};
   if (!configured[device & 63]) {
     TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 128));
@@ -784,8 +803,22 @@ int backward_ring(int device, cudaStream_t stream, const NormParams& p, const Ri
   }
   int* status = nullptr;
   if (status_word(device, &status) != 0) return -1;
-  return launch_dependent_cluster("layer_norm_backward_ring", kernel, kRingCluster, dim3(static_cast<unsigned>(ctas)),
-                                  dim3(static_cast<unsigned>(r.threads)), r.smem, stream, p, r.stages, status);
+  return launch_dependent_cluster("layer_norm_backward_ring", kernel, kRingCluster, dim3(static_cast<unsigned>(ctas)), dim3(T), r.smem, stream, p,
+                                  r.stages, status);
+}
+
+template <int DT, bool WIDE>
+int backward_ring_threads(int device, cudaStream_t stream, const NormParams& p, const Ring& r, int64_t ctas) {
+  switch (r.threads) {
+    case 64: return backward_ring<DT, 64, WIDE>(device, stream, p, r, ctas);
+    case 128: return backward_ring<DT, 128, WIDE>(device, stream, p, r, ctas);
+    case 192: return backward_ring<DT, 192, WIDE>(device, stream, p, r, ctas);
+    case 256: return backward_ring<DT, 256, WIDE>(device, stream, p, r, ctas);
+    case 384: return backward_ring<DT, 384, WIDE>(device, stream, p, r, ctas);
+    case 512: return backward_ring<DT, 512, WIDE>(device, stream, p, r, ctas);
+    case 768: return backward_ring<DT, 768, WIDE>(device, stream, p, r, ctas);
+    default: return backward_ring<DT, 1024, WIDE>(device, stream, p, r, ctas);
+  }
 }
 
 template <int DT>
@@ -804,11 +837,15 @@ int backward(int device, cudaStream_t stream, const NormParams& p, int64_t* part
   constexpr int kVec = DT == TVB_F32 ? 4 : 8;
   const bool vec = p.d % kVec == 0 && p.x_ld % kVec == 0 && p.dy_ld % kVec == 0 && aligned16(p.x) && aligned16(p.dy) &&
                    aligned16(p.y) && aligned16(p.weight) && aligned16(p.partial);
-  const Ring ring = vec ? ring_shape(p.d, DT == TVB_F32 ? 4 : 2, p.param_dtype == TVB_F32 ? 4 : 2) : Ring{};
+  const bool wide = DT == TVB_F32 || (p.param_dtype == TVB_F32 && p.weight != nullptr);
+  const Ring ring = vec ? ring_shape(p.d, DT == TVB_F32 ? 4 : 2, wide) : Ring{};
   if (ring.stages != 0) {
     const int64_t ctas = ring_ctas(p.rows, ring);
     *parts = ctas / kRingCluster;
-    return backward_ring<DT>(device, stream, p, ring, ctas);
+    if constexpr (DT != TVB_F32) {
+      if (!wide) return backward_ring_threads<DT, false>(device, stream, p, ring, ctas);
+    }
+    return backward_ring_threads<DT, true>(device, stream, p, ring, ctas);
   }
   *parts = norm_parts(p.rows, p.d);
   if (p.d > kLongestBwd) {
@@ -861,7 +898,7 @@ extern "C" int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm
 
 extern "C" uint64_t tvb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d) {
   if (rows <= 0 || d <= 0) return 0;
-  const Ring ring = ring_shape(d, 2, 2);  // (wider rows take as many CTAs or none)
+  const Ring ring = ring_shape(d, 2, false);  // (wider rows take as many CTAs or none)
   const int64_t most = std::max(norm_parts(rows, d), ring.stages != 0 ? ring_ctas(rows, ring) / kRingCluster : 0);
   return static_cast<uint64_t>(most) * 2 * static_cast<uint64_t>(d) * 4;
 }
