@@ -8,7 +8,7 @@
 //
 // Forward: a group of T threads (8 or 32 of a warp, or a CTA) keeps its row in registers between the statistics and the result.
 //
-// Backward: persistent CTAs (1024 threads per SM in all) stream their rows of x and dy through a ring in shared memory by bulk
+// Backward: persistent CTAs (512 threads per SM in all) stream their rows of x and dy through a ring in shared memory by bulk
 // copies, so the next rows are on their way whatever the CTA does with the present ones, and keep the sums of dg and db of their
 // columns in registers over all their rows. A cluster of two CTAs adds its sums through distributed shared memory and
 // leaves one partial row in the workspace; a second kernel adds those in a fixed order (no atomics: the gradients repeat bit for
@@ -486,7 +486,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 constexpr int kRingCluster = 2;
 
-constexpr int kRingCols = 16;  // columns of a thread
 
 // The streamed form: `stages` slots of one row of x and one of dy each. Row number i of this CTA (row blockIdx.x + i *
 // gridDim.x) lies in slot i % stages; the slot of row i - 1 is refilled behind the barrier inside row i's sums, which every thread
@@ -495,9 +494,9 @@ constexpr int kRingCols = 16;  // columns of a thread
 // With 16-bit rows the instructions are what bounds it (two thirds of the issue slots; they were twice as many with the
 // number of threads a variable, most of them addresses).
 // Dynamic shared memory: the ring, the weights (WIDE), two buffers for the sums over the warps.
-template <int DT, int T, bool WIDE>
-__global__ void __launch_bounds__(T, T > 512 ? 1 : 512 / T) layer_norm_backward_ring_kernel(const NormParams p, const int stages, int* status) {
-  constexpr int kSize = DT == TVB_F32 ? 4 : 2, kUnits = kRingCols / 4, threads = T, warps = T / 32;
+template <int DT, int T, int UNITS, bool WIDE>
+__global__ void __launch_bounds__(T, 512 / T) layer_norm_backward_ring_kernel(const NormParams p, const int stages, int* status) {
+  constexpr int kSize = DT == TVB_F32 ? 4 : 2, kUnits = UNITS, threads = T, warps = T / 32;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ uint64_t bars[8];
   __shared__ int abort_flag;
@@ -734,18 +733,20 @@ int norm_group(int64_t d, int vals) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// The streamed backward kernel: rows of 512 to 16384 values that fit the shared memory at least twice; up to 1024 threads per
-// SM, as one CTA or several. (A few numbers of threads, so that they can be constants of the kernel.)
+// The streamed backward kernel: rows of 512 to 16384 values that fit the shared memory at least twice. (A few numbers of threads, so that they can be constants of the
+// kernel.) A thread owns 16 columns, or 32 beyond 8192: 512 threads of up to 128 registers per SM (1024 of 64 spilled, 108 us against
+// 84 at 8192 x 8192 bfloat16; 32 columns for all: 85, but 152 against 144 at 16384 x 4096 float32).
 struct Ring {
-  int threads, per_sm, stages;
+  int cols, threads, per_sm, stages;
   size_t smem;
 };
 Ring ring_shape(int64_t d, int es, bool wide) {
   Ring r{};
-  if (d < 512 || d > 1024 * kRingCols || d % 4 != 0) return r;
-  for (int t : {64, 128, 192, 256, 384, 512, 768, 1024})
-    if (r.threads == 0 && d <= t * kRingCols) r.threads = t;
-  r.per_sm = std::max(512 / r.threads, 1);
+  if (d < 512 || d > 16384 || d % 4 != 0) return r;
+  r.cols = d <= 8192 ? 16 : 32;
+  for (int t : {64, 128, 192, 256, 384, 512})
+    if (r.threads == 0 && d <= t * r.cols) r.threads = t;
+  r.per_sm = 512 / r.threads;
   const int64_t rest = (wide ? d * 4 : 0) + r.threads / 2;  // weights, sums over the warps
   // (228 KB per SM, of which every CTA takes 1 KB for itself and some for its barriers)
   r.stages = static_cast<int>(std::min<int64_t>((228 * 1024 / r.per_sm - 1024 - 128 - rest) / (2 * d * es), 8));
@@ -793,9 +794,9 @@ int backward_vec(cudaStream_t stream, const NormParams& p, int64_t parts) {
   return launch_dependent("layer_norm_backward", kernel, dim3(static_cast<unsigned>(parts)), dim3(t < 128 ? 128 : t), 0, stream, p);
 }
 
-template <int DT, int T, bool WIDE>
+template <int DT, int T, int UNITS, bool WIDE>
 int backward_ring(int device, cudaStream_t stream, const NormParams& p, const Ring& r, int64_t ctas) {
-  auto kernel = layer_norm_backward_ring_kernel<DT, T, WIDE>;
+  auto kernel = layer_norm_backward_ring_kernel<DT, T, UNITS, WIDE>;
   static bool configured[64] = {};
   if (!configured[device & 63]) {
     TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 128));
@@ -809,15 +810,17 @@ int backward_ring(int device, cudaStream_t stream, const NormParams& p, const Ri
 
 template <int DT, bool WIDE>
 int backward_ring_threads(int device, cudaStream_t stream, const NormParams& p, const Ring& r, int64_t ctas) {
+  if (r.cols == 32) {
+    if (r.threads == 384) return backward_ring<DT, 384, 8, WIDE>(device, stream, p, r, ctas);
+    return backward_ring<DT, 512, 8, WIDE>(device, stream, p, r, ctas);
+  }
   switch (r.threads) {
-    case 64: return backward_ring<DT, 64, WIDE>(device, stream, p, r, ctas);
-    case 128: return backward_ring<DT, 128, WIDE>(device, stream, p, r, ctas);
-    case 192: return backward_ring<DT, 192, WIDE>(device, stream, p, r, ctas);
-    case 256: return backward_ring<DT, 256, WIDE>(device, stream, p, r, ctas);
-    case 384: return backward_ring<DT, 384, WIDE>(device, stream, p, r, ctas);
-    case 512: return backward_ring<DT, 512, WIDE>(device, stream, p, r, ctas);
-    case 768: return backward_ring<DT, 768, WIDE>(device, stream, p, r, ctas);
-    default: return backward_ring<DT, 1024, WIDE>(device, stream, p, r, ctas);
+    case 64: return backward_ring<DT, 64, 4, WIDE>(device, stream, p, r, ctas);
+    case 128: return backward_ring<DT, 128, 4, WIDE>(device, stream, p, r, ctas);
+    case 192: return backward_ring<DT, 192, 4, WIDE>(device, stream, p, r, ctas);
+    case 256: return backward_ring<DT, 256, 4, WIDE>(device, stream, p, r, ctas);
+    case 384: return backward_ring<DT, 384, 4, WIDE>(device, stream, p, r, ctas);
+    default: return backward_ring<DT, 512, 4, WIDE>(device, stream, p, r, ctas);
   }
 }
 
