@@ -48,7 +48,7 @@ LinearCopy make_readable(int dtype, const void** p, int64_t rows, int64_t cols, 
 
 int run_product(int device, cudaStream_t stream, const LinearProduct& p) {
   if (p.dtype == TVB_F32) return linear_simt(stream, p);
-  return linear_large(p) ? linear_pair(device, stream, &p, 1) : linear_split(device, stream, p);
+  return linear_large(p) ? linear_pair(device, stream, &p, 1) : linear_split(device, stream, &p, 1);
 }
 
 // dz needs a matrix of its own: there is an activation to differentiate, or TMA cannot read dy.
@@ -181,7 +181,11 @@ extern "C" int tvb_linear_backward(int device, const void* dy, int dtype, int64_
     d.I = k; d.J = n; d.R = m;
     d.dtype = dtype;
   }
-  if (count == 2 && dtype != TVB_F32 && linear_large(p[0]) && linear_large(p[1])) return linear_pair(device, stream, p, 2);
+  if (count == 2 && dtype != TVB_F32) {  // in one launch, where the same kernel suits both
+    const bool large0 = linear_large(p[0]), large1 = linear_large(p[1]);
+    if (large0 && large1) return linear_pair(device, stream, p, 2);
+    if (!large0 && !large1) return linear_split(device, stream, p, 2);
+  }
   for (int i = 0; i < count; i++)
     if (run_product(device, stream, p[i]) != 0) return -1;
   return 0;

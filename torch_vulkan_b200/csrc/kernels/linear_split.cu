@@ -45,14 +45,24 @@ struct SplitCfg {
 };
 
 struct SplitParams {
+  CUtensorMap map_p, map_q;
   const void* bias;
   const void* residual;
   void* out;
   void* preact;
   int64_t residual_ld;
   int I, J, blocks, tiles_j, activation, vector_ok;
-  uint32_t idesc;
+  uint32_t idesc, ctas;  // ctas: of this product
   int* status;
+};
+
+// The orders of the operands: r contiguous in both; i in P (dx); i in P and j in Q (dw); or two products in one launch, the
+// first CTAs' as kDx and the others' as kDw.
+enum Order { kForward, kDx, kDw, kDxDw };
+
+template <int ORDER>
+struct SplitArgs {
+  SplitParams product[ORDER == kDxDw ? 2 : 1];
 };
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {  // (from mapa)
@@ -167,11 +177,93 @@ __device__ __forceinline__ void finish_tile(const SplitParams& p, const Finish& 
   if (j < end) finish_columns<BF16, ACT, 1>(p, f, j);
 }
 
-template <int TN, bool P_MN, bool Q_MN, bool BF16>
-__global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
-    linear_split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const SplitParams p) {
+// Where a CTA stands in its cluster and what it multiplies.
+struct SplitWork {
+  uint32_t base, full0, empty0, tfull, half, first;
+  int i0, j0, kb0, kb1;
+};
+
+// (The two threads that run these set the pace of the whole kernel: no index arithmetic in their loops.)
+template <int TN, bool P_MN, bool Q_MN>
+__device__ __forceinline__ void load_slices(const SplitParams& p, const SplitWork& w, volatile int* abort_flag) {
   using Cfg = SplitCfg<TN>;
-  static_assert(!Q_MN || Cfg::kRowsQ >= 64, "an MN-major operand comes in columns of 64 values");
+  constexpr bool kPair = Cfg::kPair;
+  uint32_t slot = 0, phase = 0;
+  int r = w.kb0 * kStepR;
+  const int row_q = w.j0 + static_cast<int>(w.half) * Cfg::kRowsQ;
+  const uint32_t bars0 = kPair ? ptx::mapa(w.full0, w.first) : w.full0;  // the barriers that count the boxes: the pair's first CTA's
+  auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if (kPair) ptx::tma_load_2d_pair(dst, map, x, y, bar);
+    else ptx::tma_load_2d(dst, map, x, y, bar);
+  };
+#pragma unroll 1
+  for (int kb = w.kb0; kb < w.kb1; kb++, r += kStepR) {
+    const uint32_t dst = w.base + slot * Cfg::kStage, bar = bars0 + 8 * slot;
+    if (!ptx::mbar_wait(w.empty0 + 8 * slot, phase ^ 1u, abort_flag)) break;
+    if (w.half == 0) ptx::mbar_expect_tx(w.full0 + 8 * slot, (kPair ? 2 : 1) * Cfg::kStage);
+    if (P_MN) {
+#pragma unroll
+      for (int c = 0; c < kRows / 64; c++) load(dst + c * 8192, &p.map_p, w.i0 + c * 64, r, bar);
+    } else {
+      load(dst, &p.map_p, r, w.i0, bar);
+    }
+    if (Q_MN) {
+#pragma unroll
+      for (int c = 0; c < Cfg::kRowsQ / 64; c++) load(dst + Cfg::kStageP + c * 8192, &p.map_q, row_q + c * 64, r, bar);
+    } else {
+      load(dst + Cfg::kStageP, &p.map_q, r, row_q, bar);
+    }
+    if (++slot == Cfg::kStages) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  // no copy may still be in flight when the ring is used for the sums or released: the last filling of every slot
+  const int filled = (w.kb1 - w.kb0) < Cfg::kStages ? w.kb1 - w.kb0 : Cfg::kStages;
+  for (int s = 0; w.half == 0 && s < filled; s++) {  // (a pair's second CTA stays until the sums are joined)
+    volatile int never = 0;
+    ptx::mbar_wait(w.full0 + 8 * s, s < static_cast<int>(slot) ? phase : phase ^ 1u, &never);
+  }
+}
+
+template <int TN, bool P_MN, bool Q_MN>
+__device__ __forceinline__ void multiply_slices(const SplitParams& p, const SplitWork& w, uint32_t tmem, volatile int* abort_flag) {
+  using Cfg = SplitCfg<TN>;
+  constexpr bool kPair = Cfg::kPair;
+  constexpr uint64_t kP = P_MN ? 128 : 2, kQ = Q_MN ? 128 : 2;  // 16 values of r, in the descriptors' units
+  const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(w.base) : ptx::tc_smem_desc_sw128(w.base);
+  const uint64_t q0 = Q_MN ? ptx::tc_smem_desc_sw128_mn(w.base + Cfg::kStageP) : ptx::tc_smem_desc_sw128(w.base + Cfg::kStageP);
+  uint32_t slot = 0, phase = 0, more = 0;
+  bool ok = w.kb1 > w.kb0;
+#pragma unroll 1
+  for (int kb = w.kb0; kb < w.kb1; kb++) {
+    ok = ptx::mbar_wait(w.full0 + 8 * slot, phase, abort_flag);
+    if (!ok) break;
+    ptx::tc_fence_after();
+    const uint64_t pd = p0 + slot * (Cfg::kStage >> 4), qd = q0 + slot * (Cfg::kStage >> 4);
+#pragma unroll
+    for (int j = 0; j < kStepR / 16; j++) {
+      if (kPair) ptx::tc_mma_pair<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
+      else ptx::tc_mma<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
+    }
+    more = 1;
+    if (kPair) ptx::tc_commit_pair_at(w.empty0 + 8 * slot, w.first);  // (in both CTAs)
+    else ptx::tc_commit(w.empty0 + 8 * slot);
+    if (++slot == Cfg::kStages) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  if (ok) {
+    if (kPair) ptx::tc_commit_pair_at(w.tfull, w.first);
+    else ptx::tc_commit(w.tfull);
+  }
+}
+
+template <int TN, int ORDER, bool BF16>
+__global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm) linear_split_kernel(const __grid_constant__ SplitArgs<ORDER> args) {
+  using Cfg = SplitCfg<TN>;
+  static_assert(ORDER < kDw || Cfg::kRowsQ >= 64, "an MN-major operand comes in columns of 64 values");
   constexpr bool kPair = Cfg::kPair;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -187,10 +279,13 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
   const uint32_t rank = ptx::cluster_ctarank();
   // half: which CTA of its pair this is; the pair's first CTA (rank `first`) issues its MMAs
   const uint32_t half = kPair ? rank & 1u : 0u, first = rank - half, part = kPair ? rank >> 1 : rank, parts = kPair ? ctas >> 1 : ctas;
-  const int tile = static_cast<int>(blockIdx.x / ctas);
+  const bool second = ORDER == kDxDw && blockIdx.x >= args.product[0].ctas;  // (the same for a whole cluster)
+  const SplitParams& p = args.product[second ? 1 : 0];
+  const int tile = static_cast<int>((blockIdx.x - (second ? args.product[0].ctas : 0u)) / ctas);
   const int i0 = tile / p.tiles_j * Cfg::kTileI + static_cast<int>(half) * kRows, j0 = tile % p.tiles_j * TN;
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.blocks) * part / parts);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.blocks) * (part + 1) / parts);
+  const SplitWork work{base, full0, empty0, tfull, half, first, i0, j0, kb0, kb1};
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::kStages; s++) {
       ptx::mbar_init(full0 + 8 * s, 1);
@@ -200,9 +295,9 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == kProducer && lane == 0) {
-    ptx::prefetch_tensormap(&map_p);
-    ptx::prefetch_tensormap(&map_q);
+  if (warp == kProducer && lane == 0 && kb1 > kb0) {
+    ptx::prefetch_tensormap(&p.map_p);
+    ptx::prefetch_tensormap(&p.map_q);
   }
   if (warp == kMma) {
     if (kPair) ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), Cfg::kTmemCols);
@@ -216,76 +311,23 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm)
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
-  // (The two threads below set the pace of the whole kernel: no index arithmetic in their loops.)
   if (warp == kProducer) {
     if (lane == 0) {
-      uint32_t slot = 0, phase = 0;
-      int r = kb0 * kStepR;
-      const int row_q = j0 + static_cast<int>(half) * Cfg::kRowsQ;
-      const uint32_t bars0 = kPair ? ptx::mapa(full0, first) : full0;  // the barriers that count the boxes: the pair's first CTA's
-      auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-        if (kPair) ptx::tma_load_2d_pair(dst, map, x, y, bar);
-        else ptx::tma_load_2d(dst, map, x, y, bar);
-      };
-#pragma unroll 1
-      for (int kb = kb0; kb < kb1; kb++, r += kStepR) {
-        const uint32_t dst = base + slot * Cfg::kStage, bar = bars0 + 8 * slot;
-        if (!ptx::mbar_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag)) break;
-        if (half == 0) ptx::mbar_expect_tx(full0 + 8 * slot, (kPair ? 2 : 1) * Cfg::kStage);
-        if (P_MN) {
-#pragma unroll
-          for (int c = 0; c < kRows / 64; c++) load(dst + c * 8192, &map_p, i0 + c * 64, r, bar);
-        } else {
-          load(dst, &map_p, r, i0, bar);
-        }
-        if (Q_MN) {
-#pragma unroll
-          for (int c = 0; c < Cfg::kRowsQ / 64; c++) load(dst + Cfg::kStageP + c * 8192, &map_q, row_q + c * 64, r, bar);
-        } else {
-          load(dst + Cfg::kStageP, &map_q, r, row_q, bar);
-        }
-        if (++slot == Cfg::kStages) {
-          slot = 0;
-          phase ^= 1u;
-        }
-      }
-      // no copy may still be in flight when the ring is used for the sums or released: the last filling of every slot
-      const int filled = (kb1 - kb0) < Cfg::kStages ? kb1 - kb0 : Cfg::kStages;
-      for (int s = 0; half == 0 && s < filled; s++) {  // (a pair's second CTA stays until the sums are joined)
-        volatile int never = 0;
-        ptx::mbar_wait(full0 + 8 * s, s < static_cast<int>(slot) ? phase : phase ^ 1u, &never);
+      if constexpr (ORDER == kDxDw) {
+        if (second) load_slices<TN, true, true>(p, work, abort_flag);
+        else load_slices<TN, true, false>(p, work, abort_flag);
+      } else {
+        load_slices<TN, ORDER != kForward, ORDER == kDw>(p, work, abort_flag);
       }
     }
     __syncwarp();
   } else if (warp == kMma) {
     if (lane == 0 && half == 0) {
-      constexpr uint64_t kP = P_MN ? 128 : 2, kQ = Q_MN ? 128 : 2;  // 16 values of r, in the descriptors' units
-      const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(base) : ptx::tc_smem_desc_sw128(base);
-      const uint64_t q0 = Q_MN ? ptx::tc_smem_desc_sw128_mn(base + Cfg::kStageP) : ptx::tc_smem_desc_sw128(base + Cfg::kStageP);
-      uint32_t slot = 0, phase = 0, more = 0;
-      bool ok = kb1 > kb0;
-#pragma unroll 1
-      for (int kb = kb0; kb < kb1; kb++) {
-        ok = ptx::mbar_wait(full0 + 8 * slot, phase, abort_flag);
-        if (!ok) break;
-        ptx::tc_fence_after();
-        const uint64_t pd = p0 + slot * (Cfg::kStage >> 4), qd = q0 + slot * (Cfg::kStage >> 4);
-#pragma unroll
-        for (int j = 0; j < kStepR / 16; j++) {
-          if (kPair) ptx::tc_mma_pair<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
-          else ptx::tc_mma<2>(tmem, pd + kP * j, qd + kQ * j, p.idesc, j == 0 ? more : 1u);
-        }
-        more = 1;
-        if (kPair) ptx::tc_commit_pair_at(empty0 + 8 * slot, first);  // (in both CTAs)
-        else ptx::tc_commit(empty0 + 8 * slot);
-        if (++slot == Cfg::kStages) {
-          slot = 0;
-          phase ^= 1u;
-        }
-      }
-      if (ok) {
-        if (kPair) ptx::tc_commit_pair_at(tfull, first);
-        else ptx::tc_commit(tfull);
+      if constexpr (ORDER == kDxDw) {
+        if (second) multiply_slices<TN, true, true>(p, work, tmem, abort_flag);
+        else multiply_slices<TN, true, false>(p, work, tmem, abort_flag);
+      } else {
+        multiply_slices<TN, ORDER != kForward, ORDER == kDw>(p, work, tmem, abort_flag);
       }
     }
     __syncwarp();
@@ -363,52 +405,61 @@ int operand_map(CUtensorMap* map, const void* base, int dtype, int64_t inner, in
   return make_tensor_map_2d(map, base, dt, inner, outer, ld * 2, 64, box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int TN, bool P_MN, bool Q_MN, bool BF16>
-int split_run(int device, cudaStream_t stream, const LinearProduct& lp, int parts) {
+// The kernel's parameters for one product; `parts` slices of r.
+template <int TN>
+int split_params(int device, const LinearProduct& lp, int parts, SplitParams* p) {
   using Cfg = SplitCfg<TN>;
-  auto kernel = linear_split_kernel<TN, P_MN, Q_MN, BF16>;
+  if (lp.R > 0) {  // (a product over nothing: no box is ever loaded)
+    if (operand_map(&p->map_p, lp.p, lp.dtype, lp.p_mn ? lp.I : lp.R, lp.p_mn ? lp.R : lp.I, lp.p_mn ? lp.p_sr : lp.p_si, lp.p_mn ? kStepR : kRows) != 0 ||
+        operand_map(&p->map_q, lp.q, lp.dtype, lp.q_mn ? lp.J : lp.R, lp.q_mn ? lp.R : lp.J, lp.q_mn ? lp.q_sr : lp.q_sj, lp.q_mn ? kStepR : Cfg::kRowsQ) != 0)
+      return -1;
+  }
+  p->bias = lp.bias;
+  p->residual = lp.residual;
+  p->out = lp.out;
+  p->preact = lp.preact;
+  p->residual_ld = lp.residual_ld;
+  p->I = static_cast<int>(lp.I);
+  p->J = static_cast<int>(lp.J);
+  p->blocks = static_cast<int>(ceil_div(lp.R, kStepR));
+  p->tiles_j = static_cast<int>(ceil_div(lp.J, TN));
+  p->activation = lp.activation;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(lp.out) | reinterpret_cast<uintptr_t>(lp.preact) | reinterpret_cast<uintptr_t>(lp.bias) |
+                        reinterpret_cast<uintptr_t>(lp.residual);
+  p->vector_ok = (all & 7u) == 0 && lp.I % 4 == 0 && (lp.residual == nullptr || lp.residual_ld % 4 == 0);
+  const uint32_t fmt = lp.dtype == TVB_BF16 ? 1 : 0;
+  p->idesc = ptx::tc_instr_desc(1, fmt, fmt, Cfg::kTileI, TN) | (lp.p_mn ? ptx::kTcAMajorMN : 0u) | (lp.q_mn ? ptx::kTcBMajorMN : 0u);
+  const int64_t ctas = ceil_div(lp.I, Cfg::kTileI) * p->tiles_j * (Cfg::kPair ? 2 * parts : parts);
+  if (ctas >= (int64_t(1) << 30)) return fail("tvb_linear: too many output tiles");
+  p->ctas = static_cast<uint32_t>(ctas);
+  return status_word(device, &p->status);
+}
+
+template <int TN, int ORDER, bool BF16>
+int split_run(int device, cudaStream_t stream, const LinearProduct* lp, int parts) {
+  using Cfg = SplitCfg<TN>;
+  auto kernel = linear_split_kernel<TN, ORDER, BF16>;
   static bool configured[64] = {};
   if (!configured[device & 63]) {
     TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes));
     configured[device & 63] = true;
   }
-  CUtensorMap map_p, map_q;
-  if (lp.R > 0) {
-    if (operand_map(&map_p, lp.p, lp.dtype, P_MN ? lp.I : lp.R, P_MN ? lp.R : lp.I, P_MN ? lp.p_sr : lp.p_si, P_MN ? kStepR : kRows) != 0 ||
-        operand_map(&map_q, lp.q, lp.dtype, Q_MN ? lp.J : lp.R, Q_MN ? lp.R : lp.J, Q_MN ? lp.q_sr : lp.q_sj, Q_MN ? kStepR : Cfg::kRowsQ) != 0)
-      return -1;
-  } else {
-    map_p = map_q = CUtensorMap{};  // (a product over nothing: no box is ever loaded)
+  SplitArgs<ORDER> args{};
+  uint32_t grid = 0;
+  for (int k = 0; k < (ORDER == kDxDw ? 2 : 1); k++) {
+    if (split_params<TN>(device, lp[k], parts, &args.product[k]) != 0) return -1;
+    grid += args.product[k].ctas;
   }
-  SplitParams p{};
-  p.bias = lp.bias;
-  p.residual = lp.residual;
-  p.out = lp.out;
-  p.preact = lp.preact;
-  p.residual_ld = lp.residual_ld;
-  p.I = static_cast<int>(lp.I);
-  p.J = static_cast<int>(lp.J);
-  p.blocks = static_cast<int>(ceil_div(lp.R, kStepR));
-  p.tiles_j = static_cast<int>(ceil_div(lp.J, TN));
-  p.activation = lp.activation;
-  const uintptr_t all = reinterpret_cast<uintptr_t>(lp.out) | reinterpret_cast<uintptr_t>(lp.preact) | reinterpret_cast<uintptr_t>(lp.bias) |
-                        reinterpret_cast<uintptr_t>(lp.residual);
-  p.vector_ok = (all & 7u) == 0 && lp.I % 4 == 0 && (lp.residual == nullptr || lp.residual_ld % 4 == 0);
-  const uint32_t fmt = BF16 ? 1 : 0;
-  p.idesc = ptx::tc_instr_desc(1, fmt, fmt, Cfg::kTileI, TN) | (P_MN ? ptx::kTcAMajorMN : 0u) | (Q_MN ? ptx::kTcBMajorMN : 0u);
-  if (status_word(device, &p.status) != 0) return -1;
-  const int ctas = Cfg::kPair ? 2 * parts : parts;
-  const int64_t grid = ceil_div(lp.I, Cfg::kTileI) * p.tiles_j * ctas;
-  if (grid >= (int64_t(1) << 31)) return fail("tvb_linear: too many output tiles");
-  return launch_dependent_cluster("linear_split", kernel, ctas, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Cfg::kSmemBytes, stream,
-                                  map_p, map_q, p);
+  return launch_dependent_cluster("linear_split", kernel, Cfg::kPair ? 2 * parts : parts, dim3(grid), dim3(kThreads), Cfg::kSmemBytes, stream, args);
 }
 
 template <int TN, bool BF16>
-int split_orders(int device, cudaStream_t stream, const LinearProduct& lp, int parts) {
-  if (!lp.q_mn) return lp.p_mn ? split_run<TN, true, false, BF16>(device, stream, lp, parts) : split_run<TN, false, false, BF16>(device, stream, lp, parts);
+int split_orders(int device, cudaStream_t stream, const LinearProduct* lp, int count, int parts) {
+  if (count == 1 && !lp->q_mn)
+    return lp->p_mn ? split_run<TN, kDx, BF16>(device, stream, lp, parts) : split_run<TN, kForward, BF16>(device, stream, lp, parts);
   if constexpr (TN >= 128) {
-    if (lp.p_mn) return split_run<TN, true, true, BF16>(device, stream, lp, parts);
+    if (count == 1 && lp->p_mn) return split_run<TN, kDw, BF16>(device, stream, lp, parts);
+    if (count == 2 && lp[0].p_mn && !lp[0].q_mn && lp[1].p_mn && lp[1].q_mn) return split_run<TN, kDxDw, BF16>(device, stream, lp, parts);
   }
   return fail("tvb_linear: no kernel for this order of the operands");
 }
@@ -426,14 +477,22 @@ struct Shape {
   double us;
 };
 
-double split_cost(const LinearProduct& lp, int tn, int parts) {
+// `count` products in one launch share TN and S.
+double split_cost(const LinearProduct* lp, int count, int tn, int parts) {
   const bool pair = tn >= 64;
-  const double ctas = static_cast<double>(ceil_div(lp.I, pair ? 2 * kRows : kRows) * ceil_div(lp.J, tn) * parts * (pair ? 2 : 1));
+  double ctas = 0, work = 0, longest = 0;
+  for (int k = 0; k < count; k++) {
+    const double n = static_cast<double>(ceil_div(lp[k].I, pair ? 2 * kRows : kRows) * ceil_div(lp[k].J, tn) * parts * (pair ? 2 : 1));
+    const double steps = static_cast<double>(ceil_div(ceil_div(lp[k].R, kStepR), parts));
+    ctas += n;
+    work += n * steps;
+    longest = std::max(longest, steps);
+  }
   const double per_sm = tn <= 128 ? 2 : 1, load = ctas / 148, rounds = std::max(1.0, load / per_sm);
   const double alone = tn <= 32 ? 0.297 : tn == 64 ? 0.264 : tn == 128 ? 0.322 : 0.294;
   double step = alone * (1 + 0.417 * std::min(1.0, load)) * (1 + 0.678 * std::max(0.0, std::min(load, per_sm) - 1));
   if (tn == 256 && parts >= 3) step *= 1.792;
-  double us = 2.11 + 0.00994 * tn + rounds * static_cast<double>(ceil_div(ceil_div(lp.R, kStepR), parts)) * step + 6.36 * (rounds - 1);
+  double us = 2.11 + 0.00994 * tn + std::max(longest, work / ctas * rounds) * step + 6.36 * (rounds - 1);
   if (parts > 1) us += 0.309 + 0.0116 * tn / parts;
   if (parts * (pair ? 2 : 1) > 4) us += 1.07;
   return us;
@@ -445,16 +504,20 @@ double pair_cost(const LinearProduct& lp) {  // (fewer tiles than pairs)
   return 1.64 + static_cast<double>(ceil_div(lp.R, kStepR)) * (0.486 + 0.0706 * static_cast<double>(pair_tiles(lp)) / 74) + 2.49;
 }
 
-Shape split_shape(const LinearProduct& lp) {
-  const int least = lp.q_mn ? 128 : 16;
+Shape split_shape(const LinearProduct* lp, int count) {
+  const int least = lp[count - 1].q_mn ? 128 : 16;
+  int64_t rows = 0, blocks = 0;
+  for (int k = 0; k < count; k++) {
+    rows = std::max(rows, lp[k].J);
+    blocks = std::max(blocks, ceil_div(lp[k].R, kStepR));
+  }
   int fits = least;  // the smallest TN that holds the rows
-  while (fits < 256 && fits < lp.J) fits *= 2;
-  const int64_t blocks = ceil_div(lp.R, kStepR);
-  Shape best{fits, 1, split_cost(lp, fits, 1)};
-  for (int tn = fits; tn >= least && tn * 4 >= fits && tn * 8 >= lp.J; tn /= 2)
+  while (fits < 256 && fits < rows) fits *= 2;
+  Shape best{fits, 1, split_cost(lp, count, fits, 1)};
+  for (int tn = fits; tn >= least && tn * 4 >= fits && (tn * 8 >= rows || tn >= 128); tn /= 2)
     for (int parts : {1, 2, 3, 4, 6, 8}) {
       if (parts > 1 && (parts > blocks || (tn >= 64 && parts > 4))) break;
-      const double us = split_cost(lp, tn, parts);
+      const double us = split_cost(lp, count, tn, parts);
       if (us < 0.96 * best.us) best = Shape{tn, parts, us};  // (a finer split has to be worth it)
     }
   return best;
@@ -464,19 +527,18 @@ Shape split_shape(const LinearProduct& lp) {
 
 bool linear_large(const LinearProduct& lp) {
   if (lp.R == 0 || lp.J <= 64) return false;
-  return pair_tiles(lp) >= 74 || pair_cost(lp) < split_shape(lp).us;
+  return pair_tiles(lp) >= 74 || pair_cost(lp) < split_shape(&lp, 1).us;
 }
 
-int linear_split(int device, cudaStream_t stream, const LinearProduct& lp) {
-  const Shape s = split_shape(lp);
-  const int parts = s.parts;
-  const bool bf16 = lp.dtype == TVB_BF16;
+int linear_split(int device, cudaStream_t stream, const LinearProduct* lp, int count) {
+  const Shape s = split_shape(lp, count);
+  const bool bf16 = lp->dtype == TVB_BF16;
   switch (s.tn) {
-    case 16: return bf16 ? split_orders<16, true>(device, stream, lp, parts) : split_orders<16, false>(device, stream, lp, parts);
-    case 32: return bf16 ? split_orders<32, true>(device, stream, lp, parts) : split_orders<32, false>(device, stream, lp, parts);
-    case 64: return bf16 ? split_orders<64, true>(device, stream, lp, parts) : split_orders<64, false>(device, stream, lp, parts);
-    case 128: return bf16 ? split_orders<128, true>(device, stream, lp, parts) : split_orders<128, false>(device, stream, lp, parts);
-    default: return bf16 ? split_orders<256, true>(device, stream, lp, parts) : split_orders<256, false>(device, stream, lp, parts);
+    case 16: return bf16 ? split_orders<16, true>(device, stream, lp, count, s.parts) : split_orders<16, false>(device, stream, lp, count, s.parts);
+    case 32: return bf16 ? split_orders<32, true>(device, stream, lp, count, s.parts) : split_orders<32, false>(device, stream, lp, count, s.parts);
+    case 64: return bf16 ? split_orders<64, true>(device, stream, lp, count, s.parts) : split_orders<64, false>(device, stream, lp, count, s.parts);
+    case 128: return bf16 ? split_orders<128, true>(device, stream, lp, count, s.parts) : split_orders<128, false>(device, stream, lp, count, s.parts);
+    default: return bf16 ? split_orders<256, true>(device, stream, lp, count, s.parts) : split_orders<256, false>(device, stream, lp, count, s.parts);
   }
 }
 
