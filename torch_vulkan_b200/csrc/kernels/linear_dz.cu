@@ -75,43 +75,57 @@ __global__ void __launch_bounds__(kThreads) linear_dz_kernel(const LinearDz p) {
   const bool act = p.activation != TVB_ACT_NONE;
   uint64_t sum[4] = {};
   const int64_t c_end = p.n - c0;  // columns of this thread that exist
+  // kAhead rows are read before the first is worked on: a store between two loads would hold the second back
+  constexpr int kAhead = VEC && DT != TVB_F32 ? 4 : 2;
+  auto one = [&](int64_t r, uint64_t (&v)[4], const uint64_t (&z)[4]) {
+    if (act) times_slope<DT>(v, z, p.activation);
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] = ptx::add_f32x2(sum[e], v[e]);
+    if (p.dz == nullptr) return;
+    if (VEC) {
+      store8<DT>(p.dz, r * p.dz_ld + c0, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float f[2];
+        ptx::unpack_f32x2(v[e], f[0], f[1]);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (2 * e + h < c_end) store_float<DT>(p.dz, r * p.dz_ld + c0 + 2 * e + h, f[h]);
+      }
+    }
+  };
+  auto fetch = [&](int64_t r, uint64_t (&v)[4], uint64_t (&z)[4]) {
+    if (VEC) {
+      load8<DT>(p.dy, r * p.dy_ld + c0, v);
+      if (act) load8<DT>(p.z, r * p.n + c0, z);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float f[4] = {};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (2 * e + h < c_end) {
+            f[h] = load_float<DT>(p.dy, r * p.dy_ld + c0 + 2 * e + h);
+            if (act) f[2 + h] = load_float<DT>(p.z, r * p.n + c0 + 2 * e + h);
+          }
+        v[e] = ptx::pack_f32x2(__float_as_uint(f[0]), __float_as_uint(f[1]));
+        z[e] = ptx::pack_f32x2(__float_as_uint(f[2]), __float_as_uint(f[3]));
+      }
+    }
+  };
   if (c_end > 0) {
-#pragma unroll 2
-    for (int64_t r = r_begin + (threadIdx.x >> 3); r < r_end; r += kRowsPerStep) {
-      uint64_t v[4], z[4];
-      if (VEC) {
-        load8<DT>(p.dy, r * p.dy_ld + c0, v);
-        if (act) load8<DT>(p.z, r * p.n + c0, z);
-      } else {
+    int64_t r = r_begin + (threadIdx.x >> 3);
+    uint64_t v[kAhead][4], z[kAhead][4] = {};
+    for (; r + (kAhead - 1) * kRowsPerStep < r_end; r += kAhead * kRowsPerStep) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float f[4] = {};
+      for (int a = 0; a < kAhead; a++) fetch(r + a * kRowsPerStep, v[a], z[a]);
 #pragma unroll
-          for (int h = 0; h < 2; h++)
-            if (2 * e + h < c_end) {
-              f[h] = load_float<DT>(p.dy, r * p.dy_ld + c0 + 2 * e + h);
-              if (act) f[2 + h] = load_float<DT>(p.z, r * p.n + c0 + 2 * e + h);
-            }
-          v[e] = ptx::pack_f32x2(__float_as_uint(f[0]), __float_as_uint(f[1]));
-          z[e] = ptx::pack_f32x2(__float_as_uint(f[2]), __float_as_uint(f[3]));
-        }
-      }
-      if (act) times_slope<DT>(v, z, p.activation);
-#pragma unroll
-      for (int e = 0; e < 4; e++) sum[e] = ptx::add_f32x2(sum[e], v[e]);
-      if (p.dz == nullptr) continue;
-      if (VEC) {
-        store8<DT>(p.dz, r * p.dz_ld + c0, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float f[2];
-          ptx::unpack_f32x2(v[e], f[0], f[1]);
-#pragma unroll
-          for (int h = 0; h < 2; h++)
-            if (2 * e + h < c_end) store_float<DT>(p.dz, r * p.dz_ld + c0 + 2 * e + h, f[h]);
-        }
-      }
+      for (int a = 0; a < kAhead; a++) one(r + a * kRowsPerStep, v[a], z[a]);
+    }
+    for (; r < r_end; r += kRowsPerStep) {
+      fetch(r, v[0], z[0]);
+      one(r, v[0], z[0]);
     }
   }
   __shared__ float part_sums[kRowsPerStep][kStrip];
