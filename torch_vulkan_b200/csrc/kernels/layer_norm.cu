@@ -114,9 +114,11 @@ struct Piece {
     if constexpr (DT == TVB_F32) {
       load_pairs<DT>(at, 0, v);
     } else {
-      const uint4 t = *reinterpret_cast<const uint4*>(at);
-      v[0] = pair16<DT>(t.x); v[1] = pair16<DT>(t.y); v[2] = pair16<DT>(t.z); v[3] = pair16<DT>(t.w);
+      unpack(*reinterpret_cast<const uint4*>(at));
     }
+  }
+  __device__ __forceinline__ void unpack(const uint4& t) {
+    v[0] = pair16<DT>(t.x); v[1] = pair16<DT>(t.y); v[2] = pair16<DT>(t.z); v[3] = pair16<DT>(t.w);
   }
   // weight or bias: of the values' type, or (WIDE) float32 beside 16-bit values
   template <bool WIDE>
@@ -277,6 +279,7 @@ __device__ __forceinline__ void group_sum(float& a, float& b, float2 (*buf)[32],
 template <int T>
 constexpr int norm_threads() { return T < 128 ? 128 : T; }
 
+constexpr int kRingStages = 8;  // rows on their way in the forward kernel, at most
 constexpr int kValsBwd = 16;   // values of a row per thread in the backward kernels (with two sums per value)
 
 // At least this many CTAs per SM: 1024 threads of 64 registers, but for 16-bit rows of up to 4096 values, where a few registers
@@ -484,8 +487,99 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-constexpr int kRingCluster = 2;
+// Forward, long rows of 16-bit values: persistent CTAs, one per SM, whose rows come through a ring in shared memory by bulk
+// copies, so the next ones are on their way during a row's sums and barriers. 32 values of a row per thread; the parameters stay
+// in registers, as they are. (bfloat16, us, with registers and 1024 threads per row before: 4096 x 16384 71 -> 56, 8192 x 12288
+// 119 -> 87, 300 x 16384 8.9 -> 7.0. Up to 8192 values two CTAs' rows hide each other's barriers as well without a ring.)
+template <int DT, int T>
+__global__ void __launch_bounds__(T, 1) layer_norm_ring_kernel(const NormParams p, const int stages, int* status) {
+  constexpr int kPieces = 4;
+  using Values = Piece<DT, 8>;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float2 buf[2][32];
+  __shared__ uint64_t bars[kRingStages];
+  __shared__ int abort_flag;
+  const int d = p.d, row_bytes = d * 2, t = threadIdx.x;
+  const int left = d - 8 * t;  // piece c of this thread (columns 8 (c T + t) ...) exists if left > 8 c T
+  const uint32_t ring0 = ptx::smem_u32(ring), bar0 = ptx::smem_u32(bars);
+  if (t == 0) {
+    for (int s = 0; s < stages; s++) ptx::mbar_init(bar0 + 8 * s, 1);
+    abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const int64_t step = gridDim.x;
+  const int count = blockIdx.x < p.rows ? static_cast<int>((p.rows - blockIdx.x + step - 1) / step) : 0;
+  const uint8_t* next = static_cast<const uint8_t*>(p.x) + blockIdx.x * p.x_ld * 2;  // the next row to fetch (thread 0)
+  int fetched = 0;
+  auto fetch = [&](int slot) {
+    ptx::mbar_expect_tx(bar0 + 8 * slot, row_bytes);
+    bulk_load(ring0 + slot * row_bytes, next, row_bytes, bar0 + 8 * slot);
+    next += step * p.x_ld * 2;
+    fetched++;
+  };
+  if (t == 0)
+    while (fetched < count && fetched < stages) fetch(fetched);
+  const uint32_t one = DT == TVB_BF16 ? 0x3f803f80u : 0x3c003c00u;
+  uint4 g[kPieces], b[kPieces];
+#pragma unroll
+  for (int c = 0; c < kPieces; c++) {
+    g[c] = make_uint4(one, one, one, one);
+    b[c] = make_uint4(0, 0, 0, 0);
+    if (left <= 8 * c * T) continue;
+    if (p.weight != nullptr) g[c] = static_cast<const uint4*>(p.weight)[c * T + t];
+    if (p.bias != nullptr) b[c] = static_cast<const uint4*>(p.bias)[c * T + t];
+  }
+  int slot = 0, before = 0;
+  uint32_t phase = 0;
+  int64_t row = blockIdx.x;
+#pragma unroll 1
+  for (int i = 0; i < count; i++, row += step) {
+    ptx::mbar_wait(bar0 + 8 * slot, phase, &abort_flag);  // (no early exit: barriers follow)
+    const uint8_t* mine = ring + static_cast<size_t>(slot) * row_bytes + t * 16;
+    Values x[kPieces];
+    float sum = 0.0f, sq = 0.0f, none = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kPieces; c++) {
+      x[c].zero();
+      if (left > 8 * c * T) x[c].load(mine + c * T * 16);
+      sum += x[c].sum();
+    }
+    group_sum<T, 1>(sum, none, buf, 0);
+    if (t == 0 && i >= 1 && fetched < count) fetch(before);  // (all threads have read the row before)
+    const float mean = sum / static_cast<float>(d);
+#pragma unroll
+    for (int c = 0; c < kPieces; c++)
+      if (left > 8 * c * T) sq += x[c].center(mean);
+    group_sum<T, 1>(sq, none, buf, 1);
+    const float rstd = 1.0f / sqrtf(sq / static_cast<float>(d) + p.eps);
+    if (t == 0) {
+      if (p.mean != nullptr) p.mean[row] = mean;
+      if (p.rstd != nullptr) p.rstd[row] = rstd;
+    }
+    uint8_t* y = static_cast<uint8_t*>(p.y) + row * row_bytes + t * 16;
+#pragma unroll
+    for (int c = 0; c < kPieces; c++) {
+      if (left <= 8 * c * T) continue;
+      Values gv, bv;
+      gv.unpack(g[c]);
+      bv.unpack(b[c]);
+      x[c].scale(rstd, gv, bv);
+      x[c].store(y + c * T * 16);
+    }
+    before = slot;
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+  __syncthreads();
+  if (t == 0 && abort_flag != 0) atomicExch(status, 2);
+}
 
+constexpr int kRingCluster = 2;
 
 // The streamed form: `stages` slots of one row of x and one of dy each. Row number i of this CTA (row blockIdx.x + i *
 // gridDim.x) lies in slot i % stages; the slot of row i - 1 is refilled behind the barrier inside row i's sums, which every thread
@@ -721,6 +815,7 @@ __global__ void __launch_bounds__(256) layer_norm_reduce_kernel(const float* par
   if (out != nullptr) store_float_rt(out, col < d ? col : col - d, param_dtype, s);
 }
 
+constexpr int kRingRoom = 224 * 1024;       // shared memory of the forward kernel's ring, at most
 constexpr int kLongest = 32 * 1024;         // values of a row that the forward kernels keep in registers
 constexpr int kLongestBwd = 16 * 1024;      // and the plain backward kernel
 constexpr int64_t kLongSlices = 64;         // partial rows of layer_norm_columns_kernel, at most
@@ -824,13 +919,34 @@ int backward_ring_threads(int device, cudaStream_t stream, const NormParams& p, 
   }
 }
 
+template <int DT, int T>
+int forward_ring(int device, cudaStream_t stream, const NormParams& p) {
+  auto kernel = layer_norm_ring_kernel<DT, T>;
+  static bool configured[64] = {};
+  if (!configured[device & 63]) {
+    TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingRoom));
+    configured[device & 63] = true;
+  }
+  const int stages = std::min(kRingStages, kRingRoom / (p.d * 2));
+  int* status = nullptr;
+  if (status_word(device, &status) != 0) return -1;
+  const int64_t ctas = std::min<int64_t>(sm_count(device), p.rows);
+  return launch_dependent("layer_norm_ring", kernel, dim3(static_cast<unsigned>(ctas)), dim3(T), static_cast<size_t>(stages) * p.d * 2, stream, p,
+                          stages, status);
+}
+
 template <int DT>
-int forward(cudaStream_t stream, const NormParams& p) {
+int forward(int device, cudaStream_t stream, const NormParams& p) {
   constexpr int kVec = DT == TVB_F32 ? 4 : 8;
   if (p.d > kLongest)
     return launch_dependent("layer_norm_long", layer_norm_long_kernel<DT>, dim3(static_cast<unsigned>(p.rows)), dim3(1024), 0, stream, p);
   // 16-byte accesses where every row of every operand begins on 16 bytes
   const bool vec = p.d % kVec == 0 && p.x_ld % kVec == 0 && aligned16(p.x) && aligned16(p.y) && aligned16(p.weight) && aligned16(p.bias);
+  if constexpr (DT != TVB_F32) {
+    const bool wide = p.param_dtype == TVB_F32 && (p.weight != nullptr || p.bias != nullptr);
+    if (vec && !wide && p.d > 8 * 1024 && p.d <= 16 * 1024)
+      return p.d <= 32 * 384 ? forward_ring<DT, 384>(device, stream, p) : forward_ring<DT, 512>(device, stream, p);
+  }
   return vec ? forward_vec<DT, kVec>(stream, p) : forward_vec<DT, 1>(stream, p);
 }
 
@@ -894,9 +1010,9 @@ extern "C" int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm
   p.x = x; p.weight = weight; p.bias = bias; p.y = y; p.mean = mean; p.rstd = rstd;
   p.x_ld = rows > 1 ? x_sm : d;
   p.rows = rows; p.d = static_cast<int>(d); p.param_dtype = param_dtype; p.eps = eps;
-  if (dtype == TVB_F32) return forward<TVB_F32>(stream, p);
-  if (dtype == TVB_F16) return forward<TVB_F16>(stream, p);
-  return forward<TVB_BF16>(stream, p);
+  if (dtype == TVB_F32) return forward<TVB_F32>(device, stream, p);
+  if (dtype == TVB_F16) return forward<TVB_F16>(device, stream, p);
+  return forward<TVB_BF16>(device, stream, p);
 }
 
 extern "C" uint64_t tvb_layer_norm_backward_workspace_bytes(int64_t rows, int64_t d) {
