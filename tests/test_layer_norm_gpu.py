@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 SIZES = [(1, 1), (3, 2), (5, 7), (1, 64), (33, 128), (1000, 16), (7, 255), (129, 256), (2, 512), (65, 520), (300, 1003), (40, 1024),
          (17, 2048), (9, 2056), (2000, 768), (5, 4096), (6, 4097), (4, 8192), (3, 8200), (2, 16384), (3, 16392), (2, 32768), (2, 33000),
          (1300, 1032), (700, 2048), (2500, 1032), (3000, 4096), (400, 8192), (333, 8200), (500, 4104),
-         (1500, 8704), (1400, 12296), (1000, 16376)]
+         (1301, 500), (2001, 384), (303, 5120), (200, 6001), (1500, 8704), (1400, 12296), (1000, 16376)]
 
 
 def run(fn, *args, **kw):

@@ -862,8 +862,9 @@ int64_t norm_parts(int64_t rows, int64_t d) {
   return std::min(ceil_div(rows, groups), most);
 }
 
-// The forward kernel's shape (bfloat16, us: 65536 x 768 with a warp per row 44, a CTA of 128 for two rows 76; 16384 x 4096 with 32 values
-// of one row per thread 54, 16 of two rows 56; 4096 x 16384: 93 and 77).
+// The forward kernel's shape: as few threads as hold a row (bfloat16, us: 65536 x 768 with a warp per row 42, a CTA of 128 for two
+// rows 76; 65536 x 512 with 32 values of one row per thread 35, 16 of two rows 28; 16384 x 4096 50 and 56; 16384 x 5120 with 384
+// threads 84, with 512 94).
 template <int DT, int VEC>
 int forward_vec(cudaStream_t stream, const NormParams& p) {
   auto run = [&](auto kernel, int t, int rows) {
@@ -872,9 +873,11 @@ int forward_vec(cudaStream_t stream, const NormParams& p) {
   };
   if (p.d <= 16 * 8) return run(layer_norm_kernel<DT, VEC, 8, 16, 2>, 8, 2);
   if (p.d <= 32 * 8) return run(layer_norm_kernel<DT, VEC, 8, 32, 1>, 8, 1);
+  if (p.d <= 16 * 32) return run(layer_norm_kernel<DT, VEC, 32, 16, 2>, 32, 2);
   if (p.d <= 32 * 32) return run(layer_norm_kernel<DT, VEC, 32, 32, 1>, 32, 1);
   if (p.d <= 16 * 128) return run(layer_norm_kernel<DT, VEC, 128, 16, 2>, 128, 2);
   if (p.d <= 32 * 128) return run(layer_norm_kernel<DT, VEC, 128, 32, 1>, 128, 1);
+  if (p.d <= 16 * 384) return run(layer_norm_kernel<DT, VEC, 384, 16, 2>, 384, 2);
   if (p.d <= 16 * 512) return run(layer_norm_kernel<DT, VEC, 512, 16, 2>, 512, 2);
   if (p.d <= 16 * 1024) return run(layer_norm_kernel<DT, VEC, 1024, 16, 2>, 1024, 2);
   return run(layer_norm_kernel<DT, VEC, 1024, 32, 1>, 1024, 1);
