@@ -47,7 +47,7 @@ LinearCopy make_readable(int dtype, const void** p, int64_t rows, int64_t cols, 
 }
 
 int run_product(int device, cudaStream_t stream, const LinearProduct& p) {
-  if (p.dtype == TVB_F32) return linear_simt(stream, p);
+  if (p.dtype == TVB_F32) return linear_simt(device, stream, p);
   return linear_large(p) ? linear_pair(device, stream, &p, 1) : linear_split(device, stream, &p, 1);
 }
 

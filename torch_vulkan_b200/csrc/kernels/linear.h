@@ -28,7 +28,7 @@ struct LinearProduct {
   int activation;        // TvbActivation
 };
 
-int linear_simt(cudaStream_t stream, const LinearProduct& p);  // float32
+int linear_simt(int device, cudaStream_t stream, const LinearProduct& p);  // float32
 // float16 and bfloat16, on the tensor cores; every operand begins on 16 bytes and its rows are a multiple of 16 bytes apart.
 // `count`: one product, or two that share nothing but their launch.
 int linear_split(int device, cudaStream_t stream, const LinearProduct* p, int count);  // two: dx and dw, in this order
