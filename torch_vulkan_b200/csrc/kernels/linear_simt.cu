@@ -1,10 +1,13 @@
 // The products of linear.h in float32, on the CUDA cores (the tensor cores have no float32).
 //
-// A CTA of eight warps makes a tile of 128 IV columns i and 8 WJ rows j: lane l holds columns 4 l .. 4 l + 3 (of each 128), a
-// warp eight rows, and the 8 / WJ warps of the same rows take every (8 / WJ)-th r. Per r a lane reads IV float4 of P and the
-// warp's eight values of Q, which stand in shared memory twice each, as the operands of a two-float32 instruction: 16 IV of
-// those against IV + 4 loads. The next KSTEP values of r are on their way to registers meanwhile. With few tiles a cluster of
-// CTAs cuts r into parts and joins its sums through distributed shared memory, in a fixed order.
+// A CTA of eight warps makes a tile of 128 columns i and 8 WJ rows j: lane l holds columns 4 l .. 4 l + 3, a warp eight rows, and
+// the 8 / WJ warps of the same rows take every (8 / WJ)-th r. Per r a lane reads a float4 of P and the warp's eight values of Q,
+// which stand in shared memory twice each, as the operands of a two-float32 instruction: 16 of those against 5 loads. The next
+// KSTEP values of r are on their way to registers meanwhile. With few tiles a cluster of CTAs cuts r into parts and joins its
+// sums through distributed shared memory, in a fixed order.
+//
+// Few rows are bound by reading the weights (1 x 4096 x 14336: 87 us, 2.7 TB/s), many by the shared memory (2048 x 4096 x 4096:
+// 2.1 ms, 33 TFLOP/s; tiles of 256 columns by two CTAs per SM spilled registers, 2.9 ms, by one 2.2).
 #include "../core/common.h"
 #include "launch.h"
 #include "linear.h"
@@ -17,9 +20,9 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 
-template <int IV, int WJ, int KSTEP>
+template <int WJ, int KSTEP>
 struct SimtCfg {
-  static constexpr int kTI = 128 * IV, kTJ = 8 * WJ, kWR = kWarps / WJ;
+  static constexpr int kTI = 128, kTJ = 8 * WJ, kWR = kWarps / WJ;
   static constexpr int kPitchP = kTI, kPitchQ = 2 * kTJ + 4;
   // four rows r .. r + 3 of P have their float4s in an order of their own: neighbouring threads then write to different banks
   static constexpr int kTurn = KSTEP < 32 ? 32 / KSTEP : 1;
@@ -42,9 +45,9 @@ __device__ __forceinline__ float4 fetch4(const float* at, int64_t n, bool vec) {
 
 __device__ __forceinline__ uint64_t both(float f) { return ptx::both_f32x2(f); }
 
-template <int IV, int WJ, int KSTEP, bool P_MN, bool Q_MN>
+template <int WJ, int KSTEP, bool P_MN, bool Q_MN>
 __global__ void __launch_bounds__(kThreads, 2) linear_simt_kernel(const LinearProduct p, const uint32_t tiles_i, const int p_vec, const int q_vec) {
-  using Cfg = SimtCfg<IV, WJ, KSTEP>;
+  using Cfg = SimtCfg<WJ, KSTEP>;
   constexpr int kTI = Cfg::kTI, kTJ = Cfg::kTJ, kWR = Cfg::kWR, kPitchP = Cfg::kPitchP, kPitchQ = Cfg::kPitchQ;
   extern __shared__ __align__(16) float smem[];
   float* ps = smem;
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_simt_kernel(const LinearPr
     }
   };
 
-  uint64_t acc[IV][2][8] = {};
+  uint64_t acc[2][8] = {};
   if (s0 < s1) fetch(s0);
 #pragma unroll 1
   for (int64_t s = s0; s < s1; s++) {
@@ -119,30 +122,25 @@ __global__ void __launch_bounds__(kThreads, 2) linear_simt_kernel(const LinearPr
 #pragma unroll 4
     for (int r = wr; r < KSTEP; r += kWR, qr += kWR * kPitchQ) {
       const float* pr = ps + r * kPitchP + (lane ^ Cfg::turn(r >> 2)) * 4;
-      ulonglong2 a[IV], b[4];
-#pragma unroll
-      for (int v = 0; v < IV; v++) a[v] = *reinterpret_cast<const ulonglong2*>(pr + 128 * v);
+      const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(pr);
+      ulonglong2 b[4];
 #pragma unroll
       for (int c = 0; c < 4; c++) b[c] = *reinterpret_cast<const ulonglong2*>(qr + 4 * c);
 #pragma unroll
-      for (int v = 0; v < IV; v++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          acc[v][0][2 * c] = ptx::fma_f32x2(a[v].x, b[c].x, acc[v][0][2 * c]);
-          acc[v][1][2 * c] = ptx::fma_f32x2(a[v].y, b[c].x, acc[v][1][2 * c]);
-          acc[v][0][2 * c + 1] = ptx::fma_f32x2(a[v].x, b[c].y, acc[v][0][2 * c + 1]);
-          acc[v][1][2 * c + 1] = ptx::fma_f32x2(a[v].y, b[c].y, acc[v][1][2 * c + 1]);
-        }
+      for (int c = 0; c < 4; c++) {
+        acc[0][2 * c] = ptx::fma_f32x2(a.x, b[c].x, acc[0][2 * c]);
+        acc[1][2 * c] = ptx::fma_f32x2(a.y, b[c].x, acc[1][2 * c]);
+        acc[0][2 * c + 1] = ptx::fma_f32x2(a.x, b[c].y, acc[0][2 * c + 1]);
+        acc[1][2 * c + 1] = ptx::fma_f32x2(a.y, b[c].y, acc[1][2 * c + 1]);
+      }
     }
   }
 
   // the sums to shared memory, those of the warps with the same rows added up, then the cluster's
   __syncthreads();
 #pragma unroll
-  for (int v = 0; v < IV; v++)
-#pragma unroll
-    for (int c = 0; c < 8; c++)
-      *reinterpret_cast<ulonglong2*>(smem + (wr * kTJ + wj * 8 + c) * kTI + 128 * v + 4 * lane) = make_ulonglong2(acc[v][0][c], acc[v][1][c]);
+  for (int c = 0; c < 8; c++)
+    *reinterpret_cast<ulonglong2*>(smem + (wr * kTJ + wj * 8 + c) * kTI + 4 * lane) = make_ulonglong2(acc[0][c], acc[1][c]);
   const int rows = static_cast<int>(p.J - j0 < kTJ ? p.J - j0 : kTJ);
   if constexpr (kWR > 1) {
     __syncthreads();
@@ -178,10 +176,10 @@ __global__ void __launch_bounds__(kThreads, 2) linear_simt_kernel(const LinearPr
   ptx::cluster_sync();  // no CTA's shared memory is released while another may read it
 }
 
-template <int IV, int WJ, int KSTEP, bool P_MN, bool Q_MN>
+template <int WJ, int KSTEP, bool P_MN, bool Q_MN>
 int simt_run(int device, cudaStream_t stream, const LinearProduct& p) {
-  using Cfg = SimtCfg<IV, WJ, KSTEP>;
-  auto kernel = linear_simt_kernel<IV, WJ, KSTEP, P_MN, Q_MN>;
+  using Cfg = SimtCfg<WJ, KSTEP>;
+  auto kernel = linear_simt_kernel<WJ, KSTEP, P_MN, Q_MN>;
   static bool configured[64] = {};
   if (!configured[device & 63]) {
     TVB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
@@ -200,10 +198,9 @@ int simt_run(int device, cudaStream_t stream, const LinearProduct& p) {
 
 template <bool P_MN, bool Q_MN>
 int simt_shape(int device, cudaStream_t stream, const LinearProduct& p) {
-  if (p.J <= 8) return simt_run<1, 1, 64, P_MN, Q_MN>(device, stream, p);
-  if (p.J <= 32) return simt_run<1, 4, 32, P_MN, Q_MN>(device, stream, p);
-  if (ceil_div(p.I, 256) * ceil_div(p.J, 64) < 2ll * sm_count(device)) return simt_run<1, 8, 16, P_MN, Q_MN>(device, stream, p);
-  return simt_run<2, 8, 8, P_MN, Q_MN>(device, stream, p);
+  if (p.J <= 8) return simt_run<1, 64, P_MN, Q_MN>(device, stream, p);
+  if (p.J <= 32) return simt_run<4, 32, P_MN, Q_MN>(device, stream, p);
+  return simt_run<8, 16, P_MN, Q_MN>(device, stream, p);
 }
 
 }  // namespace
