@@ -322,3 +322,33 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+FIRST_CALLS = """
+import torch
+import torch_vulkan_b200
+from torch_vulkan_b200 import cabi
+x, w = torch.randn(40, 256, device="cuda").bfloat16(), torch.randn(512, 256, device="cuda").bfloat16()
+long = torch.randn(3, 12000, device="cuda").bfloat16()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, z = cabi.linear(x, w, activation="gelu", save_preactivation=True)
+    grads = cabi.linear_backward(y, x, w, z, activation="gelu")
+    norm = cabi.layer_norm(long)
+graph.replay()
+torch.cuda.synchronize()
+y2, z2 = cabi.linear(x, w, activation="gelu", save_preactivation=True)
+again = [y2, z2, *cabi.linear_backward(y2, x, w, z2, activation="gelu"), *cabi.layer_norm(long)]
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip([y, z, *grads, *norm], again))
+print("the same")
+"""
+
+
+@gpu
+def test_the_first_calls_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]

@@ -116,6 +116,25 @@ def test_backward_parts_and_repeats(dtype, d):
             assert (a is not None) == asked and (a is None or torch.equal(a, f))
 
 
+@pytest.mark.parametrize("d", [4096, 1000, 16384])
+def test_offsets_beyond_31_bits(d):
+    rows = 2 ** 31 // d + 300
+    x, dy = (torch.randn(rows, d, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    g, b = params(d, torch.bfloat16)
+    y, mean, rstd = run(cabi.layer_norm, x, g, b)
+    dx, dg, db = run(cabi.layer_norm_backward, dy, x, mean, rstd, g)
+    for part in (slice(0, 50), slice(rows - 400, rows)):
+        want = D.layer_norm64(x[part], g, b, 1e-5)
+        for name, got in (("y", y), ("mean", mean), ("rstd", rstd)):
+            D.check((name, part), got[part], *want[name])
+        D.check(("dx", part), dx[part], *D.layer_norm_backward64(dy[part], x[part], mean[part], rstd[part], g)["dx"])
+    cols = slice(d - 16, d)  # (the sums over the rows, of some columns)
+    dy64, h = dy[:, cols].double(), (x[:, cols].double() - mean.double()[:, None]) * rstd.double()[:, None]
+    slack = D.sum_slack(rows) * (1 + dy64.abs() * (1 + h.abs())).sum(0)
+    D.check("dg", dg[cols], (dy64 * h).sum(0), D.rounded((dy64 * h).sum(0), slack, torch.bfloat16))
+    D.check("db", db[cols], dy64.sum(0), D.rounded(dy64.sum(0), slack, torch.bfloat16))
+
+
 def test_gradients_against_differences():
     rows, d, eps = 5, 24, 1e-5
     x, dy = values(rows, d, torch.float32), values(rows, d, torch.float32, seed=7)

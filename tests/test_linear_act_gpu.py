@@ -211,6 +211,47 @@ def test_results_repeat_bit_for_bit(dtype, m, k, n):
         assert all(torch.equal(a, c) for a, c in zip(first, again))
 
 
+@pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 36000), (torch.float16, 36001), (torch.float32, 36000)])
+def test_offsets_beyond_31_bits(dtype, n):
+    """Outputs and gradients of more than 2^31 values, checked where the offsets pass 2^31 and at the end."""
+    m, k = 66000, 24
+    x, w, b, _ = operands(m, k, n, dtype, seed=30)[:3] + (None,)
+    r = torch.randn(m, n, device="cuda", dtype=dtype)
+    y, z = run(cabi.linear, x, w, b, residual=r, activation="silu", save_preactivation=True)
+    at = 2 ** 31 // n
+    for rows in (slice(0, 100), slice(at - 100, at + 300), slice(m - 100, m)):
+        want, tol, z64, ztol = D.linear64(x[rows], w, b, r[rows], "silu")
+        D.check(("y", rows), y[rows], want, tol)
+        D.check(("z", rows), z[rows], z64, ztol)
+    dx, dw, db = run(cabi.linear_backward, r, x, w, z, activation="silu")
+    for rows in (slice(0, 100), slice(at - 100, at + 300), slice(m - 100, m)):
+        D.check(("dx", rows), dx[rows], *D.linear_backward64(r[rows], x[rows], w, z[rows], "silu")["dx"])
+    cols = slice(n - 70, n)
+    want = D.linear_backward64(r[:, cols], x, w[cols], z[:, cols], "silu")
+    D.check("dw", dw[cols], *want["dw"])
+    D.check("db", db[cols], *want["db"])
+
+
+def test_more_rows_than_a_grids_second_dimension():
+    x, w, b, _ = operands(4_300_000, 4, 9, torch.float32, seed=31)
+    want, tol, _, _ = D.linear64(x, w, b, None, "relu")
+    D.check("y", run(cabi.linear, x, w, b, activation="relu"), want, tol)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1000, 4099), (1, 4096, 256), (3, 4095, 1024), (8, 700, 512), (9, 512, 512), (32, 4096, 128), (33, 2000, 300),
+                                   (500, 4096, 64), (64, 64, 4096)])
+def test_float32_shapes(m, k, n):
+    """Tiles of 8, 32 and 64 rows, r cut in one to eight parts, operands on and off 16 bytes."""
+    x, w, b, dy = operands(m, k, n, torch.float32, seed=32)
+    want, tol, z64, ztol = D.linear64(x, w, b, dy, "gelu")
+    y, z = run(cabi.linear, x, w, b, residual=dy, activation="gelu", save_preactivation=True)
+    D.check("y", y, want, tol)
+    D.check("z", z, z64, ztol)
+    want = D.linear_backward64(dy, x, w, z, "gelu")
+    for name, g in zip(("dx", "dw", "db"), run(cabi.linear_backward, dy, x, w, z, activation="gelu")):
+        D.check(name, g, *want[name])
+
+
 def test_gradients_against_differences():
     """d/dt L(x + t v) for L = sum(dy * y), by central differences of the 64-bit form, against the returned gradients in
     float32: the formula is the derivative of the forward pass, in every operand."""

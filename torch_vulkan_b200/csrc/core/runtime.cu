@@ -95,6 +95,25 @@ int count_devices_locked() {
   return n;
 }
 
+// The stream and the status word of a device's first use.
+int start_locked(int device, DeviceState& d) {
+  TVB_CUDA(cudaSetDevice(device));
+  if (d.own_stream == nullptr) TVB_CUDA(cudaStreamCreateWithFlags(&d.own_stream, cudaStreamNonBlocking));
+  if (d.stream == nullptr) d.stream = d.own_stream;
+  if (d.status_host == nullptr) TVB_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&d.status_host), 256, cudaHostAllocDefault));
+  *d.status_host = 0;
+  int* status = nullptr;
+  TVB_CUDA(cudaMalloc(&status, 256));
+  cudaError_t err = cudaMemsetAsync(status, 0, 256, d.own_stream);
+  if (err == cudaSuccess) err = cudaStreamSynchronize(d.own_stream);
+  if (err != cudaSuccess) {
+    cudaFree(status);
+    return fail_cuda("cudaMemsetAsync", err);
+  }
+  d.status = status;
+  return 0;
+}
+
 // Under g_mutex. Checks and initialises device state on first use.
 int state_locked(int device, DeviceState** out) {
   int n = count_devices_locked();
@@ -117,11 +136,13 @@ int state_locked(int device, DeviceState** out) {
     }
   }
   if (!d.usable) return fail(d.why);
-  if (d.own_stream == nullptr) {
-    cudaError_t err = cudaSetDevice(device);
-    if (err == cudaSuccess) err = cudaStreamCreateWithFlags(&d.own_stream, cudaStreamNonBlocking);
-    if (err != cudaSuccess) return fail_cuda("cudaStreamCreateWithFlags", err);
-    if (d.stream == nullptr) d.stream = d.own_stream;
+  if (d.own_stream == nullptr || d.status == nullptr) {
+    // (another library may be recording a graph on this thread with our first call in it: these calls are no part of that)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const int rc = start_locked(device, d);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (rc != 0) return -1;
   }
   *out = &d;
   return 0;
@@ -198,13 +219,6 @@ int status_word(int device, int** out) {
   std::lock_guard<std::mutex> lock(g_mutex);
   DeviceState* d = nullptr;
   if (state_locked(device, &d) != 0) return -1;
-  if (d->status == nullptr) {
-    TVB_CUDA(cudaSetDevice(device));
-    TVB_CUDA(cudaMalloc(&d->status, 256));
-    TVB_CUDA(cudaMemsetAsync(d->status, 0, 256, d->stream));
-    TVB_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&d->status_host), 256, cudaHostAllocDefault));
-    *d->status_host = 0;
-  }
   *out = d->status;
   return 0;
 }

@@ -12,7 +12,9 @@ int check_linear(const std::string& fn, int dtype, int activation, int64_t m, in
   TVB_REQUIRE(is_float(dtype), fn + ": float32, float16 or bfloat16 only");
   TVB_REQUIRE(activation >= TVB_ACT_NONE && activation <= TVB_ACT_SILU, fn + ": unknown activation");
   TVB_REQUIRE(m >= 0 && n >= 0 && k >= 0, fn + ": negative size");
-  TVB_REQUIRE(m < (int64_t(1) << 31) && n < (int64_t(1) << 31) && k < (int64_t(1) << 31), fn + ": a size beyond 2^31 - 1");
+  // (the last tile's far end must fit 32 bits too)
+  constexpr int64_t kMost = (int64_t(1) << 31) - 1024;
+  TVB_REQUIRE(m <= kMost && n <= kMost && k <= kMost, fn + ": a size beyond 2^31 - 1024");
   return 0;
 }
 
@@ -85,7 +87,7 @@ extern "C" int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, co
   const void* outs[3] = {y, preact, need != 0 ? workspace : nullptr};
   const int64_t out_bytes[3] = {y_bytes, y_bytes, static_cast<int64_t>(need)};
   for (int i = 0; i < 3; i++) {
-    const bool in_place = i == 0 && residual == y && residual_sm == n;  // every element is read by the thread that writes it
+    const bool in_place = i == 0 && residual == y && residual_sm == n;  // every element is read before it is written, by the same thread or the same warp
     TVB_REQUIRE(!overlap(outs[i], out_bytes[i], x, span(m, k, x_sm, es)) && !overlap(outs[i], out_bytes[i], w, span(n, k, w_sn, es)) &&
                     !overlap(outs[i], out_bytes[i], bias, n * es) &&
                     (in_place || !overlap(outs[i], out_bytes[i], residual, span(m, n, residual_sm, es))),
