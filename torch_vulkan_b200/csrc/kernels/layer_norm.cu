@@ -15,7 +15,6 @@
 // bit). Rows that are short, or not whole 16-byte pieces, take the plain form of the kernel.
 #include "../core/common.h"
 #include "launch.h"
-#include "linear_math.cuh"
 #include "numerics.cuh"
 #include "ptx_pair.cuh"
 
@@ -886,9 +885,17 @@ int forward_vec(cudaStream_t stream, const NormParams& p) {
 template <int DT, int VEC>
 int backward_vec(cudaStream_t stream, const NormParams& p, int64_t parts) {
   const int t = norm_group(p.d, kValsBwd);
-  auto kernel = t == 8 ? layer_norm_backward_kernel<DT, VEC, 8> : t == 32 ? layer_norm_backward_kernel<DT, VEC, 32>
-              : t == 128 ? layer_norm_backward_kernel<DT, VEC, 128> : t == 256 ? layer_norm_backward_kernel<DT, VEC, 256>
-              : t == 512 ? layer_norm_backward_kernel<DT, VEC, 512> : layer_norm_backward_kernel<DT, VEC, 1024>;
+  auto kernel = t == 8 ? layer_norm_backward_kernel<DT, VEC, 8> : layer_norm_backward_kernel<DT, VEC, 32>;
+  if constexpr (VEC == 1) {
+    if (t >= 128)
+      kernel = t == 128 ? layer_norm_backward_kernel<DT, VEC, 128> : t == 256 ? layer_norm_backward_kernel<DT, VEC, 256>
+             : t == 512 ? layer_norm_backward_kernel<DT, VEC, 512> : layer_norm_backward_kernel<DT, VEC, 1024>;
+  } else {  // (the rest goes through the ring, but for float32 rows of which it cannot hold two)
+    if (t > 32) {
+      if constexpr (DT != TVB_F32) return fail("tvb_layer_norm_backward: no kernel for this row");
+      else kernel = layer_norm_backward_kernel<DT, VEC, 1024>;
+    }
+  }
   return launch_dependent("layer_norm_backward", kernel, dim3(static_cast<unsigned>(parts)), dim3(t < 128 ? 128 : t), 0, stream, p);
 }
 

@@ -11,6 +11,10 @@
 // A launch takes one product or two: the backward pass multiplies dz by w and by x at once. The tiles of the product with the
 // longer r come first; pairs that get one tile of it less than others start on the second product meanwhile, and the rest of its
 // tiles are dealt out in turn. The schedule is computed from the sizes alone (no counters in memory), so launches share nothing.
+//
+// Measured (us per call, seconds-long runs, in which the GPU is held at its power limit): 2048 x 4096 x 14336 bfloat16 with gelu and its
+// input saved 213 (1.13 PFLOP/s; the product alone 195); its gradients 434, of which the pass over dz takes 40 and both products
+// 385 (1.25 PFLOP/s).
 //   warps 0-7: epilogue (warp w reads TMEM lanes 32 (w % 4) ..., every second 32 columns)
 //   warp 8, one lane: TMA; warp 9, one lane of CTA 0: MMA. All mbarrier waits are bounded.
 #include <cuda.h>
