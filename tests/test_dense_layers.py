@@ -37,6 +37,24 @@ def test_fuse_linears_keeps_the_function_and_the_parameters():
     assert L.swap_linears(b) == ["3", "7"] and isinstance(b[1], L.LinearAct)
 
 
+def test_fuse_linears_with_shared_modules_hooks_and_own_forward_passes():
+    torch.manual_seed(3)
+    relu, lin = nn.ReLU(), nn.Linear(16, 16)
+
+    class Twice(nn.Sequential):
+        def forward(self, x):
+            return super().forward(x) + self[0](x)
+
+    hooked = nn.Linear(16, 16)
+    hooked.register_forward_hook(lambda module, args, out: out + 1)
+    model = nn.Sequential(lin, relu, nn.Linear(16, 16), relu, nn.GELU(), lin, nn.Tanh(), lin, nn.SiLU(), hooked, nn.ReLU(),
+                          Twice(nn.Linear(16, 16), nn.ReLU()))
+    x = torch.randn(4, 16, generator=D.gen(2))
+    want = model(x)
+    assert L.fuse_linears(model) == ["0", "2", "7"]
+    assert torch.equal(model(x), want)
+
+
 def test_linear_act_on_the_cpu_and_what_it_refuses():
     lin = nn.Linear(8, 6)
     x, r = torch.randn(2, 3, 8), torch.randn(2, 3, 6)
@@ -199,6 +217,34 @@ def test_feed_forward_block_forward_and_backward(dtype, rel, rows):
     vx.backward(dy.to("vk"))
     for p, old in zip([p for vb, _ in pairs for p in vb.parameters()], before):
         assert torch.equal(p.grad.cpu(), old + old)
+
+
+@gpu
+@pytest.mark.parametrize("shape,n", [((3, 0), 8), ((2, 0, 16), 8), ((2, 5, 16), 0), ((16,), 8), ((1, 1, 16), 8)])
+def test_linear_act_odd_shapes(shape, n):
+    x = torch.randn(shape, generator=D.gen(1)).to(torch.bfloat16)
+    w = torch.randn(n, shape[-1], generator=D.gen(2)).to(torch.bfloat16)
+    b = torch.randn(n, generator=D.gen(3)).to(torch.bfloat16)
+    vx, vw, vb = vk_leaf(x), vk_leaf(w), vk_leaf(b)
+    y = L.linear_act(vx, vw, vb, "silu")
+    assert y.shape == (*shape[:-1], n)
+    want = F.silu(F.linear(x.double(), w.double(), b.double()))
+    assert ((y.detach().cpu().double() - want).abs() <= 2.0 ** -7 * want.abs() + 2.0 ** -9).all()
+    y.backward(torch.ones(y.shape, dtype=torch.bfloat16).to("vk"))
+    assert vx.grad.shape == x.shape and vw.grad.shape == w.shape and vb.grad.shape == b.shape
+
+
+@gpu
+def test_nothing_is_kept_where_no_gradient_is_asked_for(monkeypatch):
+    kept = []
+    plain = cabi.linear
+    monkeypatch.setattr(cabi, "linear", lambda *a, **kw: kept.append(kw["save_preactivation"]) or plain(*a, **kw))
+    layer = L.LinearAct(64, 32, activation="gelu").to(torch.bfloat16).to("vk")
+    x = torch.randn(4, 64, generator=D.gen(1)).to(torch.bfloat16).to("vk")
+    y = layer(x)
+    with torch.no_grad():
+        assert torch.equal(layer(x).cpu(), y.detach().cpu())
+    assert kept == [True, False]
 
 
 @gpu

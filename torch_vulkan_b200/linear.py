@@ -19,6 +19,8 @@ activation and the residual stream it joins in one call, act(x @ weight.T + bias
 puts it in place of the Linear / activation pairs of a model.
 """
 
+import math
+
 import torch
 import torch.nn.functional as F
 from torch import nn
@@ -173,30 +175,32 @@ class DynInt4Linear(nn.Module, _ShardedMixin):
 def _rows(t, cols):
     """A [rows, cols] form of t that the kernels can read: contiguous columns, rows that do not overlap (a copy where there is
     none, for instance of an expanded gradient)."""
-    t = t.reshape(-1, cols)
+    t = t.reshape(math.prod(t.shape[:-1]), cols)
     if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
         t = t.contiguous()
     return t
 
 
+def _apply(x, w, bias, residual, activation, keep):
+    """The kernel on matrices: (y, the values before the activation or None)."""
+    from . import cabi
+
+    r = None if residual is None else _rows(residual, w.shape[0])
+    y = cabi.linear(x, w, bias, residual=r, activation=activation, save_preactivation=keep)
+    return y if keep else (y, None)
+
+
 class _LinearAct(torch.autograd.Function):
     """cabi.linear and cabi.linear_backward as one differentiable operation. Keeps x, the weight and, with an activation, the
-    values before it; only where something needs a gradient."""
+    values before it."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        from . import cabi
-
-        n, k = weight.shape
-        x2 = _rows(x, k)
-        w2 = _rows(weight, k)
-        r2 = None if residual is None else _rows(residual, n)
-        keep = activation != "none" and any(ctx.needs_input_grad[:3])
-        y = cabi.linear(x2, w2, bias, residual=r2, activation=activation, save_preactivation=keep)
-        y, z = y if keep else (y, None)
+        x2, w2 = _rows(x, weight.shape[1]), _rows(weight, weight.shape[1])
+        y, z = _apply(x2, w2, bias, residual, activation, activation != "none" and any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x2, w2, z)
         ctx.activation, ctx.x_shape = activation, x.shape
-        return y.view(*x.shape[:-1], n)
+        return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
@@ -230,7 +234,12 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         y = {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"),
              "silu": F.silu}[activation](y)
         return y if residual is None else y + residual
-    return _LinearAct.apply(x, weight, bias if bias is None or bias.is_contiguous() else bias.contiguous(), residual, activation)
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _LinearAct.apply(x, weight, bias, residual, activation)
+    k = weight.shape[1]
+    return _apply(_rows(x, k), _rows(weight, k), bias, residual, activation, False)[0].view(*x.shape[:-1], weight.shape[0])
 
 
 class LinearAct(nn.Linear):
@@ -267,18 +276,23 @@ def _activation_name(module):
     return "silu" if type(module) is nn.SiLU else None
 
 
+def _hooked(module):
+    return any(getattr(module, kind) for kind in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
+
+
 def fuse_linears(model):
     """Replaces, in every nn.Sequential under `model` (in place), an nn.Linear that is followed by ReLU, GELU or SiLU with one
     LinearAct that shares its parameters, and the activation with nn.Identity (so that the other layers keep their names).
+    Left as they are: layers with hooks (a fused one would not run them), and containers with a forward pass of their own.
     Returns the names of the layers it replaced."""
     replaced = []
     for name, module in list(model.named_modules()):
-        if not isinstance(module, nn.Sequential):
+        if not isinstance(module, nn.Sequential) or type(module).forward is not nn.Sequential.forward:
             continue
-        children = list(module.named_children())
+        children = list(module._modules.items())  # (named_children leaves out a module's second place in the container)
         for (first, linear), (second, act) in zip(children, children[1:]):
             activation = _activation_name(act)
-            if type(linear) is not nn.Linear or activation is None:
+            if type(linear) is not nn.Linear or activation is None or _hooked(linear) or _hooked(act):
                 continue
             setattr(module, first, LinearAct.from_float(linear, activation))
             setattr(module, second, nn.Identity())
