@@ -21,6 +21,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../core/common.h"
 #include "../core/tensormap.h"
@@ -468,14 +469,22 @@ int split_orders(int device, cudaStream_t stream, const LinearProduct* lp, int c
   return fail("tvb_linear: no kernel for this order of the operands");
 }
 
+// Clusters of `size` (1, 2, 3, 4, 6, 8) CTAs that run at once, one or two CTAs per SM, as the runtime counts them on a B200: a
+// cluster stays within a GPC, so the larger ones leave SMs idle.
+int clusters_at_once(int size, int per_sm) {
+  constexpr int kOne[9] = {0, 148, 74, 45, 33, 0, 22, 0, 15}, kTwo[9] = {0, 296, 148, 93, 71, 0, 45, 0, 33};
+  return per_sm == 2 ? kTwo[size] : kOne[size];
+}
+
 // The shape of a launch: which TN and S, and whether the kernel of CTA pairs (linear_pair.cu) is faster. The rule is a model of
 // the time in us, fitted to 1137 measurements of both kernels (1 to 2048 rows, matrices from 512 x 512 to 4096 x 14336, every TN
-// and S): its choices are 2 % slower than the best of each shape on average, 30 % at worst (333 x 4096 x 6144). What it
+// and S): its choices are 1.2 % slower than the best of each shape on average, 25 % at worst (1000 x 512 x 2048). What it
 // says: a step (64 values of r) takes longer as more SMs ask the L2 at once, and as two CTAs share an SM; a tile's way out takes
-// its time by its columns, more when sums are joined; a second round of CTAs is dear; clusters of more than four CTAs start
-// late, and clusters of whole SMs do not all fit. From 74 tiles of 256 x 256 on (one for every pair of SMs) the pairs' kernel is
-// taken whatever the model says: there the GPU is bound by its power, and fetching less counts for more than in a short run
-// (2048 x 4096 x 14336 with gelu: 215 us against 255).
+// its time by its columns, more when sums are joined; clusters of more than four CTAs start late; and clusters run in whole
+// rounds of those that fit at once (200 x 14336 x 4096 bfloat16 in 16 clusters: of six CTAs 33 us, of four 43, of eight, of which
+// 15 fit, 55). From 74 tiles of 256 x 256 on (one for every pair of SMs) the pairs' kernel is taken whatever the model says: there
+// the GPU is bound by its power, and fetching less counts for more than in a short run (2048 x 4096 x 14336 with gelu: 215 us
+// against 255).
 struct Shape {
   int tn, parts;
   double us;
@@ -484,28 +493,28 @@ struct Shape {
 // `count` products in one launch share TN and S.
 double split_cost(const LinearProduct* lp, int count, int tn, int parts) {
   const bool pair = tn >= 64;
-  double ctas = 0, work = 0, longest = 0;
+  const int size = pair ? 2 * parts : parts, per_sm = tn <= 128 ? 2 : 1, fit = clusters_at_once(size, per_sm);
+  double clusters = 0, work = 0, longest = 0;
   for (int k = 0; k < count; k++) {
-    const double n = static_cast<double>(ceil_div(lp[k].I, pair ? 2 * kRows : kRows) * ceil_div(lp[k].J, tn) * parts * (pair ? 2 : 1));
+    const double n = static_cast<double>(ceil_div(lp[k].I, pair ? 2 * kRows : kRows) * ceil_div(lp[k].J, tn));
     const double steps = static_cast<double>(ceil_div(ceil_div(lp[k].R, kStepR), parts));
-    ctas += n;
+    clusters += n;
     work += n * steps;
     longest = std::max(longest, steps);
   }
-  const double per_sm = tn <= 128 ? 2 : 1, load = ctas / 148, rounds = std::max(1.0, load / per_sm);
-  const double alone = tn <= 32 ? 0.297 : tn == 64 ? 0.264 : tn == 128 ? 0.322 : 0.294;
-  double step = alone * (1 + 0.417 * std::min(1.0, load)) * (1 + 0.678 * std::max(0.0, std::min(load, per_sm) - 1));
-  if (tn == 256 && parts >= 3) step *= 1.792;
-  double us = 2.11 + 0.00994 * tn + std::max(longest, work / ctas * rounds) * step + 6.36 * (rounds - 1);
-  if (parts > 1) us += 0.309 + 0.0116 * tn / parts;
-  if (parts * (pair ? 2 : 1) > 4) us += 1.07;
+  const double rounds = std::max(1.0, std::ceil(clusters / fit)), load = std::min<double>(clusters, fit) * size / 148;
+  const double alone = tn <= 32 ? 0.227 : tn == 64 ? 0.252 : tn == 128 ? 0.305 : 0.298;
+  const double step = alone * (1 + 0.314 * std::min(1.0, load)) * (1 + 0.511 * std::max(0.0, std::min<double>(load, per_sm) - 1));
+  double us = 3.6 + 0.00826 * tn + std::max(longest, work / clusters * rounds) * step + 4.32 * (rounds - 1);
+  if (parts > 1) us += 0.379 + 0.00859 * tn / parts;
+  if (size > 4) us += 0.868;
   return us;
 }
 
 int64_t pair_tiles(const LinearProduct& lp) { return ceil_div(lp.I, 256) * ceil_div(lp.J, 256); }
 
 double pair_cost(const LinearProduct& lp) {  // (fewer tiles than pairs)
-  return 1.64 + static_cast<double>(ceil_div(lp.R, kStepR)) * (0.486 + 0.0706 * static_cast<double>(pair_tiles(lp)) / 74) + 2.49;
+  return 0.95 + static_cast<double>(ceil_div(lp.R, kStepR)) * (0.393 + 0.0124 * static_cast<double>(pair_tiles(lp)) / 74) + 3.31;
 }
 
 Shape split_shape(const LinearProduct* lp, int count) {
