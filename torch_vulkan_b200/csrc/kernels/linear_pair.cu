@@ -56,7 +56,7 @@ struct PairProduct {
   void* out;
   void* preact;
   int64_t residual_ld;
-  int I, J, blocks, tiles, tiles_i, tiles_j, q_mn, p_mn, activation, vector_ok;
+  int I, J, blocks, tiles, tiles_i, tiles_j, q_mn, p_mn, activation, vector_ok, alone;
   uint32_t fmt;  // instruction descriptor without the columns
 };
 
@@ -224,6 +224,24 @@ __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, u
     pack32<BF16>(v, y[q]);
   }
   if (d.preact != nullptr) store_tile(&d.map_preact, tile, lane, i, row0);
+  wait_tile(lane);
+  stage32(tile, lane, 0, y[0]);
+  stage32(tile, lane, 1, y[1]);
+  store_tile(&d.map_out, tile, lane, i, row0);
+}
+
+// The same for a product alone (the gradients): nothing between the sums and their rounding. With a short r the read-back is what
+// takes the time, and few warps do it: no branches, both reads of the TMEM on their way at once.
+template <bool BF16>
+__device__ __forceinline__ void store64(const PairProduct& d, uint32_t taddr, uint32_t tile, int lane, int row0, int i) {
+  uint32_t acc[2][32], y[2][16];
+  ptx::tmem_ld_32x32(taddr, acc[0]);
+  ptx::tmem_ld_32x32(taddr + 32, acc[1]);
+  ptx::tmem_ld_wait();
+#pragma unroll
+  for (int q = 0; q < 2; q++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) y[q][e] = pack16<BF16>(ptx::pack_f32x2(acc[q][2 * e], acc[q][2 * e + 1]));
   wait_tile(lane);
   stage32(tile, lane, 0, y[0]);
   stage32(tile, lane, 1, y[1]);
@@ -430,7 +448,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
 #pragma unroll 1
         for (int c = (warp >> 2) * 64; c < t.cols; c += 128) {
           if (row0 >= d.J || t.col + c >= d.I) break;  // (nothing of it is inside)
-          if (d.vector_ok) {
+          if (d.alone) {
+            store64<BF16>(d, taddr + c, tile, lane, row0, t.col + c);
+          } else if (d.vector_ok) {
             finish64<BF16>(d, taddr + c, tile, lane, row0, t.col + c);
           } else {
 #pragma unroll 1
@@ -513,6 +533,7 @@ int pair_product(const LinearProduct& lp, PairProduct* d) {
   const uintptr_t all = reinterpret_cast<uintptr_t>(lp.out) | reinterpret_cast<uintptr_t>(lp.preact) | reinterpret_cast<uintptr_t>(lp.bias) |
                         reinterpret_cast<uintptr_t>(lp.residual);
   d->vector_ok = (all & 15u) == 0 && lp.I % 8 == 0 && (lp.residual == nullptr || lp.residual_ld % 8 == 0);
+  d->alone = d->vector_ok && lp.activation == TVB_ACT_NONE && lp.bias == nullptr && lp.preact == nullptr && lp.residual == nullptr;
   if (d->vector_ok) {
     const CUtensorMapDataType dt = lp.dtype == TVB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (make_tensor_map_2d(&d->map_out, lp.out, dt, lp.I, lp.J, lp.I * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B) != 0) return -1;
