@@ -211,6 +211,23 @@ def test_results_repeat_bit_for_bit(dtype, m, k, n):
         assert all(torch.equal(a, c) for a, c in zip(first, again))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,k,n", [(200, 8192, 2048), (100, 4096, 1000), (40, 6000, 520), (4, 8000, 1024), (500, 1024, 2048), (1000, 1024, 1000),
+                                   (24, 512, 2048), (130, 4104, 264)])
+def test_products_cut_along_their_sums(dtype, m, k, n):
+    """Clusters of two to eight CTAs per tile, ragged last parts, both gradients in one launch and alone."""
+    x, w, b, dy = operands(m, k, n, dtype, seed=33)
+    want, tol, z64, ztol = D.linear64(x, w, b, dy, "relu")
+    y, z = run(cabi.linear, x, w, b, residual=dy, activation="relu", save_preactivation=True)
+    D.check("y", y, want, tol)
+    D.check("z", z, z64, ztol)
+    want = D.linear_backward64(dy, x, w, z, "relu")
+    for need in ((True, True, True), (True, False, False), (False, True, True)):
+        for name, g, asked in zip(("dx", "dw", "db"), run(cabi.linear_backward, dy, x, w, z, activation="relu", need=need), need):
+            if asked:
+                D.check((need, name), g, *want[name])
+
+
 @pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 36000), (torch.float16, 36001), (torch.float32, 36000)])
 def test_offsets_beyond_31_bits(dtype, n):
     """Outputs and gradients of more than 2^31 values, checked where the offsets pass 2^31 and at the end."""
