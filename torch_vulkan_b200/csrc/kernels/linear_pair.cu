@@ -143,16 +143,19 @@ struct PairSchedule {
   }
 };
 
+__device__ __forceinline__ void fetch32(const void* base, int64_t at, uint4 (&x)[4]) {
+  const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
+#pragma unroll
+  for (int q = 0; q < 4; q++) x[q] = s[q];
+}
 template <bool BF16>
-__device__ __forceinline__ void add32(const void* src, int64_t at, uint64_t (&v)[16]) {  // (16-byte aligned)
-  const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + at);
+__device__ __forceinline__ void add32(const uint4 (&x)[4], uint64_t (&v)[16]) {
 #pragma unroll
   for (int q = 0; q < 4; q++) {
-    const uint4 x = s[q];
-    v[4 * q] = ptx::add_f32x2(v[4 * q], unpack16<BF16>(x.x));
-    v[4 * q + 1] = ptx::add_f32x2(v[4 * q + 1], unpack16<BF16>(x.y));
-    v[4 * q + 2] = ptx::add_f32x2(v[4 * q + 2], unpack16<BF16>(x.z));
-    v[4 * q + 3] = ptx::add_f32x2(v[4 * q + 3], unpack16<BF16>(x.w));
+    v[4 * q] = ptx::add_f32x2(v[4 * q], unpack16<BF16>(x[q].x));
+    v[4 * q + 1] = ptx::add_f32x2(v[4 * q + 1], unpack16<BF16>(x[q].y));
+    v[4 * q + 2] = ptx::add_f32x2(v[4 * q + 2], unpack16<BF16>(x[q].z));
+    v[4 * q + 3] = ptx::add_f32x2(v[4 * q + 3], unpack16<BF16>(x[q].w));
   }
 }
 
@@ -203,11 +206,15 @@ __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, u
   for (int q = 0; q < 2; q++) {
     uint32_t w[16];
     uint64_t v[16];
-    load32(taddr + 32 * q, v);
     const int at = i + 32 * q;
     const bool inside = at + 32 <= d.I;  // (else the row's last columns: fewer than 32, a multiple of 8)
+    const int64_t r = static_cast<int64_t>(row0 + lane) * d.residual_ld + at;
+    uint4 bias[4], residual[4];  // (on their way while the TMEM is read)
+    if (d.bias != nullptr && inside) fetch32(d.bias, at, bias);
+    if (d.residual != nullptr && live && inside) fetch32(d.residual, r, residual);
+    load32(taddr + 32 * q, v);
     if (d.bias != nullptr) {
-      if (inside) add32<BF16>(d.bias, at, v);
+      if (inside) add32<BF16>(bias, v);
       else add_singly<BF16>(d.bias, at, d.I - at, v);
     }
     if (d.preact != nullptr) {
@@ -217,8 +224,7 @@ __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, u
     }
     activate_pairs(v, d.activation);
     if (d.residual != nullptr && live) {
-      const int64_t r = static_cast<int64_t>(row0 + lane) * d.residual_ld + at;
-      if (inside) add32<BF16>(d.residual, r, v);
+      if (inside) add32<BF16>(residual, v);
       else add_singly<BF16>(d.residual, r, d.I - at, v);
     }
     pack32<BF16>(v, y[q]);
