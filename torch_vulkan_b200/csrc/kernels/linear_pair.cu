@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
                       : load_tile<HALVES, false, false>(d, t, rank, at, base, full0, empty0, bar0, abort_flag);
       }
       // no copy of either CTA may still be in flight when the pair's shared memory is released: wait for the last filling of
-      // every slot (slots before at.slot were filled in this round, the others in the round before, if there was one)
+      // every slot (slots before at.slot were filled in this turn of the ring, the others in the turn before, if there was one)
       for (uint32_t s = 0; rank == 0 && s < kStages; s++) {
         volatile int never = 0;
         if (s < at.slot) ptx::mbar_wait(full0 + 8 * s, at.phase, &never);
