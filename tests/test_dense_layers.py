@@ -350,6 +350,47 @@ def test_cuda_tensors_run_on_torchs_stream_and_in_its_graphs():
 
 
 @gpu
+def test_two_streams_and_two_graphs_at_once():
+    """Calls on two streams share nothing: the same bits as one after the other, queued directly and as graphs."""
+    def case(seed):
+        x, w, dy = (torch.randn(*shape, generator=D.gen(seed + i)).to(torch.bfloat16).cuda()
+                    for i, shape in enumerate([(300, 1100), (1300, 1100), (300, 1300)]))
+        return x[:, :1003], w[:, :1003], dy
+
+    def step(x, w, dy):
+        y, z = cabi.linear(x, w, activation="gelu", save_preactivation=True)
+        h, mean, rstd = cabi.layer_norm(y)
+        return [y, h, *cabi.linear_backward(dy, x, w, z, activation="gelu"), *cabi.layer_norm_backward(dy, y, mean, rstd)]
+
+    cases = [case(1), case(50)]
+    torch.cuda.synchronize()
+    want = [step(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(outs, want[i]))
+    graphs, outs = [], []
+    for c in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(*c))
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(outs[i], want[i]))
+
+
+@gpu
 def test_two_threads_at_once():
     x = torch.randn(200, 512, generator=D.gen(1)).to(torch.float16)
     w = (torch.randn(640, 512, generator=D.gen(2)) / 20).to(torch.float16)
