@@ -17,6 +17,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <vector>
 
@@ -31,6 +32,10 @@ struct Block {
   int device;
   uint64_t recording;  // the recording (tvb_graph_begin) during which it was allocated, or 0
 };
+
+// A block that no tensor has any more, out of the pool for as long as a recording may touch it. Several may: one that was made
+// with it, and one during which its tensor went away.
+using Kept = std::shared_ptr<std::pair<uint64_t, void*>>;
 
 struct DeviceState {
   bool checked = false;
@@ -56,7 +61,7 @@ struct DeviceState {
   // reads them as they are).
   uint64_t recording = 0;
   std::multimap<uint64_t, void*> recording_free;
-  std::vector<std::pair<uint64_t, void*>> recording_held;
+  std::vector<Kept> recording_held;
 };
 
 // What a finished recording keeps out of the pool for as long as it can be replayed: its kernels write to blocks whose tensors
@@ -64,7 +69,7 @@ struct DeviceState {
 struct Recording {
   int device;
   uint64_t number;
-  std::vector<std::pair<uint64_t, void*>> blocks;
+  std::vector<Kept> blocks;
 };
 
 std::mutex g_mutex;
@@ -74,7 +79,8 @@ bool g_shutdown = false;
 int g_count = 0;
 uint64_t g_dispatches = 0;
 uint64_t g_recordings = 0;
-std::map<void*, Recording> g_graphs;  // by executable graph
+std::map<void*, Recording> g_graphs;              // by executable graph
+std::map<uint64_t, Recording*> g_graphs_by_number;  // the same, by the number of the recording
 
 bool env_flag(const char* name) {
   const char* v = std::getenv(name);
@@ -161,6 +167,13 @@ void trim_locked(DeviceState& d) {
     d.blocks -= 1;
   }
   d.free_blocks.clear();
+}
+
+// A recording lets go of its blocks: those that no other recording holds go back to the pool.
+void release_locked(DeviceState& d, std::vector<Kept>& blocks) {
+  for (Kept& b : blocks)
+    if (b.use_count() == 1) d.free_blocks.emplace(b->first, b->second);
+  blocks.clear();
 }
 
 }  // namespace
@@ -335,14 +348,19 @@ void tvb_free(void* handle) {
     if (!g_shutdown && b->device < static_cast<int>(g_devices.size())) {
       DeviceState& d = g_devices[b->device];
       // Later users of the block are queued on the same stream, so reuse is ordered after the last use. What a recording uses
-      // stays with it.
-      Recording* owner = nullptr;
-      for (auto& g : g_graphs)
-        if (b->recording != 0 && g.second.device == b->device && g.second.number == b->recording) owner = &g.second;
-      if (d.recording != 0 && b->recording == d.recording) d.recording_free.emplace(b->size, b->ptr);
-      else if (owner != nullptr) owner->blocks.emplace_back(b->size, b->ptr);
-      else if (d.recording != 0) d.recording_held.emplace_back(b->size, b->ptr);
-      else d.free_blocks.emplace(b->size, b->ptr);
+      // stays with it: with the one that it was allocated in, and with the one that is being made.
+      if (d.recording != 0 && b->recording == d.recording) {
+        d.recording_free.emplace(b->size, b->ptr);
+      } else {
+        const auto owner = b->recording != 0 ? g_graphs_by_number.find(b->recording) : g_graphs_by_number.end();
+        if (owner == g_graphs_by_number.end() && d.recording == 0) {
+          d.free_blocks.emplace(b->size, b->ptr);
+        } else {
+          const Kept kept = std::make_shared<std::pair<uint64_t, void*>>(b->size, b->ptr);
+          if (owner != g_graphs_by_number.end()) owner->second->blocks.push_back(kept);
+          if (d.recording != 0) d.recording_held.push_back(kept);
+        }
+      }
       d.allocated -= b->size;
     }
   }
@@ -569,13 +587,12 @@ int tvb_graph_end(int device, void** graph_exec) {
     std::lock_guard<std::mutex> lock(g_mutex);
     DeviceState& d = g_devices[device];
     Recording r{device, d.recording, std::move(d.recording_held)};
-    r.blocks.insert(r.blocks.end(), d.recording_free.begin(), d.recording_free.end());
+    for (auto& b : d.recording_free) r.blocks.push_back(std::make_shared<std::pair<uint64_t, void*>>(b.first, b.second));
     d.recording_held.clear();
     d.recording_free.clear();
     d.recording = 0;
-    if (joined == 0 && err == cudaSuccess) g_graphs.emplace(exec, std::move(r));
-    else
-      for (auto& b : r.blocks) d.free_blocks.emplace(b.first, b.second);
+    if (exec != nullptr) g_graphs_by_number[r.number] = &g_graphs.emplace(exec, std::move(r)).first->second;
+    else release_locked(d, r.blocks);
   }
   if (joined != 0) return -1;
   if (err != cudaSuccess) return fail_cuda(what, err);
@@ -597,8 +614,9 @@ void tvb_graph_destroy(void* graph_exec) {
     std::lock_guard<std::mutex> lock(g_mutex);
     auto it = g_graphs.find(graph_exec);
     if (it != g_graphs.end()) {
+      g_graphs_by_number.erase(it->second.number);
       if (!g_shutdown)  // (replays that are still queued run before whatever takes these blocks next: one stream)
-        for (auto& b : it->second.blocks) g_devices[it->second.device].free_blocks.emplace(b.first, b.second);
+        release_locked(g_devices[it->second.device], it->second.blocks);
       g_graphs.erase(it);
     }
   }
