@@ -53,3 +53,76 @@ def test_a_block_of_one_recording_given_back_during_another(first_to_go):
     again = torch.empty(shape, device="vk")
     assert tv.memory_stats()["reserved_bytes"] == reserved
     del again
+
+
+class FakeLibrary:
+    """The calls of a recording, without a device."""
+
+    def __init__(self, end_rc=0):
+        self.calls, self.end_rc = [], end_rc
+
+    def tvb_synchronize(self, device):
+        return 0
+
+    def tvb_graph_begin(self, device):
+        self.calls.append("begin")
+        return 0
+
+    def tvb_graph_end(self, device, out):
+        self.calls.append("end")
+        if self.end_rc == 0:
+            out._obj.value = 1234
+        return self.end_rc
+
+    def tvb_graph_destroy(self, graph):
+        self.calls.append(("destroy", graph.value))
+
+    def tvb_last_error(self):
+        return b"the capture was lost"
+
+
+@pytest.mark.parametrize("end_rc,calls", [(0, ["begin", "end", ("destroy", 1234)]), (-1, ["begin", "end"])])
+def test_a_step_that_raises_leaves_no_recording(monkeypatch, end_rc, calls):
+    from torch_vulkan_b200 import cabi
+
+    fake = FakeLibrary(end_rc)
+    monkeypatch.setattr(cabi, "lib", lambda: fake)
+
+    def step():
+        raise KeyError("in the step")
+
+    with pytest.raises(KeyError, match="in the step"):
+        shard.StepGraph(step, warm=False)
+    gc.collect()
+    assert fake.calls == calls
+
+
+def test_a_recording_that_cannot_end_is_an_error(monkeypatch):
+    from torch_vulkan_b200 import cabi
+
+    fake = FakeLibrary(-1)
+    monkeypatch.setattr(cabi, "lib", lambda: fake)
+    with pytest.raises(RuntimeError):
+        shard.StepGraph(lambda: [], warm=False)
+    assert fake.calls == ["begin", "end"]
+
+
+@pytest.mark.gpu
+def test_a_failed_step_gives_its_memory_back():
+    tv.synchronize()
+    made = []
+
+    def step():
+        made.append(torch.empty(333, 4096, device="vk"))  # a size that nothing else here has
+        made.clear()
+        raise KeyError("in the step")
+
+    with pytest.raises(KeyError):
+        shard.StepGraph(step, warm=False)
+    reserved = tv.memory_stats()["reserved_bytes"]
+    again = torch.empty(333, 4096, device="vk")
+    assert tv.memory_stats()["reserved_bytes"] == reserved
+    # the stream runs again
+    x = torch.arange(8.0)
+    assert torch.equal((x.to("vk") + x.to("vk")).cpu(), x + x)
+    del again

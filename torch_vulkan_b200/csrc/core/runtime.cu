@@ -577,12 +577,13 @@ int tvb_graph_end(int device, void** graph_exec) {
   cudaGraph_t graph = nullptr;
   cudaGraphExec_t exec = nullptr;
   const char* what = "cudaStreamEndCapture";
-  cudaError_t err = joined == 0 ? cudaStreamEndCapture(s, &graph) : cudaSuccess;
+  cudaError_t err = cudaStreamEndCapture(s, &graph);  // (also where the lane could not be joined: the stream has to run again)
   if (joined == 0 && err == cudaSuccess) {
     what = "cudaGraphInstantiate";
     err = cudaGraphInstantiate(&exec, graph, 0);
-    cudaGraphDestroy(graph);
+    if (err != cudaSuccess) exec = nullptr;
   }
+  if (graph != nullptr) cudaGraphDestroy(graph);
   {
     std::lock_guard<std::mutex> lock(g_mutex);
     DeviceState& d = g_devices[device];
@@ -594,7 +595,10 @@ int tvb_graph_end(int device, void** graph_exec) {
     if (exec != nullptr) g_graphs_by_number[r.number] = &g_graphs.emplace(exec, std::move(r)).first->second;
     else release_locked(d, r.blocks);
   }
-  if (joined != 0) return -1;
+  if (joined != 0) {
+    cudaGetLastError();
+    return -1;
+  }
   if (err != cudaSuccess) return fail_cuda(what, err);
   *graph_exec = exec;
   return 0;

@@ -449,11 +449,15 @@ class StepGraph:
             fn()
         cabi.check(lib.tvb_synchronize(device_index))
         cabi.check(lib.tvb_graph_begin(device_index))
+        exec_ = ctypes.c_void_p(0)
         try:
             self.outputs = fn()
-        finally:
-            exec_ = ctypes.c_void_p(0)
-            cabi.check(lib.tvb_graph_end(device_index, ctypes.byref(exec_)))
+        except BaseException:
+            # (the step's own error is the one to report; a recording of half a step keeps no memory)
+            if lib.tvb_graph_end(device_index, ctypes.byref(exec_)) == 0:
+                lib.tvb_graph_destroy(exec_)
+            raise
+        cabi.check(lib.tvb_graph_end(device_index, ctypes.byref(exec_)))
         self.exec = exec_
 
     def replay(self):
