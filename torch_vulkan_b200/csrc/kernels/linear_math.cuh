@@ -31,7 +31,17 @@ __device__ __forceinline__ float act_value(float z, int act) {
   }
 }
 
+// max(-most, min(z, most)), a NaN staying one. The derivatives take z so: from `most` on they are at their limits (0 or 1) in float32,
+// and a z far beyond it, or an infinite one, would make them 0 times infinity.
+__device__ __forceinline__ float within(float z, float most) {
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(most));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(-most));
+  return z;
+}
+constexpr float kGeluMost = 30.0f, kSiluMost = 128.0f;
+
 __device__ __forceinline__ float act_slope(float z, int act) {
+  z = within(z, act == TVB_ACT_SILU ? kSiluMost : kGeluMost);
   switch (act) {
     case TVB_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
     case TVB_ACT_GELU: return 0.5f * (1.0f + erff(z * kSqrtHalf)) + z * expf(-0.5f * z * z) * kInvSqrt2Pi;
@@ -84,9 +94,15 @@ __device__ __forceinline__ uint64_t relu_pair(uint64_t z) {
 __device__ __forceinline__ uint64_t size_pair(uint64_t z) {
   float a, b;
   ptx::unpack_f32x2(z, a, b);
-  a = fminf(fabsf(a), 30.0f);
-  b = fminf(fabsf(b), 30.0f);
+  a = fminf(fabsf(a), kGeluMost);
+  b = fminf(fabsf(b), kGeluMost);
   return ptx::pack_f32x2(__float_as_uint(a), __float_as_uint(b));
+}
+
+__device__ __forceinline__ uint64_t within_pair(uint64_t z, float most) {
+  float a, b;
+  ptx::unpack_f32x2(z, a, b);
+  return ptx::pack_f32x2(__float_as_uint(within(a, most)), __float_as_uint(within(b, most)));
 }
 
 // Phi(-a) for a >= 0; *density receives exp(-a^2 / 2). With t = 1 / (1 + 0.36 a), Phi(-a) = exp(-a^2 / 2) t P(t), P of degree 6,
@@ -131,6 +147,7 @@ __device__ __forceinline__ uint64_t slope_pair(uint64_t z) {
   }
   if constexpr (ACT == TVB_ACT_GELU) {  // Phi(z) + z exp(-z^2 / 2) / sqrt(2 pi), Phi(z) = 0.5 + sign(z) (0.5 - Phi(-|z|))
     uint64_t e;
+    z = within_pair(z, kGeluMost);
     const uint64_t q = tail_pair(size_pair(z), &e);
     float s0, s1, z0, z1;
     ptx::unpack_f32x2(ptx::fma_f32x2(q, two(-1.0f), two(0.5f)), s0, s1);
@@ -139,6 +156,7 @@ __device__ __forceinline__ uint64_t slope_pair(uint64_t z) {
     return ptx::fma_f32x2(ptx::mul_f32x2(z, two(kInvSqrt2Pi)), e, ptx::add_f32x2(s, two(0.5f)));
   }
   if constexpr (ACT == TVB_ACT_GELU_TANH) {  // with s = sigmoid(2 u): s + z s (1 - s) 2 u'
+    z = within_pair(z, kGeluMost);
     const uint64_t z2 = ptx::mul_f32x2(z, z);
     const uint64_t u = ptx::fma_f32x2(z2, two(-2.0f * kGeluC * kGeluA * kLog2e), two(-2.0f * kGeluC * kLog2e));
     const uint64_t s = sigmoid2_pair(ptx::mul_f32x2(z, u));
@@ -147,6 +165,7 @@ __device__ __forceinline__ uint64_t slope_pair(uint64_t z) {
     return ptx::fma_f32x2(ptx::mul_f32x2(s, rest), ptx::mul_f32x2(z, du), s);
   }
   if constexpr (ACT == TVB_ACT_SILU) {
+    z = within_pair(z, kSiluMost);
     const uint64_t s = sigmoid2_pair(ptx::mul_f32x2(z, two(-kLog2e)));
     const uint64_t rest = ptx::fma_f32x2(s, two(-1.0f), two(1.0f));
     return ptx::fma_f32x2(ptx::mul_f32x2(s, rest), z, s);
