@@ -1009,11 +1009,16 @@ extern "C" int tvb_layer_norm(int device, const void* x, int dtype, int64_t x_sm
   TVB_REQUIRE(rows <= 1 || x_sm >= d, "tvb_layer_norm: rows of x must be at least d apart");
   if (rows == 0 || d == 0) return 0;
   TVB_REQUIRE(x != nullptr && y != nullptr, "tvb_layer_norm: NULL pointer");
-  const int64_t es = dtype_size(dtype), x_bytes = ((rows - 1) * x_sm + d) * es, y_bytes = rows * d * es;
-  TVB_REQUIRE(!overlap(y, y_bytes, x, x_bytes) && !overlap(mean, rows * 4, x, x_bytes) && !overlap(rstd, rows * 4, x, x_bytes) &&
-                  !overlap(mean, rows * 4, y, y_bytes) && !overlap(rstd, rows * 4, y, y_bytes) && !overlap(mean, rows * 4, rstd, rows * 4) &&
-                  !overlap(y, y_bytes, weight, d * dtype_size(param_dtype)) && !overlap(y, y_bytes, bias, d * dtype_size(param_dtype)),
-              "tvb_layer_norm: an output overlaps another operand");
+  const int64_t es = dtype_size(dtype), x_bytes = ((rows - 1) * x_sm + d) * es, p_bytes = d * dtype_size(param_dtype);
+  const void* outs[3] = {y, mean, rstd};
+  const int64_t out_bytes[3] = {rows * d * es, rows * 4, rows * 4};
+  for (int i = 0; i < 3; i++) {
+    TVB_REQUIRE(!overlap(outs[i], out_bytes[i], x, x_bytes) && !overlap(outs[i], out_bytes[i], weight, p_bytes) &&
+                    !overlap(outs[i], out_bytes[i], bias, p_bytes),
+                "tvb_layer_norm: an output overlaps an operand");
+    for (int j = 0; j < i; j++)
+      TVB_REQUIRE(!overlap(outs[i], out_bytes[i], outs[j], out_bytes[j]), "tvb_layer_norm: one output overlaps another");
+  }
   cudaStream_t stream;
   if (enter_on(device, caller_stream, &stream) != 0) return -1;
   NormParams p{};
