@@ -403,7 +403,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _native.layer_norm(x, weight, bias, eps)
 
 
-def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True)):
+def layer_norm_backward(dy, x, mean, rstd, weight=None, need=(True, True, True), param_dtype=None):
     """tvb_layer_norm_backward on device tensors: (dx, dweight, dbias), None where `need` is false; mean and rstd [rows] as
-    layer_norm returned them. dweight and dbias have weight's dtype (x's without a weight)."""
-    return _native.layer_norm_backward(dy, x, mean, rstd, weight, need[0], need[1], need[2])
+    layer_norm returned them. dweight and dbias have weight's dtype (without a weight: param_dtype, x's or float32)."""
+    return _native.layer_norm_backward(dy, x, mean, rstd, weight, need[0], need[1], need[2], param_dtype)

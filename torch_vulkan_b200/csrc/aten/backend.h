@@ -55,7 +55,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor& x, c
                                                           const std::optional<at::Tensor>& bias, double eps);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& mean,
                                                                    const at::Tensor& rstd, const std::optional<at::Tensor>& weight,
-                                                                   bool need_x, bool need_weight, bool need_bias);
+                                                                   bool need_x, bool need_weight, bool need_bias,
+                                                                   std::optional<at::ScalarType> param_type);
 
 void register_backend();
 void shutdown_backend();

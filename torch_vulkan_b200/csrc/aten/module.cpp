@@ -80,6 +80,13 @@ PYBIND11_MODULE(_native, m) {
   m.def("linear_act", &vkb::linear_act, py::call_guard<py::gil_scoped_release>());
   m.def("linear_act_backward", &vkb::linear_act_backward, py::call_guard<py::gil_scoped_release>());
   m.def("layer_norm", &vkb::layer_norm, py::call_guard<py::gil_scoped_release>());
-  m.def("layer_norm_backward", &vkb::layer_norm_backward, py::call_guard<py::gil_scoped_release>());
+  m.def(
+      "layer_norm_backward",
+      [](const at::Tensor& dy, const at::Tensor& x, const at::Tensor& mean, const at::Tensor& rstd, const std::optional<at::Tensor>& weight,
+         bool need_x, bool need_weight, bool need_bias, std::optional<at::ScalarType> param_type) {
+        return vkb::layer_norm_backward(dy, x, mean, rstd, weight, need_x, need_weight, need_bias, param_type);
+      },
+      py::arg("dy"), py::arg("x"), py::arg("mean"), py::arg("rstd"), py::arg("weight"), py::arg("need_x"), py::arg("need_weight"),
+      py::arg("need_bias"), py::arg("param_type") = py::none(), py::call_guard<py::gil_scoped_release>());
   m.def("shutdown", &vkb::shutdown_backend);
 }

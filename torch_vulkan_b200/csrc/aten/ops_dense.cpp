@@ -144,18 +144,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor& x, c
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& mean,
                                                                    const at::Tensor& rstd, const std::optional<at::Tensor>& weight,
-                                                                   bool need_x, bool need_weight, bool need_bias) {
+                                                                   bool need_x, bool need_weight, bool need_bias,
+                                                                   std::optional<at::ScalarType> param_type) {
   const char* fn = "layer_norm_backward";
   const int code = float_code(fn, x);
   TORCH_CHECK_VALUE(x.dim() == 2, fn, ": x [rows, d] expected");
   const int64_t rows = x.size(0), d = x.size(1), x_sm = matrix(fn, "x", x, rows, d, x), dy_sm = matrix(fn, "dy", dy, rows, d, x);
-  const int pcode = param_code(fn, x, d, weight, std::nullopt);
+  // without a weight the gradients of the parameters are of param_type (the bias's), or of x's
+  const at::ScalarType ptype = weight.has_value() ? weight->scalar_type() : param_type.value_or(x.scalar_type());
+  const int pcode = weight.has_value() ? param_code(fn, x, d, weight, std::nullopt) : dtype_code(ptype);
+  TORCH_CHECK_VALUE(ptype == x.scalar_type() || ptype == at::kFloat, fn, ": parameters must be of ", x.scalar_type(), " or float32, got ", ptype);
   for (const at::Tensor* t : {&mean, &rstd})
     TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == rows && t->device() == x.device() && t->is_contiguous() && t->scalar_type() == at::kFloat,
                       fn, ": mean and rstd must be contiguous float32 vectors of ", rows, " values on ", x.device());
   check_device(fn, x);
   Where at(x);
-  const at::TensorOptions params = weight.has_value() ? weight->options() : x.options();
+  const at::TensorOptions params = x.options().dtype(ptype);
   at::Tensor dx = optional_empty(need_x, {rows, d}, x.options());
   at::Tensor dw = optional_empty(need_weight, {d}, params), db = optional_empty(need_bias, {d}, params);
   const uint64_t bytes = need_weight || need_bias ? tvb_layer_norm_backward_workspace_bytes(rows, d) : 0;
@@ -230,9 +234,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> native_layer_norm_backward(const 
   const NormShape s = norm_shape(input, normalized_shape, weight, bias);
   const std::optional<at::Tensor> go = grad_out, in = input, me = mean, rs = rstd;
   require_all_vk("aten::native_layer_norm_backward", {&go, &in, &me, &rs, &weight, &bias});
-  std::optional<at::Tensor> w = flat(weight);
+  const std::optional<at::Tensor> w = flat(weight);
+  const bool has_bias = bias.has_value() && bias->defined();
   auto [dx, dw, db] = layer_norm_backward(as_rows(grad_out, s), as_rows(input, s), mean.contiguous().view({s.rows}),
-                                          rstd.contiguous().view({s.rows}), w, mask[0], mask[1], mask[2]);
+                                          rstd.contiguous().view({s.rows}), w, mask[0], mask[1], mask[2],
+                                          has_bias ? std::optional<at::ScalarType>(bias->scalar_type()) : std::nullopt);
   if (dx.defined()) dx = dx.view(input.sizes());
   if (dw.defined()) dw = dw.view(normalized_shape);
   if (db.defined()) db = db.view(normalized_shape);
