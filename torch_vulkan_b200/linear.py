@@ -190,6 +190,12 @@ def _apply(x, w, bias, residual, activation, keep):
     return y if keep else (y, None)
 
 
+def _shaped(y, lead):
+    """y [rows, n] in the caller's shape, as a tensor of its own: a view (of a custom function's output, or made while gradients
+    are off) could not be written to in place afterwards, as an nn.Linear's output can."""
+    return y if len(lead) == 1 else torch.ops.aten._unsafe_view(y, (*lead, y.shape[1]))
+
+
 class _LinearAct(torch.autograd.Function):
     """cabi.linear and cabi.linear_backward as one differentiable operation. Keeps x, the weight and, with an activation, the
     values before it."""
@@ -200,7 +206,7 @@ class _LinearAct(torch.autograd.Function):
         y, z = _apply(x2, w2, bias, residual, activation, activation != "none" and any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x2, w2, z)
         ctx.activation, ctx.x_shape = activation, x.shape
-        return y.view(*x.shape[:-1], weight.shape[0])
+        return _shaped(y, x.shape[:-1])
 
     @staticmethod
     @once_differentiable
@@ -239,7 +245,7 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return _LinearAct.apply(x, weight, bias, residual, activation)
     k = weight.shape[1]
-    return _apply(_rows(x, k), _rows(weight, k), bias, residual, activation, False)[0].view(*x.shape[:-1], weight.shape[0])
+    return _shaped(_apply(_rows(x, k), _rows(weight, k), bias, residual, activation, False)[0], x.shape[:-1])
 
 
 class LinearAct(nn.Linear):
