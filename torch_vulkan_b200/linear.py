@@ -218,7 +218,8 @@ class _LinearAct(torch.autograd.Function):
         dx = dw = db = None
         if any(need):
             dx, dw, db = cabi.linear_backward(_rows(dy, w2.shape[0]), x2, w2, z, activation=ctx.activation, need=need)
-        return (None if dx is None else dx.view(ctx.x_shape)), dw, db, (dy if ctx.needs_input_grad[3] else None), None
+        # (contiguous, so that it can be added to other gradients of the same tensor: x may be its own residual)
+        return (None if dx is None else dx.view(ctx.x_shape)), dw, db, (dy.contiguous() if ctx.needs_input_grad[3] else None), None
 
 
 def linear_act(x, weight, bias=None, activation="none", residual=None):
