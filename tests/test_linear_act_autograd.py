@@ -60,3 +60,48 @@ def test_an_input_that_is_its_own_residual(how, dtype, rel):
     (F.gelu(cx @ cw.t()) + cx).backward(dy.double())
     near(vx.grad, cx.grad, rel)
     near(vw.grad, cw.grad, rel)
+
+
+@pytest.mark.parametrize("act", D.ACTS)
+def test_a_fused_model_on_the_meta_device(act):
+    layer = L.LinearAct(12, 20, activation=act, device="meta")
+    x = torch.empty(3, 5, 12, device="meta", requires_grad=True)
+    y = layer(x, residual=torch.empty(3, 5, 20, device="meta"))
+    assert y.device.type == "meta" and y.shape == (3, 5, 20)
+    y.backward(torch.empty_like(y))
+    assert x.grad.shape == x.shape and layer.weight.grad.shape == (20, 12)
+
+
+@gpu
+@pytest.mark.parametrize("act", D.ACTS)
+def test_cuda_tensors_in_float64_and_under_autocast(act):
+    torch.manual_seed(1)
+    layer = L.LinearAct(40, 24, activation=act)
+    x = torch.randn(7, 40)
+    want = layer.double()(x.double())
+    layer = layer.cuda()
+    with torch.no_grad():
+        got = layer(x.double().cuda())
+        assert got.dtype == torch.float64
+        near(got, want.detach(), 2.0 ** -45)
+        layer = layer.float()
+        with torch.autocast("cuda", torch.bfloat16):
+            got, plain = layer(x.cuda()), F.linear(x.cuda(), layer.weight, layer.bias)
+        assert plain.dtype == torch.bfloat16 and got.dtype in (torch.bfloat16, torch.float32)
+        near(got, want.detach(), 2.0 ** -6)
+
+
+@gpu
+def test_cuda_tensors_that_require_gradients_run_forward_and_refuse_backward():
+    x = torch.randn(7, 40, generator=D.gen(1)).cuda().requires_grad_(True)
+    w = torch.randn(24, 40, generator=D.gen(2)).cuda().requires_grad_(True)
+    y = L.linear_act(x, w, None, "gelu")
+    with torch.no_grad():
+        assert torch.equal(y, L.linear_act(x, w, None, "gelu"))
+    assert y.requires_grad and y.grad_fn.saved_tensors == ()  # (nothing is kept for a pass that cannot be run)
+    with pytest.raises(RuntimeError):
+        y.backward(torch.ones_like(y))
+    assert x.grad is None and w.grad is None
+    vx = x.detach().cpu().to("vk").requires_grad_(True)  # the device's own gradients go on
+    L.linear_act(vx, w.detach().cpu().to("vk"), None, "gelu").backward(torch.ones(7, 24).to("vk"))
+    assert vx.grad.shape == vx.shape

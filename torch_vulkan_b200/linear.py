@@ -203,8 +203,10 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
         x2, w2 = _rows(x, weight.shape[1]), _rows(weight, weight.shape[1])
-        y, z = _apply(x2, w2, bias, residual, activation, activation != "none" and any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x2, w2, z)
+        ctx.on_vk = x.device.type == "vk"
+        y, z = _apply(x2, w2, bias, residual, activation, ctx.on_vk and activation != "none" and any(ctx.needs_input_grad[:3]))
+        if ctx.on_vk:
+            ctx.save_for_backward(x2, w2, z)
         ctx.activation, ctx.x_shape = activation, x.shape
         return _shaped(y, x.shape[:-1])
 
@@ -213,6 +215,9 @@ class _LinearAct(torch.autograd.Function):
     def backward(ctx, dy):
         from . import cabi
 
+        if not ctx.on_vk:
+            raise NotImplementedError("no gradients through CUDA tensors (PyTorch's autograd engine serves device \"vk\" in this "
+                                      "process): call cabi.linear_backward")
         x2, w2, z = ctx.saved_tensors
         need = ctx.needs_input_grad[:3]
         dx = dw = db = None
@@ -222,12 +227,20 @@ class _LinearAct(torch.autograd.Function):
         return (None if dx is None else dx.view(ctx.x_shape)), dw, db, (dy.contiguous() if ctx.needs_input_grad[3] else None), None
 
 
+def _has_kernel(x):
+    """Whether the fused kernel serves x: on "vk" always (it refuses what it cannot do), of CUDA tensors those of its types where
+    autocast asks for no other."""
+    return x.device.type == "vk" or (x.device.type == "cuda" and x.dtype in (torch.float32, torch.float16, torch.bfloat16)
+                                     and not torch.is_autocast_enabled("cuda"))
+
+
 def linear_act(x, weight, bias=None, activation="none", residual=None):
     """act(x @ weight.T + bias) + residual: x [..., in], weight [out, in], bias [out], residual [..., out], all of one dtype
     (float32, float16 or bfloat16). activation: "none", "relu", "gelu" (by erf), "gelu_tanh" or "silu". Differentiable (once)
-    in every operand. On "vk" one kernel computes it (tvb_linear; the gradients: tvb_linear_backward); on the CPU PyTorch's own
-    operations do. CUDA tensors take the kernel too, without gradients: PyTorch's autograd engine serves one accelerator per
-    process, and here that is "vk" (cabi.linear_backward computes them when called)."""
+    in every operand. On "vk" one kernel computes it (tvb_linear; the gradients: tvb_linear_backward). CUDA tensors of those types
+    take the kernel too, without gradients: PyTorch's autograd engine serves one accelerator per process, and here that is
+    "vk" (a backward pass through them raises, as through any CUDA tensor; cabi.linear_backward computes them when called).
+    Anything else that an nn.Linear runs on (the CPU, the meta device, float64, autocast on CUDA) takes PyTorch's own operations."""
     from . import cabi
 
     if activation not in cabi.ACTIVATIONS:
@@ -236,7 +249,7 @@ def linear_act(x, weight, bias=None, activation="none", residual=None):
         raise ValueError(f"x of shape {tuple(x.shape)} does not go with a weight of shape {tuple(weight.shape)}")
     if residual is not None and residual.shape != (*x.shape[:-1], weight.shape[0]):
         raise ValueError(f"residual of shape {tuple(residual.shape)} for an output of shape {(*x.shape[:-1], weight.shape[0])}")
-    if x.device.type == "cpu":
+    if not _has_kernel(x):
         y = F.linear(x, weight, bias)
         y = {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"),
              "silu": F.silu}[activation](y)
