@@ -105,3 +105,54 @@ def test_cuda_tensors_that_require_gradients_run_forward_and_refuse_backward():
     vx = x.detach().cpu().to("vk").requires_grad_(True)  # the device's own gradients go on
     L.linear_act(vx, w.detach().cpu().to("vk"), None, "gelu").backward(torch.ones(7, 24).to("vk"))
     assert vx.grad.shape == vx.shape
+
+
+class TwoBlocks(nn.Module):
+    """Linears in every place that fuse_linears has to find: before an activation, alone, in a ModuleDict, one in two places."""
+
+    def __init__(self, d=64, h=160, seed=3):
+        super().__init__()
+        torch.manual_seed(seed)
+        self.ffn = nn.Sequential(nn.LayerNorm(d), nn.Linear(d, h), nn.GELU(), nn.Linear(h, d))
+        self.rest = nn.ModuleDict({"gate": nn.Linear(d, h, bias=False), "down": nn.Linear(h, d)})
+        self.tied = self.rest["down"]
+
+    def forward(self, x):
+        h = self.rest["gate"](self.ffn(x))
+        return self.rest["down"](h) + self.tied(h)
+
+
+def test_fuse_linears_with_the_plain_ones():
+    a, b = TwoBlocks(), TwoBlocks()
+    kept = b.rest["gate"].register_forward_hook(lambda module, args, out: out)
+    assert L.fuse_linears(b, plain=True) == ["ffn.1", "tied", "ffn.3", "rest.down"]
+    assert type(b.rest["gate"]) is nn.Linear  # (hooked)
+    kept.remove()
+    assert L.fuse_linears(b, plain=True) == ["rest.gate"]
+    assert all(type(m) is L.LinearAct for m in b.modules() if isinstance(m, nn.Linear)) and b.tied is b.rest["down"]
+    assert b.ffn[1].activation == "gelu" and b.ffn[3].activation == "none"
+    assert list(a.state_dict()) == list(b.state_dict())
+    x = torch.randn(5, 64, generator=D.gen(1))
+    assert torch.equal(a(x), b(x))
+    assert L.fuse_linears(TwoBlocks()) == ["ffn.1"]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,rel", [(torch.float32, 2.0 ** -17), (torch.bfloat16, 2.0 ** -5)])
+def test_a_fused_model_trains_on_vk(dtype, rel):
+    """One step's gradients of every parameter against 64 bits (16 bits: some ten roundings between the output and the first
+    layer, half a step each)."""
+    model, twin = TwoBlocks().to(dtype), TwoBlocks().to(dtype).double()
+    L.fuse_linears(model, plain=True)
+    model = model.to("vk")
+    x, dy = (torch.randn(3, 17, 64, generator=D.gen(i)).to(dtype) for i in (1, 2))
+    vx, cx = x.to("vk").requires_grad_(True), x.double().requires_grad_(True)
+    y = model(vx)
+    y.backward(dy.to("vk"))
+    want = twin(cx)
+    want.backward(dy.double())
+    near(y, want.detach(), rel)
+    near(vx.grad, cx.grad, rel)
+    names = dict(twin.named_parameters())
+    for name, p in model.named_parameters():
+        near(p.grad, names[name].grad, rel)

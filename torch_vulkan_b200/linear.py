@@ -300,11 +300,13 @@ def _hooked(module):
     return any(getattr(module, kind) for kind in ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
 
 
-def fuse_linears(model):
+def fuse_linears(model, plain=False):
     """Replaces, in every nn.Sequential under `model` (in place), an nn.Linear that is followed by ReLU, GELU or SiLU with one
     LinearAct that shares its parameters, and the activation with nn.Identity (so that the other layers keep their names).
-    Left as they are: layers with hooks (a fused one would not run them), and containers with a forward pass of their own.
-    Returns the names of the layers it replaced."""
+    plain: every other nn.Linear under `model`, whatever it stands in, becomes a LinearAct without an activation too. A model that
+    trains on "vk" needs that: an nn.Linear's own backward pass asks for the sum of its bias's gradient, which has no kernel there.
+    Left as they are: layers with hooks (a fused one would not run them), and containers with a forward pass of their own (but for
+    `plain`). Returns the names of the layers it replaced."""
     replaced = []
     for name, module in list(model.named_modules()):
         if not isinstance(module, nn.Sequential) or type(module).forward is not nn.Sequential.forward:
@@ -317,6 +319,15 @@ def fuse_linears(model):
             setattr(module, first, LinearAct.from_float(linear, activation))
             setattr(module, second, nn.Identity())
             replaced.append(f"{name}.{first}" if name else first)
+    made = {}  # (a layer that stands in two places stays one)
+    for name, module in list(model.named_modules()) if plain else []:
+        for key, child in list(module._modules.items()):
+            if type(child) is not nn.Linear or _hooked(child):
+                continue
+            if child not in made:
+                made[child] = LinearAct.from_float(child)
+            setattr(module, key, made[child])
+            replaced.append(f"{name}.{key}" if name else key)
     return replaced
 
 
