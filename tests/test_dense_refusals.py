@@ -14,3 +14,16 @@ def test_layer_norm_refuses_statistics_over_its_parameters(place, param):
     at = {"y": Y, "mean": MEAN, "rstd": RSTD, **place}
     rc = cabi.lib().tvb_layer_norm(0, X, cabi.BF16, 64, W, B, param, 1e-5, at["y"], at["mean"], at["rstd"], 4, 64, None)
     assert rc == -1 and "overlaps" in cabi.lib().tvb_last_error().decode()
+
+
+def test_the_extension_does_not_need_a_cuda_build_of_pytorch():
+    """The backend has a runtime of its own: none of PyTorch's CUDA libraries is among those that its extension asks for."""
+    import subprocess
+
+    from torch_vulkan_b200 import _build
+
+    table = subprocess.run(["readelf", "-d", _build.native_path()], capture_output=True, text=True)
+    if table.returncode != 0:
+        pytest.skip("no readelf here")
+    needed = [line for line in table.stdout.splitlines() if "NEEDED" in line]
+    assert any("libtorch_cpu" in line for line in needed) and not any("cuda" in line for line in needed), needed

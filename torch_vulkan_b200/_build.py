@@ -99,7 +99,6 @@ def build_native(verbose=False):
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cflags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_native",
               "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-Wno-deprecated-declarations"]
-    includes.append(os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include"))  # (c10/cuda/CUDAStream.h needs cuda_runtime_api.h)
     for inc in includes:
         cflags += ["-isystem", inc]
     objects, jobs = [], []
@@ -120,7 +119,7 @@ def build_native(verbose=False):
                 raise RuntimeError("g++ failed for " + cmd[-3])
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = ["g++", "-shared", "-o", out] + objects + [
-        "-L", torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python",
+        "-L", torch_lib, "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python",
         "-L", os.path.dirname(LIB), "-ltvb200", "-Wl,-rpath,$ORIGIN/lib", "-Wl,-rpath," + torch_lib]
     subprocess.check_call(cmd)
     return out

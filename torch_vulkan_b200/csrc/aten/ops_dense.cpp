@@ -5,7 +5,7 @@
 // outputs and workspaces from torch's allocator, so that they behave like any CUDA op). The reference dispatches these
 // layers as separate matrix, elementwise and reduction kernels (crates/pyvk/csrc/linalg.cpp:227-321).
 #include <c10/core/DeviceGuard.h>
-#include <c10/cuda/CUDAStream.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/library.h>
 
 #include "backend.h"
@@ -16,8 +16,8 @@ namespace {
 // Where a call runs: the operands' device made current for its duration, and the stream for the C ABI.
 struct Where {
   explicit Where(const at::Tensor& t) : guard(t.device()), device(t.device().index()) {
-    if (t.is_cuda()) {
-      stream = c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+    if (t.is_cuda()) {  // (asked through the device-independent interface: the extension needs no CUDA build of PyTorch to load)
+      stream = c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getStream(t.device()).native_handle();
       if (stream == nullptr) stream = reinterpret_cast<void*>(uintptr_t(1));  // cudaStreamLegacy: NULL means the backend's own
     }
   }
