@@ -8,9 +8,8 @@
 // fill a round of pairs are cut into smaller ones (256 rows, 256 or 128 columns).
 // Outputs leave through shared memory and TMA stores (a thread of the epilogue holds a row's 64 columns; stored from
 // registers they are 32 scattered pieces per instruction, and the read-back took four times as long).
-// A launch takes one product or two: the backward pass multiplies dz by w and by x at once. The tiles of the product with the
-// longer r come first; pairs that get one tile of it less than others start on the second product meanwhile, and the rest of its
-// tiles are dealt out in turn. The schedule is computed from the sizes alone (no counters in memory), so launches share nothing.
+// A launch takes one product or two (256-row tiles): the backward pass multiplies dz by w and by x at once. Who makes which tile, and
+// when, stands in linear_schedule.h.
 //
 // Measured (us per call, seconds-long runs, in which the GPU is held at its power limit): 2048 x 4096 x 14336 bfloat16 with gelu and its
 // input saved 213 (1.13 PFLOP/s; the product alone 195); its gradients 434, of which the pass over dz takes 40 and both products
@@ -26,21 +25,20 @@
 #include "launch.h"
 #include "linear.h"
 #include "linear_epilogue.cuh"
+#include "linear_schedule.h"
 #include "ptx_pair.cuh"
 
 namespace tvb {
 namespace {
 
-constexpr int kHalfJ = 256, kTileI = 256, kRowsQ = 128, kStepR = 64;
+constexpr int kRowsQ = 128, kStepR = 64;
 constexpr int kBoxQ = kRowsQ * 128;  // bytes of one half's rows of Q in a stage
 // HALVES: 2 for tiles of 512 rows, 1 for tiles of 256.
 template <int HALVES>
 struct PairCfg {
-  static constexpr int kTileJ = HALVES * kHalfJ;
   static constexpr int kP = HALVES * kBoxQ;  // where P begins in a stage
   static constexpr int kStage = kP + 128 * 128;
   static constexpr int kStages = HALVES == 2 ? 4 : 6;
-  static constexpr int kBand = 16 / HALVES;  // tile rows per band of the tile order
 };
 constexpr int kRing = 192 * 1024;
 static_assert(PairCfg<1>::kStages * PairCfg<1>::kStage == kRing && PairCfg<2>::kStages * PairCfg<2>::kStage == kRing, "the ring's size");
@@ -56,91 +54,15 @@ struct PairProduct {
   void* out;
   void* preact;
   int64_t residual_ld;
-  int I, J, blocks, tiles, tiles_i, tiles_j, q_mn, p_mn, activation, vector_ok, alone;
+  PairExtent extent;
+  int q_mn, p_mn, activation, vector_ok, alone;
   uint32_t fmt;  // instruction descriptor without the columns
 };
 
-// Product 0 may be empty (tiles == 0): a launch of one product has it as product 1.
 struct PairParams {
   PairProduct prod[2];
-  int extra;        // tiles of product 1 that a pair with fewer tiles of product 0 takes first
-  int light_first;  // which pairs come first when the rest of product 1 is dealt out
-  int whole;        // tiles of product 1 that are not cut; the others become cut tiles of 256 rows x cut_cols columns
-  int cut_cols;
+  PairPlan plan;
   int* status;
-};
-
-struct PairTile {
-  int product, row, col, cols, halves;
-};
-
-// Walks the tiles of one pair: its tiles of product 0, its share of product 1, its share of what was cut.
-template <int HALVES>
-struct PairSchedule {
-  using Cfg = PairCfg<HALVES>;
-  int pair, pairs, at, heavy, rank_among, order, stage;
-  bool is_light;
-  __device__ PairSchedule(const PairParams& p, int pair_, int pairs_) : pair(pair_), pairs(pairs_) {
-    heavy = p.prod[0].tiles % pairs;  // pairs 0 ... heavy - 1 have one tile of product 0 more than the others
-    is_light = heavy != 0 && pair >= heavy;
-    rank_among = is_light ? pair - heavy : pair;
-    order = heavy != 0 && p.light_first ? (is_light ? rank_among : pairs - heavy + pair) : pair;
-    stage = 0;
-    at = pair;
-  }
-  __device__ static void place(const PairProduct& d, int index, PairTile& t) {
-    const int per_band = Cfg::kBand * d.tiles_i, b = index / per_band, first = b * Cfg::kBand;
-    const int rows = d.tiles_j - first < Cfg::kBand ? d.tiles_j - first : Cfg::kBand;
-    const int r = index - b * per_band;
-    t.row = (first + r % rows) * Cfg::kTileJ;
-    t.col = r / rows * kTileI;
-    t.cols = kTileI;
-    t.halves = HALVES == 2 && t.row + kHalfJ < d.J ? 2 : 1;
-  }
-  __device__ bool next(const PairParams& p, PairTile& t) {
-    const int light = heavy != 0 ? pairs - heavy : 0, early = light * p.extra;
-    for (;;) {
-      if (stage == 0) {
-        if (at < p.prod[0].tiles) {
-          t.product = 0;
-          place(p.prod[0], at, t);
-          at += pairs;
-          return true;
-        }
-        stage = 1;
-        at = rank_among;
-      }
-      t.product = 1;
-      if (stage == 1) {
-        if (is_light && at < early && at < p.whole) {
-          place(p.prod[1], at, t);
-          at += light;
-          return true;
-        }
-        stage = 2;
-        at = early + order;
-      }
-      if (stage == 2) {
-        if (at < p.whole) {
-          place(p.prod[1], at, t);
-          at += pairs;
-          return true;
-        }
-        stage = 3;
-        at = order;
-      }
-      const int per_half = kTileI / p.cut_cols, per_tile = HALVES * per_half;
-      const int index = p.whole + at / per_tile, sub = at % per_tile;
-      if (index >= p.prod[1].tiles) return false;
-      at += pairs;
-      place(p.prod[1], index, t);
-      t.row += sub / per_half * kHalfJ;
-      t.col += sub % per_half * p.cut_cols;
-      t.cols = p.cut_cols;
-      t.halves = 1;
-      if (t.row < p.prod[1].J && t.col < p.prod[1].I) return true;  // (a cut tile may lie outside altogether)
-    }
-  }
 };
 
 __device__ __forceinline__ void fetch32(const void* base, int64_t at, uint4 (&x)[4]) {
@@ -201,13 +123,13 @@ __device__ __forceinline__ void wait_tile(int lane) {
 template <bool BF16>
 __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, uint32_t tile, int lane, int row0, int i) {
   uint32_t y[2][16];
-  const bool live = row0 + lane < d.J;
+  const bool live = row0 + lane < d.extent.J;
 #pragma unroll
   for (int q = 0; q < 2; q++) {
     uint32_t w[16];
     uint64_t v[16];
     const int at = i + 32 * q;
-    const bool inside = at + 32 <= d.I;  // (else the row's last columns: fewer than 32, a multiple of 8)
+    const bool inside = at + 32 <= d.extent.I;  // (else the row's last columns: fewer than 32, a multiple of 8)
     const int64_t r = static_cast<int64_t>(row0 + lane) * d.residual_ld + at;
     uint4 bias[4], residual[4];  // (on their way while the TMEM is read)
     if (d.bias != nullptr && inside) fetch32(d.bias, at, bias);
@@ -215,7 +137,7 @@ __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, u
     load32(taddr + 32 * q, v);
     if (d.bias != nullptr) {
       if (inside) add32<BF16>(bias, v);
-      else add_singly<BF16>(d.bias, at, d.I - at, v);
+      else add_singly<BF16>(d.bias, at, d.extent.I - at, v);
     }
     if (d.preact != nullptr) {
       pack32<BF16>(v, w);
@@ -225,7 +147,7 @@ __device__ __forceinline__ void finish64(const PairProduct& d, uint32_t taddr, u
     activate_pairs(v, d.activation);
     if (d.residual != nullptr && live) {
       if (inside) add32<BF16>(residual, v);
-      else add_singly<BF16>(d.residual, r, d.I - at, v);
+      else add_singly<BF16>(d.residual, r, d.extent.I - at, v);
     }
     pack32<BF16>(v, y[q]);
   }
@@ -259,9 +181,9 @@ template <bool BF16>
 __device__ __forceinline__ void finish32(const PairProduct& d, uint32_t taddr, int64_t j, int i) {
   uint64_t v[16];
   load32(taddr, v);
-  if (j >= d.J || i >= d.I) return;
-  const int count = d.I - i;
-  const int64_t o = j * d.I + i;
+  if (j >= d.extent.J || i >= d.extent.I) return;
+  const int count = d.extent.I - i;
+  const int64_t o = j * d.extent.I + i;
   if (d.bias != nullptr) add_singly<BF16>(d.bias, i, count, v);
   if (d.preact != nullptr) store_singly<BF16>(d.preact, o, count, v);
   activate_pairs(v, d.activation);
@@ -292,7 +214,7 @@ __device__ __forceinline__ bool load_tile(const PairProduct& d, const PairTile& 
   const int row_q = t.row + static_cast<int>(rank) * kRowsQ, row_p = t.col + static_cast<int>(rank) * (t.cols >> 1);
   const bool two = HALVES == 2 && t.halves == 2, wide = t.cols == kTileI;
   const uint32_t bytes = 2u * ((two ? 2 : 1) * kBoxQ + (wide ? 2 : 1) * 8192);
-  const int blocks = d.blocks;
+  const int blocks = d.extent.blocks;
   int r = 0;
 #pragma unroll 1
   for (int kb = 0; kb < blocks; kb++, r += kStepR, at.step()) {
@@ -331,7 +253,7 @@ __device__ __forceinline__ bool multiply_tile(const PairProduct& d, const PairTi
   const uint64_t q0 = Q_MN ? ptx::tc_smem_desc_sw128_mn(base) : ptx::tc_smem_desc_sw128(base);
   const uint64_t p0 = P_MN ? ptx::tc_smem_desc_sw128_mn(base + kPAt) : ptx::tc_smem_desc_sw128(base + kPAt);
   const bool two = HALVES == 2 && t.halves == 2;
-  const int blocks = d.blocks;
+  const int blocks = d.extent.blocks;
   uint32_t more = 0;  // (the first instruction of a tile overwrites the sums)
 #pragma unroll 1
   for (int kb = 0; kb < blocks; kb++, at.step()) {
@@ -384,14 +306,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
 
-  PairSchedule<HALVES> sched(p, pair, pairs);
+  PairSchedule<HALVES> sched(p.plan, p.prod[0].extent, pair, pairs);
   PairTile t;
   if (warp == kProducer) {
     if (lane == 0) {
       RingAt<kStages> at;
       const uint32_t bar0 = ptx::mapa(full0, 0);  // the leader's barriers, from either CTA
       bool ok = true;
-      while (ok && sched.next(p, t)) {
+      while (ok && sched.next(p.plan, p.prod[0].extent, p.prod[1].extent, t)) {
         const PairProduct& d = p.prod[t.product];
         ok = d.q_mn   ? load_tile<HALVES, true, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
              : d.p_mn ? load_tile<HALVES, false, true>(d, t, rank, at, base, full0, empty0, bar0, abort_flag)
@@ -412,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
       uint32_t used0 = 0, used1 = 0;  // tiles (or halves) that each buffer of sums has held
       int turn = 0;
       bool ok = true;
-      while (ok && sched.next(p, t)) {
+      while (ok && sched.next(p.plan, p.prod[0].extent, p.prod[1].extent, t)) {
         const PairProduct& d = p.prod[t.product];
         const bool both = t.halves == 2;
         const int buffer = both ? 0 : turn;  // (a single half takes the buffers in turn)
@@ -439,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
     uint32_t used0 = 0, used1 = 0;
     int turn = 0;
     bool ok = true;
-    while (ok && sched.next(p, t)) {
+    while (ok && sched.next(p.plan, p.prod[0].extent, p.prod[1].extent, t)) {
       const PairProduct& d = p.prod[t.product];
       for (int h = 0; h < t.halves; h++) {
         const int b = t.halves == 2 ? h : turn;
@@ -453,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
         const uint32_t tile = base + kRing + warp * kOut;
 #pragma unroll 1
         for (int c = (warp >> 2) * 64; c < t.cols; c += 128) {
-          if (row0 >= d.J || t.col + c >= d.I) break;  // (nothing of it is inside)
+          if (row0 >= d.extent.J || t.col + c >= d.extent.I) break;  // (nothing of it is inside)
           if (d.alone) {
             store64<BF16>(d, taddr + c, tile, lane, row0, t.col + c);
           } else if (d.vector_ok) {
@@ -526,13 +448,14 @@ int pair_product(const LinearProduct& lp, PairProduct* d) {
   d->out = lp.out;
   d->preact = lp.preact;
   d->residual_ld = lp.residual_ld;
-  d->I = static_cast<int>(lp.I);
-  d->J = static_cast<int>(lp.J);
-  d->blocks = static_cast<int>(ceil_div(lp.R, kStepR));
-  d->tiles_i = static_cast<int>(ceil_div(lp.I, kTileI));
-  d->tiles_j = static_cast<int>(ceil_div(lp.J, PairCfg<HALVES>::kTileJ));
-  TVB_REQUIRE(static_cast<int64_t>(d->tiles_i) * d->tiles_j < (int64_t(1) << 28), "tvb_linear: too many output tiles");
-  d->tiles = d->tiles_i * d->tiles_j;
+  PairExtent& e = d->extent;
+  e.I = static_cast<int>(lp.I);
+  e.J = static_cast<int>(lp.J);
+  e.blocks = static_cast<int>(ceil_div(lp.R, kStepR));
+  e.tiles_i = static_cast<int>(ceil_div(lp.I, kTileI));
+  e.tiles_j = static_cast<int>(ceil_div(lp.J, PairSchedule<HALVES>::kTileJ));
+  TVB_REQUIRE(static_cast<int64_t>(e.tiles_i) * e.tiles_j < (int64_t(1) << 28), "tvb_linear: too many output tiles");
+  e.tiles = e.tiles_i * e.tiles_j;
   d->q_mn = lp.q_mn;
   d->p_mn = lp.p_mn;
   d->activation = lp.activation;
@@ -559,27 +482,8 @@ int pair_run(int device, cudaStream_t stream, const LinearProduct* lp, int count
   const bool swap = count == 2 && lp[0].R < lp[1].R;  // the longer r first
   if (count == 2 && pair_product<HALVES>(lp[swap ? 1 : 0], &p.prod[0]) != 0) return -1;
   if (pair_product<HALVES>(lp[count == 2 && !swap ? 1 : 0], &p.prod[1]) != 0) return -1;
-  int light = 0;
-  if (p.prod[0].tiles % pairs != 0) {
-    const int a = p.prod[0].blocks, b = p.prod[1].blocks;
-    light = pairs - p.prod[0].tiles % pairs;
-    p.extra = (2 * a + b) / (2 * b);  // a / b, rounded
-    p.light_first = p.extra * b < a;
-  }
-  // Tiles of product 1 beyond whole rounds of pairs: a round of tiles as they are, or rounds of smaller ones. Relative costs of a
-  // step (512 or 256 rows x 256 columns, 256 x 128), by the bytes an SM stages: 48, 32 and 24 KB.
-  const int early = std::min(light * p.extra, p.prod[1].tiles), rest = (p.prod[1].tiles - early) % pairs;
-  const int64_t uncut = HALVES == 2 ? 48 : 32, half = ceil_div(HALVES * rest, pairs) * 32, quarter = ceil_div(2 * HALVES * rest, pairs) * 24;
-  p.cut_cols = kTileI;
-  p.whole = p.prod[1].tiles;
-  if (rest != 0 && std::min(half, quarter) < uncut) {
-    p.whole -= rest;
-    p.cut_cols = half <= quarter ? kTileI : kTileI / 2;
-  }
+  pairs = plan_pairs<HALVES>(p.prod[0].extent, p.prod[1].extent, pairs, &p.plan);
   if (status_word(device, &p.status) != 0) return -1;
-  const int per_cut = HALVES * kTileI / p.cut_cols;
-  const int64_t tiles = static_cast<int64_t>(p.prod[0].tiles) + p.whole + static_cast<int64_t>(p.prod[1].tiles - p.whole) * per_cut;
-  pairs = static_cast<int>(std::min<int64_t>(pairs, tiles));
   return launch_dependent_cluster("linear_pair", linear_pair_kernel<HALVES, BF16>, 2, dim3(2 * static_cast<unsigned>(pairs)), dim3(kThreads), kSmemBytes,
                                   stream, p);
 }
