@@ -39,3 +39,18 @@ def test_slopes_far_out_and_at_infinity(dtype, act, cols):
         dx = run(cabi.linear_backward, dy.cuda(), torch.zeros(3, cols, dtype=dtype, device="cuda"), w.cuda(), z.cuda(), activation=act,
                  need=(True, False, False))[0]
         assert torch.isnan(dx[2]).all() and torch.isfinite(dx[:2]).all()
+
+
+def test_the_longest_sum():
+    """The weight gradient of 2^31 - 1024 rows (34 GB each of x and dy): one cluster's work, and more of it than its other waits
+    are allowed to last. Rows are zero but for some at the beginning, around 2^30 and at the end, whose products are exact."""
+    m, k, n = 2 ** 31 - 1024, 8, 8
+    x, dy = (torch.zeros(m, c, dtype=torch.bfloat16, device="cuda") for c in (k, n))
+    want = torch.zeros(n, k, dtype=torch.float64)
+    for seed, first in enumerate((0, 2 ** 30 - 40, m - 77)):
+        a, b = (torch.randint(-4, 5, (77, c), generator=D.gen(2 * seed + i)).float() for i, c in enumerate((k, n)))
+        x[first:first + 77], dy[first:first + 77] = a.to(torch.bfloat16).cuda(), b.to(torch.bfloat16).cuda()
+        want += b.double().t() @ a.double()
+    w = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda")
+    dw = run(cabi.linear_backward, dy, x, w, need=(False, True, False))[1]
+    assert torch.equal(dw.cpu(), want.to(torch.bfloat16))  # (whole numbers below 2^24, rounded once)

@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_pair_kernel(const __grid_c
       const PairProduct& d = p.prod[t.product];
       for (int h = 0; h < t.halves; h++) {
         const int b = t.halves == 2 ? h : turn;
-        ok = ptx::mbar_wait(tfull0 + 8 * b, (b ? used1 : used0) & 1u, abort_flag);
+        ok = ptx::mbar_wait(tfull0 + 8 * b, (b ? used1 : used0) & 1u, abort_flag, ptx::kWaitLimitCycles + d.extent.blocks * 4096ll);
         if (b) used1++;
         else used0++;
         if (!ok) break;

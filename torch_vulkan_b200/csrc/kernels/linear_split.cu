@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(kThreads, SplitCfg<TN>::kCtasPerSm) linear_spl
     __syncwarp();
   } else {
     const bool empty = kb1 == kb0;  // no values of r here: sums of nothing
-    const bool ok = empty || ptx::mbar_wait(tfull, 0, abort_flag);
+    // (the longest sum, 2^31 values in a cluster of eight, takes 2.6 seconds; a step takes some 500 clocks)
+    const bool ok = empty || ptx::mbar_wait(tfull, 0, abort_flag, ptx::kWaitLimitCycles + static_cast<long long>(kb1 - kb0) * 4096);
     ptx::tc_fence_after();
     const uint32_t dst = base + (warp * 32 + lane) * 4;
     if (ok) {

@@ -76,7 +76,8 @@ constexpr long long kWaitLimitCycles = 4000000000ll;
 
 // Waits for the barrier's phase `parity`; false if the wait ran out or another
 // thread of the CTA already gave up (`*abort` != 0). Sets *abort on running out.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+// `limit`: a wait for a whole tile's sums may be longer, by as much as they have steps.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort, long long limit = kWaitLimitCycles) {
   if (mbar_try_wait(bar, parity)) return true;
   long long start = clock64();
   for (;;) {
@@ -84,7 +85,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     for (int i = 0; i < 64; i++)
       if (mbar_try_wait(bar, parity)) return true;
     if (*abort != 0) return false;
-    if (clock64() - start > kWaitLimitCycles) {
+    if (clock64() - start > limit) {
       *abort = 1;
       return false;
     }
