@@ -476,8 +476,10 @@ TVB_API int tvb_linear(int device, const void* x, int dtype, int64_t x_sm, const
  * [m, n]; may be NULL without an activation):
  *   dz = dy * act'(preact)   dx[m, k] = dz @ w   dw[n, k] = dz^T @ x   db[n] = sum of dz over the rows
  * (the residual's gradient is dy itself). dx, dw and db are contiguous, of `dtype`, and any of them may be NULL. relu's
- * derivative at 0 is 0; an infinite preact (a float16 one beyond 65504) takes the derivative's limit, 0 or 1. dz is rounded to dtype once on its way into the two products; db sums the unrounded values in
- * float32, in a fixed order. Workspace as above; `want`: the TVB_WANT_* of the outputs that are not NULL. */
+ * derivative at 0 is 0; an infinite preact (a float16 one beyond 65504) takes the derivative's limit, 0 or 1. dz is rounded to
+ * dtype once on its way into the two products: in float16 a dz of less than 3e-8 is 0 there and one beyond 65504 infinite, so
+ * gradients of that type are scaled by the caller, as float16 training does anyway. db sums the unrounded values in float32,
+ * in a fixed order. Workspace as above; `want`: the TVB_WANT_* of the outputs that are not NULL. */
 enum TvbWant { TVB_WANT_DX = 1, TVB_WANT_DW = 2, TVB_WANT_DB = 4 };
 TVB_API uint64_t tvb_linear_backward_workspace_bytes(int dtype, const void* dy, int64_t dy_sm, const void* x, int64_t x_sm, const void* w,
                                                      int64_t w_sn, int activation, int want, int64_t m, int64_t n, int64_t k);

@@ -10,9 +10,11 @@ csrc/aten) and names it "vk", exactly as the reference's package does
 (python/torch_vulkan/__init__.py:29-33), so code written for torch_vulkan's
 `_weight_int8pack_mm`, `_dyn_quant_pack_4bit_weight`, `_dyn_quant_matmul_4bit` and
 `_scaled_mm` runs unchanged. The kernels are hand-written CUDA for sm_100a behind the
-C ABI of include/tvb200.h. Nothing else of PyTorch is implemented on this device and
-nothing ever runs on the CPU instead: an op without a kernel raises NotImplementedError
-(the reference's TORCH_VK_STRICT behaviour is the only mode).
+C ABI of include/tvb200.h. Beside them stand the layers that a model keeps in 16 or 32
+bits (mm / addmm, layer norm and its gradients, the fused Linear of the `linear` module)
+and the copies, casts and additions around them. Nothing else of PyTorch is implemented
+on this device and nothing ever runs on the CPU instead: an op without a kernel raises
+NotImplementedError (the reference's TORCH_VK_STRICT behaviour is the only mode).
 
 The public functions mirror python/torch_vulkan/__init__.py:54-148.
 """

@@ -373,7 +373,8 @@ def scaled_mm(a, b, scale_a, scale_b, bias=None, scale_result=None, out_dtype=No
 
 
 # ---- the fused Linear layer and layer norm. "vk" tensors: queued on the backend's stream, like every op of the device.
-# torch.cuda tensors: queued on torch's current stream, allocations included, like any CUDA op (and capturable with it).
+# torch.cuda tensors: queued on torch's current stream, allocations included, like any CUDA op (and capturable with it). A wait in a
+# kernel that runs out is reported by the next synchronize() of this module, of either kind of tensors.
 
 def _activation(fn, activation):
     code = ACTIVATIONS.get(activation)

@@ -584,8 +584,9 @@ constexpr int kRingCluster = 2;
 // gridDim.x) lies in slot i % stages; the slot of row i - 1 is refilled behind the barrier inside row i's sums, which every thread
 // reaches only after it is done with row i - 1. A row is read from shared memory twice (for the sums, for dx), which leaves the
 // registers to the column sums and, where they are 16-bit, the weights; others (WIDE: float32) lie in shared memory.
-// With 16-bit rows the instructions are what bounds it (two thirds of the issue slots; they were twice as many with the
-// number of threads a variable, most of them addresses).
+// 8192 x 8192 bfloat16: 84 us, 4.8 TB/s, with 53 % of the issue slots used: neither memory nor instructions are at their limit; what is
+// left is the block-wide sum per row, which one CTA per SM cannot hide behind another's. (The instructions were twice as many
+// with the number of threads a variable, most of them addresses.)
 // Dynamic shared memory: the ring, the weights (WIDE), two buffers for the sums over the warps.
 template <int DT, int T, int UNITS, bool WIDE>
 __global__ void __launch_bounds__(T, 512 / T) layer_norm_backward_ring_kernel(const NormParams p, const int stages, int* status) {

@@ -6,7 +6,8 @@
 // Float32 results take the library's functions, one value at a time. Results that are rounded to 16 bits take the forms on pairs
 // below: the epilogue of a product has 64 clocks per output of a tile with 1024 values of r, and what it costs is instructions, so
 // they work on two values at once wherever the hardware can, and take the exponential and the reciprocal from its
-// approximations (a few units of 2^-22 off, 2^-11 of the rounding of a float16 that follows).
+// approximations. Those are a few units of 2^-22 off, relative, and the exponent that goes in is itself rounded, which adds its size
+// times 2^-24: 2^-18 for silu(-40), near 2^-17 at the far end of the tails. Half a step of the float16 that follows is 2^-11.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -106,8 +107,8 @@ __device__ __forceinline__ uint64_t within_pair(uint64_t z, float most) {
 }
 
 // Phi(-a) for a >= 0; *density receives exp(-a^2 / 2). With t = 1 / (1 + 0.36 a), Phi(-a) = exp(-a^2 / 2) t P(t), P of degree 6,
-// fitted by weighted least squares to erfcx for the least relative error (6.3e-7 for a <= 12): about half of the instructions
-// of 1 + erf, accurate in the tail where that sum cancels, and the exponential is the one that the derivative needs as well.
+// fitted by weighted least squares to erfcx for the least relative error (6.3e-7 for a <= 12 in exact arithmetic, 9.2e-7 with
+// float32's roundings, to which the exponential adds its own): about half of the instructions of 1 + erf, accurate in the tail where that sum cancels, and the exponential is the one that the derivative needs as well.
 __device__ __forceinline__ uint64_t tail_pair(uint64_t a, uint64_t* density) {
   const uint64_t e = exp2_pair(ptx::mul_f32x2(ptx::mul_f32x2(a, a), two(-0.5f * kLog2e)));
   const uint64_t t = rcp_pair(ptx::fma_f32x2(a, two(0.36f), two(1.0f)));
